@@ -23,6 +23,8 @@ SYMBOLS = [
     "mi355_local_bandwidth", "mi355_host_alloc", "mi355_host_free", "mi355_copy_async",
     "mi355_fill_f16", "mi355_fill_fp8_e5m2", "mi355_fill_i8", "mi355_gemm_f16", "mi355_gemm_i8", "mi355_gemm_fp8_e5m2",
     "mi355_gemm_f32", "mi355_gemm_f64", "mi355_fill_f64",
+    "mi355_open_on_stream", "mi355_glu_forward", "mi355_glu_backward_workspace", "mi355_glu_backward", "mi355_quantize_i8",
+    "mi355_gemm_i8_scaled_workspace", "mi355_gemm_i8_scaled", "mi355_glu_i8",
     "mi355_gemm_mxfp4", "mi355_gemm_mxfp4_static", "mi355_fill_bytes",
     "mi355_gemm_mxfp4_prepare_scales", "mi355_gemm_mxfp4_prepared", "mi355_scratch_bytes", "mi355_gemm_tiling",
 ]
@@ -35,6 +37,8 @@ MAD_F32, MAD_F16, MAD_F64, MAD_MP, MAD_BF16, MAD_I32, MAD_I8DP = range(7)
  MFMA_FP8_16x16x128, MFMA_BF8_16x16x128, MFMA_MXFP6_E2M3, MFMA_MXFP6_E3M2, MFMA_MXFP4_E2M1) = range(10)
 SMFMAC_F16_16x16x64, SMFMAC_BF16_16x16x64, SMFMAC_FP8_16x16x128, SMFMAC_BF8_16x16x128, SMFMAC_I8_16x16x128 = range(5)
 GEMM_TILING_AUTO, GEMM_TILING_256, GEMM_TILING_128 = 0, 1, 2
+TYPE_BF16, TYPE_F16, TYPE_F32 = 0, 1, 2
+GLU_SILU, GLU_GELU, GLU_GELU_TANH, GLU_RELU = range(4)
 MATRIX_ON_HALF_THE_CUS = 0x200   # diagnosis: only the workgroups of the first 16 CUs of every XCD take part
 MFMA_ONE_OPERAND_SET = 0x100   # OR into an MFMA / SMFMAC kind: every chain of a wave takes chain 0's operands
 
@@ -106,6 +110,15 @@ def load_library(path=LIB_PATH):
     lib.mi355_gemm_mxfp4_prepared.argtypes = [vp, vp, vp, vp, vp, u32, u32, u32]
     lib.mi355_scratch_bytes.argtypes = [vp, C.POINTER(C.c_size_t)]
     lib.mi355_fill_bytes.argtypes = [vp, vp, u64, u64, u32, u32, u32]
+    sz = C.c_size_t
+    lib.mi355_open_on_stream.argtypes = [C.c_int, vp, C.POINTER(vp)]
+    lib.mi355_glu_forward.argtypes = [vp, i32, i32, vp, u64, vp, vp, u64, vp, u64, vp, vp, u64, u32, u32, u32]
+    lib.mi355_glu_backward_workspace.argtypes = [vp, u32, u32, u32, C.POINTER(sz)]
+    lib.mi355_glu_backward.argtypes = [vp, i32, i32, vp, u64, vp, u64, vp, vp, u64, vp, vp, u64, vp, u64, vp, vp, u64, u32, u32, u32, vp, sz]
+    lib.mi355_quantize_i8.argtypes = [vp, i32, vp, u64, vp, u64, vp, u32, u32, u32]
+    lib.mi355_gemm_i8_scaled_workspace.argtypes = [vp, u32, u32, u32, C.POINTER(sz)]
+    lib.mi355_gemm_i8_scaled.argtypes = [vp, vp, u64, vp, u64, vp, vp, vp, i32, vp, u64, u32, u32, u32, vp, sz]
+    lib.mi355_glu_i8.argtypes = [vp, i32, vp, u64, vp, vp, u64, vp, vp, vp, i32, vp, u64, u32, u32, u32]
     lib.mi355_host_alloc.argtypes = [vp, C.c_size_t, C.POINTER(vp)]
     lib.mi355_host_free.argtypes = [vp, vp]
     lib.mi355_copy_async.argtypes = [vp, vp, vp, C.c_size_t, i32]
@@ -113,6 +126,14 @@ def load_library(path=LIB_PATH):
         if name != "mi355_last_error":
             getattr(lib, name).restype = C.c_int
     return lib
+
+
+def _ptr(buf):
+    """The device address of a DeviceBuffer, of anything else that has data_ptr() (a torch tensor), or a plain address;
+    None stays None."""
+    if buf is None or isinstance(buf, int):
+        return buf
+    return buf.data_ptr() if hasattr(buf, "data_ptr") else buf.ptr
 
 
 class DeviceBuffer:
@@ -150,10 +171,12 @@ class DeviceBuffer:
 class Device:
     """One opened GPU: thin, one-to-one wrappers over the C entry points."""
 
-    def __init__(self, ordinal=0, lib=None):
+    def __init__(self, ordinal=0, lib=None, stream=None):
+        """stream: a HIP stream of the caller's as an integer (torch.cuda.current_stream().cuda_stream; 0 is the
+        default stream), which the handle enqueues on instead of one of its own."""
         self.lib = lib or load_library()
         h = C.c_void_p()
-        rc = self.lib.mi355_open(ordinal, C.byref(h))
+        rc = self.lib.mi355_open(ordinal, C.byref(h)) if stream is None else self.lib.mi355_open_on_stream(ordinal, stream, C.byref(h))
         if rc != OK:
             raise Mi355Error(rc, (self.lib.mi355_last_error(None) or b"").decode())
         self.h = h
@@ -319,3 +342,34 @@ class Device:
 
     def gemm_fp8_e4m3(self, A, B, Cbuf, M, N, K, scale_a, scale_b):
         self._check(self.lib.mi355_gemm_fp8_e4m3(self.h, A.ptr, B.ptr, Cbuf.ptr, M, N, K, scale_a, scale_b))
+
+    # --- feed-forward operators: buffers are DeviceBuffers, torch tensors or addresses; strides in elements ---------------
+    def glu_forward(self, type, act, X, ldx, Wg, Wu, ldw, H, ldh, G, U, ldg, T, F, D):
+        self._check(self.lib.mi355_glu_forward(self.h, type, act, _ptr(X), ldx, _ptr(Wg), _ptr(Wu), ldw, _ptr(H), ldh, _ptr(G), _ptr(U), ldg,
+                                               T, F, D))
+
+    def glu_backward_workspace(self, T, F, D):
+        n = C.c_size_t()
+        self._check(self.lib.mi355_glu_backward_workspace(self.h, T, F, D, C.byref(n)))
+        return n.value
+
+    def glu_backward(self, type, act, dH, lddh, X, ldx, Wg, Wu, ldw, G, U, ldg, dX, lddx, dWg, dWu, lddw, T, F, D, workspace,
+                     workspace_bytes):
+        self._check(self.lib.mi355_glu_backward(self.h, type, act, _ptr(dH), lddh, _ptr(X), ldx, _ptr(Wg), _ptr(Wu), ldw, _ptr(G), _ptr(U), ldg,
+                                                _ptr(dX), lddx, _ptr(dWg), _ptr(dWu), lddw, T, F, D, _ptr(workspace), workspace_bytes))
+
+    def quantize_i8(self, type, X, ldx, Q, ldq, scale, M, K, k_pad):
+        self._check(self.lib.mi355_quantize_i8(self.h, type, _ptr(X), ldx, _ptr(Q), ldq, _ptr(scale), M, K, k_pad))
+
+    def gemm_i8_scaled_workspace(self, M, N, K):
+        n = C.c_size_t()
+        self._check(self.lib.mi355_gemm_i8_scaled_workspace(self.h, M, N, K, C.byref(n)))
+        return n.value
+
+    def gemm_i8_scaled(self, A, lda, B, ldb, scale_a, scale_b, bias, type, Cbuf, ldc, M, N, K, workspace=None, workspace_bytes=0):
+        self._check(self.lib.mi355_gemm_i8_scaled(self.h, _ptr(A), lda, _ptr(B), ldb, _ptr(scale_a), _ptr(scale_b), _ptr(bias), type,
+                                                  _ptr(Cbuf), ldc, M, N, K, _ptr(workspace), workspace_bytes))
+
+    def glu_i8(self, act, A, lda, Bg, Bu, ldb, scale_a, scale_g, scale_u, type, H, ldh, M, F, K):
+        self._check(self.lib.mi355_glu_i8(self.h, act, _ptr(A), lda, _ptr(Bg), _ptr(Bu), ldb, _ptr(scale_a), _ptr(scale_g), _ptr(scale_u),
+                                          type, _ptr(H), ldh, M, F, K))

@@ -35,7 +35,8 @@ extern "C" int mi355_device_count(int *count) {
   return MI355_OK;
 }
 
-extern "C" int mi355_open(int ordinal, mi355_dev **out) {
+// `stream`: the caller's, or null for one of the handle's own.
+static int open_device(int ordinal, const hipStream_t *stream, mi355_dev **out) {
   if (!out) return mi355_fail(nullptr, MI355_ERR_ARG, "out is null");
   *out = nullptr;
   int n = 0;
@@ -73,7 +74,9 @@ extern "C" int mi355_open(int ordinal, mi355_dev **out) {
   d->props.clock_khz = p.clockRate;
   d->props.total_mem = (uint64_t)p.totalGlobalMem;
 
-  if ((e = hipStreamCreateWithFlags(&d->stream, hipStreamNonBlocking)) != hipSuccess ||
+  d->owns_stream = stream == nullptr;
+  if (stream) d->stream = *stream;
+  if ((d->owns_stream && (e = hipStreamCreateWithFlags(&d->stream, hipStreamNonBlocking)) != hipSuccess) ||
       (e = hipEventCreate(&d->ev_start)) != hipSuccess ||
       (e = hipEventCreate(&d->ev_stop)) != hipSuccess) {
     int code = mi355_fail(nullptr, MI355_ERR_HIP, "stream/event creation: %s", hipGetErrorString(e));
@@ -90,14 +93,28 @@ extern "C" int mi355_open(int ordinal, mi355_dev **out) {
   return MI355_OK;
 }
 
+extern "C" int mi355_open(int ordinal, mi355_dev **out) { return open_device(ordinal, nullptr, out); }
+
+extern "C" int mi355_open_on_stream(int ordinal, void *stream, mi355_dev **out) {
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (s) {   // (null is the default stream of whichever device is current)
+    hipDevice_t on = -1;
+    const hipError_t e = hipStreamGetDevice(s, &on);
+    if (e != hipSuccess) return mi355_fail(nullptr, MI355_ERR_HIP, "hipStreamGetDevice: %s", hipGetErrorString(e));
+    if (on != ordinal) return mi355_fail(nullptr, MI355_ERR_ARG, "the stream belongs to device %d, not to %d", (int)on, ordinal);
+  }
+  return open_device(ordinal, &s, out);
+}
+
 extern "C" int mi355_close(mi355_dev *dev) {
   if (!dev) return MI355_OK;
   (void)hipSetDevice(dev->ordinal);
-  if (dev->stream) (void)hipStreamSynchronize(dev->stream);
+  // (a borrowed stream may be gone already: only the release of scratch memory below waits, for the whole device)
+  if (dev->owns_stream && dev->stream) (void)hipStreamSynchronize(dev->stream);
   if (dev->mx_scratch) (void)hipFree(dev->mx_scratch);
   if (dev->ev_start) (void)hipEventDestroy(dev->ev_start);
   if (dev->ev_stop) (void)hipEventDestroy(dev->ev_stop);
-  if (dev->stream) (void)hipStreamDestroy(dev->stream);
+  if (dev->owns_stream && dev->stream) (void)hipStreamDestroy(dev->stream);
   delete dev;
   return MI355_OK;
 }

@@ -1,0 +1,188 @@
+// The gradients of the gated projection.  dG and dU are one elementwise pass; what follows are products whose operands
+// have the sum's index on the outside (dX sums over F, the rows of the weights; dW over T, the rows of X and of dG, dU),
+// while the product kernels want it innermost.  So the pass that makes dG and dU writes them both ways, and X and the
+// weights are turned once into the workspace: per product of 2 T F D operations a few bytes of T F + F D + T D, some
+// percent of the products' time at the sizes of a training batch.  Rows of the turned copies are padded with zeros to
+// the product kernels' 128 bytes, which is what lets T and F be anything.
+#include "ffn.h"
+
+namespace {
+
+constexpr int kTileEdge = 64, kThreads = 256, kVec = 8;
+
+__host__ __device__ constexpr uint64_t round_up(uint64_t x, uint64_t to) { return (x + to - 1) / to * to; }
+
+// The workspace: dG | dU by rows [T][2 Fk], by columns 2 x [Fp][Tp], the weights turned [D][2 Fk], X turned [D][Tp].
+struct Plan {
+  uint64_t fk, fp, tp;                      // F padded to a row of a product, F padded to whole tiles, T padded to a row
+  uint64_t rows, cols, wt, xt, bytes;       // offsets
+};
+Plan plan_of(uint32_t T, uint32_t F, uint32_t D) {
+  Plan p;
+  p.fk = round_up(F, 64);
+  p.fp = round_up(F, 256);
+  p.tp = T ? round_up(T, 64) : 64;
+  p.rows = 0;
+  p.cols = round_up(p.rows + (uint64_t)T * 2 * p.fk * 2, 256);
+  p.wt = round_up(p.cols + 2 * p.fp * p.tp * 2, 256);
+  p.xt = round_up(p.wt + (uint64_t)D * 2 * p.fk * 2, 256);
+  p.bytes = round_up(p.xt + (uint64_t)D * p.tp * 2, 256);
+  return p;
+}
+
+// A 64x64 tile of 16-bit values in LDS, written by rows and read by columns.
+struct Tile {
+  uint16_t at[kTileEdge][kTileEdge + 2];
+};
+
+struct Vec8 {
+  uint16_t v[kVec];
+};
+// 8 values of a row from an address that is element-aligned only; past the end of the row: 0.
+__device__ __forceinline__ Vec8 load8(const uint16_t *row, uint32_t at, uint32_t n) {
+  Vec8 x;
+  if (at + kVec <= n) {
+    __builtin_memcpy(&x, row + at, sizeof(x));
+  } else {
+#pragma unroll
+    for (int e = 0; e < kVec; e++) x.v[e] = at + e < n ? row[at + e] : 0;
+  }
+  return x;
+}
+template <int TYPE>
+__device__ __forceinline__ float widen(uint16_t h) {
+  if constexpr (TYPE == MI355_TYPE_F16) return (float)__builtin_bit_cast(_Float16, h);
+  else return __builtin_bit_cast(float, (uint32_t)h << 16);
+}
+template <int TYPE>
+__device__ __forceinline__ uint16_t narrow(float x) {
+  return (uint16_t)(TYPE == MI355_TYPE_F16 ? mi355_pack_f16x2(x, 0.0f) : mi355_pack_bf16x2(x, 0.0f));
+}
+
+// Column c of the tile (8 of its values from row r on) to 16 bytes of dst.
+__device__ __forceinline__ void store_column(const Tile &t, uint32_t c, uint32_t r, uint16_t *dst) {
+  Vec8 x;
+#pragma unroll
+  for (int e = 0; e < kVec; e++) x.v[e] = t.at[r + e][c];
+  *reinterpret_cast<uint4 *>(dst) = __builtin_bit_cast(uint4, x);
+}
+
+// dG and dU of a 64x64 tile: by rows (dG at column f, dU at column fk + f of a row of 2 fk; zeros from F to fk) and by
+// columns (row f of [fp][tp], dU fp rows on; zeros from T to tp).
+template <int TYPE>
+__global__ void __launch_bounds__(kThreads)
+glu_gate_grad_kernel(const uint16_t *dH, uint64_t lddh, const uint16_t *G, const uint16_t *U, uint64_t ldg, uint16_t *rows, uint16_t *cols,
+                     uint32_t T, uint32_t F, uint32_t fk, uint64_t fp, uint32_t tp, int act, uint32_t tiles_f) {
+  __shared__ Tile tg, tu;
+  const uint32_t f0 = blockIdx.x % tiles_f * kTileEdge, t0 = blockIdx.x / tiles_f * kTileEdge;
+  const uint32_t c = threadIdx.x % 8u * kVec, r0 = threadIdx.x / 8u;
+#pragma unroll
+  for (uint32_t r = r0; r < kTileEdge; r += kThreads / 8) {
+    const uint32_t t = t0 + r, f = f0 + c;
+    Vec8 dg{}, du{};
+    if (t < T) {
+      const Vec8 h = load8(dH + (uint64_t)t * lddh, f, F), g = load8(G + (uint64_t)t * ldg, f, F), u = load8(U + (uint64_t)t * ldg, f, F);
+#pragma unroll
+      for (int e = 0; e < kVec; e++) {
+        float a, da;
+        ffn_act_grad(act, widen<TYPE>(g.v[e]), a, da);
+        const float d = widen<TYPE>(h.v[e]);
+        dg.v[e] = narrow<TYPE>(d * widen<TYPE>(u.v[e]) * da);   // (past F: 0 * 0)
+        du.v[e] = narrow<TYPE>(d * a);
+      }
+      uint16_t *to = rows + (uint64_t)t * 2u * fk + f;
+      *reinterpret_cast<uint4 *>(to) = __builtin_bit_cast(uint4, dg);
+      *reinterpret_cast<uint4 *>(to + fk) = __builtin_bit_cast(uint4, du);
+    }
+#pragma unroll
+    for (int e = 0; e < kVec; e++) {
+      tg.at[r][c + e] = dg.v[e];
+      tu.at[r][c + e] = du.v[e];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (uint32_t r = r0; r < kTileEdge; r += kThreads / 8) {   // r: a column of the tile, c: 8 of its rows
+    if (f0 + r < F) {
+      uint16_t *to = cols + (uint64_t)(f0 + r) * tp + t0 + c;
+      store_column(tg, r, c, to);
+      store_column(tu, r, c, to + fp * tp);
+    }
+  }
+}
+
+// dst[c][r] = src[r][c], rows of dst padded with zeros from R to rp.  C and rp are multiples of 64; src rows on 16 bytes.
+__global__ void __launch_bounds__(kThreads) turn_kernel(const uint16_t *src, uint64_t ld, uint16_t *dst, uint64_t ld_dst, uint32_t R, uint32_t tiles_c) {
+  __shared__ Tile tile;
+  const uint32_t c0 = blockIdx.x % tiles_c * kTileEdge, r0 = blockIdx.x / tiles_c * kTileEdge;
+  const uint32_t c = threadIdx.x % 8u * kVec;
+#pragma unroll
+  for (uint32_t r = threadIdx.x / 8u; r < kTileEdge; r += kThreads / 8) {
+    Vec8 x{};
+    if (r0 + r < R) x = __builtin_bit_cast(Vec8, *reinterpret_cast<const uint4 *>(src + (uint64_t)(r0 + r) * ld + c0 + c));
+#pragma unroll
+    for (int e = 0; e < kVec; e++) tile.at[r][c + e] = x.v[e];
+  }
+  __syncthreads();
+#pragma unroll
+  for (uint32_t r = threadIdx.x / 8u; r < kTileEdge; r += kThreads / 8) store_column(tile, r, c, dst + (uint64_t)(c0 + r) * ld_dst + r0 + c);
+}
+
+int turn(mi355_dev *dev, const void *src, uint64_t ld, uint8_t *dst, uint64_t ld_dst, uint32_t R, uint64_t rp, uint32_t C) {
+  const uint64_t tiles = (uint64_t)(C / 64u) * (rp / 64u);
+  MI355_REQUIRE(dev, tiles <= 0x7fffffffull, "glu_backward: %u x %u values are more than one launch takes", R, C);
+  turn_kernel<<<(uint32_t)tiles, kThreads, 0, dev->stream>>>((const uint16_t *)src, ld, (uint16_t *)dst, ld_dst, R, C / 64u);
+  MI355_LAUNCH_CHECK(dev, "glu_backward (turn)");
+  return MI355_OK;
+}
+
+}  // namespace
+
+int mi355_glu_backward_limits(mi355_dev *dev, const char *what, uint32_t T, uint32_t F) {
+  // T and 2 F are depths of products here: their rows are held to 64 MiB too
+  MI355_REQUIRE(dev, T <= (32u << 20) && F <= (16u << 20) - 64u, "%s: T = %u, F = %u: at most 2^25 and 2^24 - 64 are taken", what, T, F);
+  return MI355_OK;
+}
+
+size_t mi355_glu_backward_bytes(uint32_t T, uint32_t F, uint32_t D) { return (size_t)plan_of(T, F, D).bytes; }
+
+int mi355_launch_glu_backward(mi355_dev *dev, int type, int act, const void *dH, uint64_t lddh, const void *X, uint64_t ldx, const void *Wg,
+                              const void *Wu, uint64_t ldw, const void *G, const void *U, uint64_t ldg, void *dX, uint64_t lddx, void *dWg,
+                              void *dWu, uint64_t lddw, uint32_t T, uint32_t F, uint32_t D, uint8_t *ws) {
+  const Plan p = plan_of(T, F, D);
+  const int op = type == MI355_TYPE_BF16 ? kQuadBf16 : kQuadF16;
+  const uint64_t tiles = p.fk / 64u * (p.tp / 64u);
+  MI355_REQUIRE(dev, tiles <= 0x7fffffffull, "glu_backward: %u x %u values are more than one launch takes", T, F);
+  auto *rows = (uint16_t *)(ws + p.rows), *cols = (uint16_t *)(ws + p.cols);
+#define GO(TYPE)                                                                                                             \
+  glu_gate_grad_kernel<TYPE><<<(uint32_t)tiles, kThreads, 0, dev->stream>>>((const uint16_t *)dH, lddh, (const uint16_t *)G,   \
+      (const uint16_t *)U, ldg, rows, cols, T, F, (uint32_t)p.fk, p.fp, (uint32_t)p.tp, act, (uint32_t)(p.fk / 64u))
+  if (type == MI355_TYPE_BF16) GO(MI355_TYPE_BF16);
+  else GO(MI355_TYPE_F16);
+#undef GO
+  MI355_LAUNCH_CHECK(dev, "glu_backward (gate)");
+  FfnProduct q{};
+  q.out.type = type;
+  if (dX) {
+    if (int rc = turn(dev, Wg, ldw, ws + p.wt, 2 * p.fk, F, p.fk, D)) return rc;
+    if (int rc = turn(dev, Wu, ldw, ws + p.wt + p.fk * 2, 2 * p.fk, F, p.fk, D)) return rc;
+    q.a = ws + p.rows; q.lda = 4 * p.fk;
+    q.b = ws + p.wt; q.ldb = 4 * p.fk;
+    q.m = T; q.n = D; q.k_bytes = (uint32_t)(4 * p.fk);
+    q.out.c = dX; q.out.ldc = lddx;
+    if (int rc = mi355_ffn_product(dev, op, kEpiPlain, "glu_backward (dX)", q)) return rc;
+  }
+  if (dWg) {
+    if (int rc = turn(dev, X, ldx, ws + p.xt, p.tp, T, p.tp, D)) return rc;
+    q.lda = q.ldb = 2 * p.tp;
+    q.b = ws + p.xt;
+    q.m = F; q.n = D; q.k_bytes = (uint32_t)(2 * p.tp);
+    q.out.ldc = lddw;
+    for (int half = 0; half < 2; half++) {
+      q.a = ws + p.cols + half * p.fp * p.tp * 2;
+      q.out.c = half ? dWu : dWg;
+      if (int rc = mi355_ffn_product(dev, op, kEpiPlain, "glu_backward (dW)", q)) return rc;
+    }
+  }
+  return MI355_OK;
+}

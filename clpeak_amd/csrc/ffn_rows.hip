@@ -1,0 +1,138 @@
+// Products of few rows (generated tokens, one or some of each stream): every weight is read once and used for a handful
+// of rows, so the time is that of reading the weights.
+//
+// A workgroup of eight waves owns 16 rows of B (gated: 16 of the gate's and the same 16 of the other projection's) and
+// 16 MT rows of A, over the whole of K.  K is cut into windows of 128 bytes, which the waves take in turn: a wave reads
+// its window's fragments straight from memory into registers (nothing is shared between the waves, so LDS would only
+// add a trip), the workgroup's eight windows are 1 KiB of every row, and the waves' sums meet in LDS at the end, added
+// in the order of the waves: results do not depend on timing.  No sum is split over workgroups: N = 4096 rows are 256
+// workgroups, one for each CU.
+#include "ffn.h"
+
+namespace {
+
+constexpr int kRowWaves = 8, kRowThreads = 64 * kRowWaves;
+
+template <int OP>
+__device__ __forceinline__ i32x4v rows_mfma(const i32x4v &b, const i32x4v &a, const i32x4v &c) {
+  // the product is issued transposed (B first): a lane then holds 4 consecutive columns of one row
+  if constexpr (OP == kQuadI8) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(b, a, c, 0, 0, 0);
+  } else if constexpr (OP == kQuadBf16) {
+    return __builtin_bit_cast(i32x4v, __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8v, b), __builtin_bit_cast(bf16x8v, a),
+                                                                           __builtin_bit_cast(f32x4v, c), 0, 0, 0));
+  } else {
+    return __builtin_bit_cast(i32x4v, __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8v, b), __builtin_bit_cast(half8v, a),
+                                                                          __builtin_bit_cast(f32x4v, c), 0, 0, 0));
+  }
+}
+
+// One window: the fragments of both K halves (16 bytes at 16 * (lane / 16), and 64 bytes on).
+template <int OP, int MT, int NB>
+struct RowWindow {
+  i32x4v a[MT][2], b[NB][2];
+  __device__ __forceinline__ void load(const uint8_t *const (&pa)[MT], const uint8_t *const (&pb)[NB], uint64_t at) {
+#pragma unroll
+    for (int j = 0; j < NB; j++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) b[j][h] = *reinterpret_cast<const i32x4v *>(pb[j] + at + 64 * h);
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) a[i][h] = *reinterpret_cast<const i32x4v *>(pa[i] + at + 64 * h);
+  }
+  __device__ __forceinline__ void multiply(i32x4v (&acc)[MT][NB]) const {
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int j = 0; j < NB; j++) acc[i][j] = rows_mfma<OP>(b[j][h], a[i][h], acc[i][j]);
+  }
+};
+
+template <int OP, int EPI, int MT>
+__global__ void __launch_bounds__(kRowThreads) ffn_rows_kernel(FfnProduct p, uint32_t tiles_n) {
+  constexpr int NB = epi_is_gated(EPI) ? 2 : 1;
+  constexpr int kUnroll = MT == 4 ? 2 : 4;   // 64 KiB in flight per workgroup, what the registers of 8 waves hold
+  __shared__ int32_t sums[kRowWaves][MT][NB][16][16];   // [row][column]
+  const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const uint32_t r = lane % 16, g = lane / 16;
+  const uint32_t tn = blockIdx.x % tiles_n, tm = blockIdx.x / tiles_n;
+  const uint32_t m0 = tm * 16u * MT, n0 = tn * 16u;
+
+  // Rows past the last one are read as the last one; what they give is never stored.
+  const uint8_t *pa[MT], *pb[NB];
+#pragma unroll
+  for (int i = 0; i < MT; i++) pa[i] = p.a + (uint64_t)min(m0 + 16u * i + r, p.m - 1u) * p.lda + 16u * g;
+  const uint64_t b_row = (uint64_t)min(n0 + r, p.n - 1u) * p.ldb + 16u * g;
+  pb[0] = p.b + b_row;
+  if constexpr (NB == 2) pb[1] = p.b2 + b_row;
+
+  i32x4v acc[MT][NB];
+#pragma unroll
+  for (int i = 0; i < MT; i++)
+#pragma unroll
+    for (int j = 0; j < NB; j++) acc[i][j] = (i32x4v){0, 0, 0, 0};
+
+  const uint32_t windows = p.k_bytes / 128u;
+  uint32_t w = wave;
+  for (; w + kRowWaves * (kUnroll - 1) < windows; w += kRowWaves * kUnroll) {
+    RowWindow<OP, MT, NB> win[kUnroll];
+#pragma unroll
+    for (int k = 0; k < kUnroll; k++) win[k].load(pa, pb, (uint64_t)(w + kRowWaves * k) * 128u);
+#pragma unroll
+    for (int k = 0; k < kUnroll; k++) win[k].multiply(acc);
+  }
+  for (; w < windows; w += kRowWaves) {
+    RowWindow<OP, MT, NB> win;
+    win.load(pa, pb, (uint64_t)w * 128u);
+    win.multiply(acc);
+  }
+
+#pragma unroll
+  for (int i = 0; i < MT; i++)
+#pragma unroll
+    for (int j = 0; j < NB; j++) *reinterpret_cast<i32x4v *>(&sums[wave][i][j][r][4 * g]) = acc[i][j];
+  __syncthreads();
+  for (uint32_t e = threadIdx.x; e < MT * 256u; e += kRowThreads) {
+    const uint32_t i = e / 256u, row = e / 16u % 16u, col = e % 16u;
+    int32_t s[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < NB; j++) {
+      if constexpr (OP == kQuadI8) {
+#pragma unroll
+        for (int v = 0; v < kRowWaves; v++) s[j] += sums[v][i][j][row][col];
+      } else {
+        float f = 0.0f;
+#pragma unroll
+        for (int v = 0; v < kRowWaves; v++) f += __builtin_bit_cast(float, sums[v][i][j][row][col]);
+        s[j] = __builtin_bit_cast(int32_t, f);
+      }
+    }
+    if (m0 + 16u * i + row < p.m && n0 + col < p.n) ffn_finish1<EPI>(p.out, m0 + 16u * i + row, n0 + col, s[0], s[1]);
+  }
+}
+
+template <int OP, int EPI, int MT>
+int launch(mi355_dev *dev, const char *what, const FfnProduct &p) {
+  const uint64_t tiles_n = (p.n + 15ull) / 16u, tiles_m = (p.m + 16ull * MT - 1u) / (16u * MT);
+  MI355_REQUIRE(dev, tiles_n * tiles_m <= 0x7fffffffull, "%s: %u x %u outputs are more than one launch takes", what, p.m, p.n);
+  ffn_rows_kernel<OP, EPI, MT><<<(uint32_t)(tiles_n * tiles_m), kRowThreads, 0, dev->stream>>>(p, (uint32_t)tiles_n);
+  MI355_LAUNCH_CHECK(dev, what);
+  return MI355_OK;
+}
+template <int OP, int EPI>
+int launch_by_rows(mi355_dev *dev, const char *what, const FfnProduct &p) {
+  if (p.m <= 16u) return launch<OP, EPI, 1>(dev, what, p);
+  if (p.m <= 32u) return launch<OP, EPI, 2>(dev, what, p);
+  return launch<OP, EPI, 4>(dev, what, p);
+}
+
+}  // namespace
+
+int mi355_launch_ffn_rows(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p) {
+  if (op == kQuadI8) return epi == kEpiScaled ? launch_by_rows<kQuadI8, kEpiScaled>(dev, what, p) : launch_by_rows<kQuadI8, kEpiGatedScaled>(dev, what, p);
+  if (op == kQuadBf16) return epi == kEpiPlain ? launch_by_rows<kQuadBf16, kEpiPlain>(dev, what, p) : launch_by_rows<kQuadBf16, kEpiGated>(dev, what, p);
+  return epi == kEpiPlain ? launch_by_rows<kQuadF16, kEpiPlain>(dev, what, p) : launch_by_rows<kQuadF16, kEpiGated>(dev, what, p);
+}

@@ -196,10 +196,10 @@ constexpr size_t kRingBytes = 5 * (size_t)kSlabBytes;   // five 32 KiB slots: al
 enum { kLdsF32 = 0 /* gemm_quad.h: kLdsQuad0 + the operand kind of gemm_quad_kernel */ };
 template <typename Kernel>
 inline int allow_full_lds(mi355_dev *dev, Kernel kernel, unsigned bit) {
-  if (dev->full_lds_allowed & (1u << bit)) return MI355_OK;
+  if (dev->full_lds_allowed & (1ull << bit)) return MI355_OK;
   MI355_HIP(dev, hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                                      (int)kRingBytes));
-  dev->full_lds_allowed |= 1u << bit;
+  dev->full_lds_allowed |= 1ull << bit;
   return MI355_OK;
 }
 

@@ -9,6 +9,7 @@
 struct mi355_dev {
   int          ordinal   = -1;
   hipStream_t  stream    = nullptr;
+  bool         owns_stream = false;   // false: the stream belongs to the caller of mi355_open_on_stream
   hipEvent_t   ev_start  = nullptr;
   hipEvent_t   ev_stop   = nullptr;
   mi355_props_t props{};
@@ -19,7 +20,7 @@ struct mi355_dev {
   // device address, on this handle's device, of the static array behind mi355_gemm_mxfp4_static (set by mi355_open)
   void        *mx_static_scratch = nullptr;
   // GEMM kernels that have been allowed the whole LDS of a CU on this device (one bit per kernel)
-  uint32_t     full_lds_allowed = 0;
+  uint64_t     full_lds_allowed = 0;
   // which tiling the 4-, 8- and 16-bit GEMM entry points take (MI355_GEMM_TILING_*; set by mi355_gemm_tiling)
   int          gemm_tiling = 0;
 };
@@ -52,6 +53,13 @@ int mi355_mx_resolve_static_scratch(mi355_dev *dev);
   do {                                                                                  \
     if (!(cond)) return mi355_fail((dev), MI355_ERR_ARG, __VA_ARGS__);                  \
   } while (0)
+
+// The two halves of MI355_ENTER below, for entry points that check their arguments before they touch the device.
+#define MI355_HANDLE(dev)                                                               \
+  do {                                                                                  \
+    if (!(dev)) return mi355_fail(nullptr, MI355_ERR_ARG, "null device handle");        \
+  } while (0)
+#define MI355_SET_DEVICE(dev) MI355_HIP((dev), hipSetDevice((dev)->ordinal))
 
 // Every entry point that touches the device starts with this: validates the handle
 // and makes its device current on the calling thread.

@@ -3,7 +3,8 @@
  *
  * This is the only door through which host code reaches HIP.  Everything is
  * plain C: opaque device handle, raw device pointers, sizes, int status codes.
- * No C++ types, no exceptions, no torch types.  One handle owns one HIP stream;
+ * No C++ types, no exceptions, no torch types.  One handle owns one HIP stream
+ * (or, opened by mi355_open_on_stream, borrows one);
  * a handle is not thread-safe, different handles may be used from different
  * threads.  Every `*_launch_*`-style entry point ENQUEUES on the handle's stream
  * and returns without waiting; use mi355_sync() or the timer pair to wait.
@@ -56,6 +57,11 @@ int mi355_device_count(int *count);
 /* src/rocm/rocm_device.cpp:42-85 (RocmDevice::init: hipSetDevice, props,
  * non-blocking stream).  Refuses anything that is not gfx950. */
 int mi355_open(int ordinal, mi355_dev **out);
+/* The same on a stream of the caller's (a hipStream_t of that device; NULL: its default stream), for programs whose
+ * other work on the GPU runs on a stream already: what the handle enqueues is then ordered with it, and can be captured
+ * into a graph where an entry point below says so.  The stream is borrowed: it has to outlive the handle's last call but
+ * mi355_close, which leaves it as it is and does not wait for it.  No counterpart in the reference. */
+int mi355_open_on_stream(int ordinal, void *stream, mi355_dev **out);
 /* src/rocm/rocm_device.cpp:87-98 (RocmDevice::cleanup). */
 int mi355_close(mi355_dev *dev);
 int mi355_get_props(mi355_dev *dev, mi355_props_t *out);
@@ -339,6 +345,69 @@ int mi355_scratch_bytes(mi355_dev *dev, size_t *handle_bytes);
  * (span 256, lo 0: random code pairs; lo 123, span 9: scales 2^-4 .. 2^4). */
 int mi355_fill_bytes(mi355_dev *dev, uint8_t *dst, uint64_t n, uint64_t seed, uint32_t stream,
                      uint32_t lo, uint32_t span);
+
+/* ---- feed-forward operators of a language model ------------------------------- */
+/* No counterpart in the reference, which measures its products bare; these are the products as a model's feed-forward
+ * layer calls them: the gated projection with its gradients in 16 bits, and the same layer with 8-bit integer weights.
+ *
+ * Common rules.  Matrices are row-major, ld* is the distance of two rows in elements of that matrix.  All buffers are
+ * device memory of the handle's GPU; outputs overlap neither each other nor an input.  Operands of the products (X, W*, A,
+ * B) start on 16 bytes, their rows are a multiple of 16 bytes apart, and a row of K is a multiple of 128 bytes (64 16-bit values, 128
+ * int8) and at most 64 MiB; every other matrix needs the alignment of its elements only.  Numbers of rows and columns are
+ * otherwise free.  No rows (T or M zero) is a call that writes nothing (mi355_glu_backward: zero weight gradients);
+ * anything else empty is refused.  Of an output only its rows and columns are written, not what lies between them.
+ * Calls enqueue and return; they allocate nothing, keep nothing from one call to the next and launch kernels only,
+ * so that they can be captured into a graph.  A workspace belongs to a call until that call's work is done: calls
+ * that may overlap (two streams, two graphs) need one each.  Results do not depend on timing: a call repeated gives the
+ * same bits. */
+#define MI355_TYPE_BF16 0
+#define MI355_TYPE_F16  1
+#define MI355_TYPE_F32  2
+#define MI355_GLU_SILU      0   /* x / (1 + exp(-x)) */
+#define MI355_GLU_GELU      1   /* x / 2 (1 + erf(x / sqrt 2)) */
+#define MI355_GLU_GELU_TANH 2   /* x / 2 (1 + tanh(sqrt(2 / pi) (x + 0.044715 x^3))) */
+#define MI355_GLU_RELU      3   /* max(x, 0); its derivative at 0 is 0 */
+
+/* The gated projection in one kernel:  G = X Wg^T,  U = X Wu^T,  H = act(G) * U.   X[T][D], Wg[F][D], Wu[F][D] (both ldw
+ * apart), H[T][F], all of `type` (MI355_TYPE_BF16 or _F16).  Sums, activation and product are fp32, H is rounded once.
+ * G, U: where both sums are kept, rounded to `type`, rows ldg apart, for mi355_glu_backward; both NULL: not kept. */
+int mi355_glu_forward(mi355_dev *dev, int type, int act, const void *X, uint64_t ldx, const void *Wg, const void *Wu, uint64_t ldw,
+                      void *H, uint64_t ldh, void *G, void *U, uint64_t ldg, uint32_t T, uint32_t F, uint32_t D);
+/* Its gradients, from dH[T][F] and the kept G and U:
+ *     dG = dH * U * act'(G),  dU = dH * act(G)      (fp32, rounded to `type` for the products that follow)
+ *     dX[T][D] = dG Wg + dU Wu,   dWg[F][D] = dG^T X,   dWu[F][D] = dU^T X      (fp32 sums, rounded once to `type`)
+ * dX NULL, or dWg and dWu NULL: that part is left out (a frozen weight, a first layer); its operand (Wg and Wu, or X)
+ * may then be NULL too.  `workspace` holds what mi355_glu_backward_workspace says, on 256 bytes.  T up to 2^25, F up to
+ * 2^24 - 64. */
+int mi355_glu_backward_workspace(mi355_dev *dev, uint32_t T, uint32_t F, uint32_t D, size_t *bytes);
+int mi355_glu_backward(mi355_dev *dev, int type, int act, const void *dH, uint64_t lddh, const void *X, uint64_t ldx,
+                       const void *Wg, const void *Wu, uint64_t ldw, const void *G, const void *U, uint64_t ldg,
+                       void *dX, uint64_t lddx, void *dWg, void *dWu, uint64_t lddw, uint32_t T, uint32_t F, uint32_t D,
+                       void *workspace, size_t workspace_bytes);
+
+/* Rows to int8 with a scale each (activations for each token, weights for each channel):
+ *     scale[m] = amax / 127,   Q[m][k] = 127 X[m][k] / amax rounded to the nearest whole number, ties to even,
+ * amax the largest magnitude of row m of X[M][K] (bf16, fp16 or fp32).  The rounding is that of the exact quotient.  A row
+ * of zeros: zeros and scale 0.  A row with an infinity or a NaN: zeros and scale NaN, so that products of it are NaN.
+ * Columns K .. k_pad-1 of Q are written as 0 (k_pad >= K: the multiple of 128 that the products below ask for). */
+int mi355_quantize_i8(mi355_dev *dev, int type, const void *X, uint64_t ldx, int8_t *Q, uint64_t ldq, float *scale,
+                      uint32_t M, uint32_t K, uint32_t k_pad);
+/* The product of such rows:  C[m][n] = scale_a[m] * scale_b[n] * sum_k A[m][k] B[n][k] + bias[n].   A[M][K], B[N][K] int8,
+ * scales and bias fp32 (bias NULL: none), C[M][N] of `type` (MI355_TYPE_*).  The sum is exact (int32; K at most 130944);
+ * the rest is fp32, C is rounded once.
+ * A workspace lets a product of few tiles and a long K be split along K (the sums stay exact); without one (NULL, 0) it
+ * is not split.  mi355_gemm_i8_scaled_workspace: the bytes that M, N, K can use, 0 where the product is not split anyway;
+ * a smaller workspace counts as none.  On 16 bytes. */
+int mi355_gemm_i8_scaled_workspace(mi355_dev *dev, uint32_t M, uint32_t N, uint32_t K, size_t *bytes);
+int mi355_gemm_i8_scaled(mi355_dev *dev, const int8_t *A, uint64_t lda, const int8_t *B, uint64_t ldb, const float *scale_a,
+                         const float *scale_b, const float *bias, int type, void *C, uint64_t ldc, uint32_t M, uint32_t N, uint32_t K,
+                         void *workspace, size_t workspace_bytes);
+/* The gated projection on such rows, in one kernel:
+ *     H[m][f] = act(scale_a[m] * scale_g[f] * (A Bg^T)[m][f]) * (scale_a[m] * scale_u[f] * (A Bu^T)[m][f])
+ * A[M][K], Bg[F][K], Bu[F][K] (both ldb apart) int8, H[M][F] of `type`. */
+int mi355_glu_i8(mi355_dev *dev, int act, const int8_t *A, uint64_t lda, const int8_t *Bg, const int8_t *Bu, uint64_t ldb,
+                 const float *scale_a, const float *scale_g, const float *scale_u, int type, void *H, uint64_t ldh,
+                 uint32_t M, uint32_t F, uint32_t K);
 
 #ifdef __cplusplus
 }
