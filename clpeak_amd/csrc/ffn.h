@@ -12,6 +12,7 @@ enum FfnEpi {
   kEpiScaled = 1,       // int8 operands: C = sum * scale_a[row] * scale_b[col] (+ bias[col])
   kEpiGated = 2,        // 16-bit operands, two products: H = act(gate) * up, the two sums kept where asked for
   kEpiGatedScaled = 3,  // int8 operands, two products, each sum scaled first
+  kEpiPartial = 4,      // the sums of a slice of K, as they are (32 bits each)
 };
 constexpr bool epi_is_gated(int epi) { return epi == kEpiGated || epi == kEpiGatedScaled; }
 
@@ -37,8 +38,19 @@ struct FfnProduct {
 // ffn_rows.hip: any shape; the kernel for few rows.  op: kQuadBf16 / kQuadF16 / kQuadI8.
 int mi355_launch_ffn_rows(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p);
 
-// ffn.hip: the kernel that suits the product.
-int mi355_ffn_product(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p);
+// ffn_quad.hip / ffn_small.hip: on 256x256 and on 128x128 tiles of sums (gated: of 256x128 / 128x64 outputs).
+int mi355_launch_ffn_quad(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p);
+// slices > 1 (one product, not gated): K is cut into so many, `workspace` holds `slices` matrices of m rows of
+// mi355_ffn_slice_row(n) 32-bit sums, on 16 bytes.
+int mi355_launch_ffn_small(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p, uint32_t slices, void *workspace);
+inline uint64_t mi355_ffn_slice_row(uint32_t n) { return (n + 3ull) / 4u * 4u; }
+// Bits of mi355_dev::full_lds_allowed: three operand types with up to three kinds of product each.
+enum { kLdsFfnQuad0 = 24, kLdsFfnSmall0 = 36 };
+constexpr int ffn_kind(int op, int epi) { return (op - kQuadBf16) * 3 + (epi == kEpiPartial ? 2 : epi_is_gated(epi) ? 1 : 0); }
+
+// ffn.hip: the product on the kernel that suits it, and the workspace that it can use.
+int mi355_ffn_product(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p, void *workspace, size_t workspace_bytes);
+size_t mi355_ffn_workspace(const mi355_dev *dev, int epi, uint32_t m, uint32_t n, uint32_t k_bytes);
 
 // ffn_backward.hip (arguments checked by the caller).
 int mi355_glu_backward_limits(mi355_dev *dev, const char *what, uint32_t T, uint32_t F);
@@ -60,10 +72,18 @@ __device__ __forceinline__ float ffn_gelu_tanh_arg(float x) {
   const float c = fminf(fmaxf(x, -16.0f), 16.0f);
   return 1.59576912160573071f * c * fmaf(0.044715f * c, c, 1.0f);
 }
+// erf to 1.5e-7 absolute (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26: a polynomial of fifth degree in
+// 1 / (1 + 0.3275911 |x|), times exp(-x^2)): what 1 + erf keeps of it in fp32 anyway, in a dozen instructions.
+__device__ __forceinline__ float ffn_erf(float x) {
+  const float a = fabsf(x), t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, a, 1.0f));
+  const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+  const float e = __builtin_amdgcn_exp2f(x * x * -1.44269504088896341f);
+  return copysignf(fmaf(-p, e, 1.0f), x);
+}
 __device__ __forceinline__ float ffn_act(int act, float x) {
   if (act == MI355_GLU_SILU) return x * ffn_sigmoid(x);
   if (act == MI355_GLU_GELU_TANH) return x * ffn_sigmoid(ffn_gelu_tanh_arg(x));
-  if (act == MI355_GLU_GELU) return 0.5f * x * (1.0f + erff(x * 0.707106781186547524f));
+  if (act == MI355_GLU_GELU) return 0.5f * x * (1.0f + ffn_erf(x * 0.707106781186547524f));
   return x < 0.0f ? 0.0f : x;   // (a NaN stays one)
 }
 // The activation and its derivative.
@@ -78,7 +98,7 @@ __device__ __forceinline__ void ffn_act_grad(int act, float x, float &a, float &
     a = x * p;
     da = fmaf(a * (1.0f - p), 1.59576912160573071f * fmaf(0.134145f * c, c, 1.0f), p);
   } else if (act == MI355_GLU_GELU) {
-    const float cdf = 0.5f * (1.0f + erff(x * 0.707106781186547524f));
+    const float cdf = 0.5f * (1.0f + ffn_erf(x * 0.707106781186547524f));
     a = x * cdf;
     const float c = fminf(fmaxf(x, -16.0f), 16.0f);
     da = fmaf(c * 0.398942280401432678f, __builtin_amdgcn_exp2f(c * c * -0.72134752044448170f), cdf);
@@ -105,6 +125,130 @@ __device__ __forceinline__ float ffn_load1(const void *base, uint64_t at, int ty
 // int32 sum -> value.  The sum is rounded to fp32 (exact below 2^24), then multiplied by the two scales in turn, so that
 // neither product of a small and a large scale leaves the range before the sum is in it.
 __device__ __forceinline__ float ffn_scaled(int32_t sum, float sa, float sb) { return (float)sum * sa * sb; }
+// (the addition as one operation with the second product, in every kernel alike)
+__device__ __forceinline__ float ffn_scaled_plus(int32_t sum, float sa, float sb, float bias) { return fmaf((float)sum * sa, sb, bias); }
+
+// ---- finished tiles of the tile kernels --------------------------------------------------------------------------------
+// A wave's sums are tiles of 16x16, and a lane holds 4 consecutive columns of one row of a tile: row lane % 16, columns
+// 4 (lane / 16) on (the products are issued transposed).  Two neighbouring tiles are finished together: of 16-bit
+// outputs the two first trade halves (v_permlane16_swap exchanges the odd lane groups of the first tile with the even
+// ones of the second), after which a lane holds 8 consecutive columns, 16 bytes.
+struct FfnPair {
+  float x[2][4];
+};
+// Rows end at m, columns at n.  Addresses are aligned to the elements only: the part's vector stores take that.
+__device__ __forceinline__ void ffn_store_pair(void *base, uint64_t ld, int type, uint32_t row, uint32_t col0, uint32_t lane, uint32_t m, uint32_t n,
+                                               const FfnPair &v) {
+  const uint32_t g = lane / 16u;
+  if (type == MI355_TYPE_F32) {
+    if (row < m) {
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+        const uint32_t col = col0 + 16u * t + 4u * g;
+        float *to = static_cast<float *>(base) + (uint64_t)row * ld + col;
+        if (col + 4u <= n) {
+          __builtin_memcpy(__builtin_assume_aligned(to, 4), v.x[t], 16);
+        } else {   // (a loop, so that this rare case stays short code)
+          float x0 = v.x[t][0], x1 = v.x[t][1], x2 = v.x[t][2];
+#pragma unroll 1
+          for (uint32_t c = col; c < n; c++) {
+            *to++ = x0;
+            x0 = x1; x1 = x2;
+          }
+        }
+      }
+    }
+    return;
+  }
+  uint32_t p[2][2];
+#pragma unroll
+  for (int t = 0; t < 2; t++)
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+      p[t][h] = type == MI355_TYPE_F16 ? mi355_pack_f16x2(v.x[t][2 * h], v.x[t][2 * h + 1]) : mi355_pack_bf16x2(v.x[t][2 * h], v.x[t][2 * h + 1]);
+  const auto q01 = __builtin_amdgcn_permlane16_swap(p[0][0], p[1][0], false, false);
+  const auto q23 = __builtin_amdgcn_permlane16_swap(p[0][1], p[1][1], false, false);
+  const uint32_t w[4] = {q01[0], q23[0], q01[1], q23[1]};
+  const uint32_t col = col0 + 16u * (g & 1u) + 8u * (g >> 1);
+  if (row < m) {
+    uint16_t *to = static_cast<uint16_t *>(base) + (uint64_t)row * ld + col;
+    if (col + 8u <= n) {
+      __builtin_memcpy(__builtin_assume_aligned(to, 2), w, 16);
+    } else {   // (a loop, so that this rare case stays short code)
+      uint64_t lo = (uint64_t)w[1] << 32 | w[0], hi = (uint64_t)w[3] << 32 | w[2];
+#pragma unroll 1
+      for (uint32_t c = col; c < n; c++) {
+        *to++ = (uint16_t)lo;
+        lo = lo >> 16 | hi << 48;
+        hi >>= 16;
+      }
+    }
+  }
+}
+
+// What a lane needs for its columns of a pair of tiles, and for a row.
+template <int EPI>
+struct FfnColumns {
+  float sb[2][4], sb2[2][4], bias[2][4];
+  __device__ __forceinline__ void load(const FfnOut &o, uint32_t col0, uint32_t lane, uint32_t n) {
+    if constexpr (EPI == kEpiScaled || EPI == kEpiGatedScaled) {
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const uint32_t col = min(col0 + 16u * t + 4u * (lane / 16u) + e, n - 1u);
+          sb[t][e] = o.sb[col];
+          if constexpr (EPI == kEpiGatedScaled) sb2[t][e] = o.sb2[col];
+          else bias[t][e] = o.bias ? o.bias[col] : 0.0f;
+        }
+    }
+  }
+};
+
+// A pair of finished tiles (gated: of the gate, s, and of the other product, s2), as raw bits of fp32 or int32.
+template <int OP, int EPI>
+__device__ __forceinline__ void ffn_finish_pair(const FfnOut &o, uint32_t row, uint32_t col0, uint32_t lane, uint32_t m, uint32_t n, float sa,
+                                                const FfnColumns<EPI> &c, const i32x4v (&s)[2], const i32x4v (&s2)[2]) {
+  const int type = EPI == kEpiPartial ? MI355_TYPE_F32 : OP == kQuadBf16 ? MI355_TYPE_BF16 : OP == kQuadF16 ? MI355_TYPE_F16 : o.type;
+  FfnPair a, b;
+#pragma unroll
+  for (int t = 0; t < 2; t++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const int32_t v = s[t][e], v2 = s2[t][e];   // (through a scalar: __builtin_bit_cast of a vector's element reads element 0)
+      if constexpr (EPI == kEpiPartial) {
+        a.x[t][e] = __builtin_bit_cast(float, v);
+      } else if constexpr (OP == kQuadI8) {
+        a.x[t][e] = EPI == kEpiScaled && o.bias ? ffn_scaled_plus(v, sa, c.sb[t][e], c.bias[t][e]) : ffn_scaled(v, sa, c.sb[t][e]);
+        if constexpr (EPI == kEpiGatedScaled) b.x[t][e] = ffn_scaled(v2, sa, c.sb2[t][e]);
+      } else {
+        a.x[t][e] = __builtin_bit_cast(float, v);
+        if constexpr (EPI == kEpiGated) b.x[t][e] = __builtin_bit_cast(float, v2);
+      }
+    }
+  if constexpr (epi_is_gated(EPI)) {
+    if constexpr (EPI == kEpiGated)
+      if (o.g) {
+        ffn_store_pair(o.g, o.ldg, type, row, col0, lane, m, n, a);
+        ffn_store_pair(o.u, o.ldg, type, row, col0, lane, m, n, b);
+      }
+    // one branch on the activation for the 8 values
+    if (o.act == MI355_GLU_SILU) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) a.x[i / 4][i % 4] = ffn_act(MI355_GLU_SILU, a.x[i / 4][i % 4]) * b.x[i / 4][i % 4];
+    } else if (o.act == MI355_GLU_GELU_TANH) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) a.x[i / 4][i % 4] = ffn_act(MI355_GLU_GELU_TANH, a.x[i / 4][i % 4]) * b.x[i / 4][i % 4];
+    } else if (o.act == MI355_GLU_GELU) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) a.x[i / 4][i % 4] = ffn_act(MI355_GLU_GELU, a.x[i / 4][i % 4]) * b.x[i / 4][i % 4];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++) a.x[i / 4][i % 4] = ffn_act(MI355_GLU_RELU, a.x[i / 4][i % 4]) * b.x[i / 4][i % 4];
+    }
+  }
+  ffn_store_pair(o.c, o.ldc, type, row, col0, lane, m, n, a);
+}
 
 // One element of the output from its sum (gated: from its two sums), as raw bits of fp32 or int32.
 template <int EPI>
@@ -113,9 +257,8 @@ __device__ __forceinline__ void ffn_finish1(const FfnOut &o, uint32_t row, uint3
   if constexpr (EPI == kEpiPlain) {
     ffn_store1(o.c, at, o.type, __builtin_bit_cast(float, s0));
   } else if constexpr (EPI == kEpiScaled) {
-    float v = ffn_scaled(s0, o.sa[row], o.sb[col]);
-    if (o.bias) v += o.bias[col];
-    ffn_store1(o.c, at, o.type, v);
+    const float sa = o.sa[row], sb = o.sb[col];
+    ffn_store1(o.c, at, o.type, o.bias ? ffn_scaled_plus(s0, sa, sb, o.bias[col]) : ffn_scaled(s0, sa, sb));
   } else if constexpr (EPI == kEpiGated) {
     const float g = __builtin_bit_cast(float, s0), u = __builtin_bit_cast(float, s1);
     ffn_store1(o.c, at, o.type, ffn_act(o.act, g) * u);

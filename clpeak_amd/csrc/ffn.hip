@@ -41,9 +41,51 @@ int check_sizes(mi355_dev *dev, const char *what, uint32_t rows, uint32_t cols, 
 
 }  // namespace
 
-// Which kernel.  The caller has checked everything.
-int mi355_ffn_product(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p) {
-  return mi355_launch_ffn_rows(dev, op, epi, what, p);
+// Which kernel.  Up to 64 rows the weights' bytes are the time: ffn_rows.hip.  Above, the two tilings by their measured
+// time per step of K (0.85 us for a 256x256 tile of sums, 0.40 us for a 128x128 one, and some 5 us around the walk) and
+// the rounds of tiles that the CUs have to make; slices of K where those leave CUs idle, at the price of a second launch
+// and of the sums' way through memory.
+namespace {
+
+struct Choice {
+  enum { kRows, kQuad, kSmall } kernel;
+  uint32_t slices;
+};
+Choice choose(const mi355_dev *dev, int epi, uint32_t m, uint32_t n, uint32_t k_bytes, bool can_slice) {
+  if (dev->gemm_tiling == MI355_GEMM_TILING_256) return {Choice::kQuad, 1};
+  const bool pinned = dev->gemm_tiling == MI355_GEMM_TILING_128;
+  if (m <= 64u && !pinned) return {Choice::kRows, 1};
+  const uint64_t cus = dev->props.num_cus > 0 ? (uint64_t)dev->props.num_cus : 1u, steps = k_bytes / 128u;
+  const uint64_t sums_n = epi_is_gated(epi) ? 2ull * n : n;
+  const uint64_t big = ((m + 255ull) / 256u) * ((sums_n + 255u) / 256u), small = ((m + 127ull) / 128u) * ((sums_n + 127u) / 128u);
+  auto rounds = [&](uint64_t tiles) { return (double)((tiles + cus - 1u) / cus); };
+  const double big_us = rounds(big) * (double)steps * 0.85 + 6.0;
+  double best = rounds(small) * (double)steps * 0.40 + 5.0;
+  Choice c{Choice::kSmall, 1};
+  if (can_slice && !epi_is_gated(epi)) {
+    for (uint32_t s = 2; s <= 16u && s * 4u <= steps; s++) {
+      const double us = rounds(small * s) * (double)((steps + s - 1u) / s) * 0.40 + 5.0 + 4.0 + (double)m * n * (s * 8.0 + 2.0) / 4e6;
+      if (us < best) { best = us; c.slices = s; }
+    }
+  }
+  if (big_us < best && !pinned) return {Choice::kQuad, 1};
+  return c;
+}
+
+}  // namespace
+
+size_t mi355_ffn_workspace(const mi355_dev *dev, int epi, uint32_t m, uint32_t n, uint32_t k_bytes) {
+  const Choice c = choose(dev, epi, m, n, k_bytes, true);
+  return c.slices > 1 ? (size_t)(c.slices * (uint64_t)m * mi355_ffn_slice_row(n) * 4u) : 0;
+}
+
+// The caller has checked everything.
+int mi355_ffn_product(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p, void *workspace, size_t workspace_bytes) {
+  Choice c = choose(dev, epi, p.m, p.n, p.k_bytes, true);
+  if (c.slices > 1 && (!workspace || workspace_bytes < mi355_ffn_workspace(dev, epi, p.m, p.n, p.k_bytes))) c = choose(dev, epi, p.m, p.n, p.k_bytes, false);
+  if (c.kernel == Choice::kRows) return mi355_launch_ffn_rows(dev, op, epi, what, p);
+  if (c.kernel == Choice::kQuad) return mi355_launch_ffn_quad(dev, op, epi, what, p);
+  return mi355_launch_ffn_small(dev, op, epi, what, p, c.slices, workspace);
 }
 
 extern "C" int mi355_glu_forward(mi355_dev *dev, int type, int act, const void *X, uint64_t ldx, const void *Wg, const void *Wu, uint64_t ldw,
@@ -68,7 +110,7 @@ extern "C" int mi355_glu_forward(mi355_dev *dev, int type, int act, const void *
   p.lda = ldx * 2; p.ldb = ldw * 2;
   p.m = T; p.n = F; p.k_bytes = D * 2;
   p.out.c = H; p.out.ldc = ldh; p.out.g = G; p.out.u = U; p.out.ldg = ldg; p.out.type = type; p.out.act = act;
-  return mi355_ffn_product(dev, type == MI355_TYPE_BF16 ? kQuadBf16 : kQuadF16, kEpiGated, what, p);
+  return mi355_ffn_product(dev, type == MI355_TYPE_BF16 ? kQuadBf16 : kQuadF16, kEpiGated, what, p, nullptr, 0);
 }
 
 extern "C" int mi355_glu_backward_workspace(mi355_dev *dev, uint32_t T, uint32_t F, uint32_t D, size_t *bytes) {
@@ -121,6 +163,7 @@ extern "C" int mi355_gemm_i8_scaled_workspace(mi355_dev *dev, uint32_t M, uint32
   MI355_REQUIRE(dev, bytes, "gemm_i8_scaled_workspace: null out pointer");
   *bytes = 0;
   if (int rc = check_sizes(dev, "gemm_i8_scaled_workspace", M, N, K, 1)) return rc;
+  if (M > 0) *bytes = mi355_ffn_workspace(dev, kEpiScaled, M, N, K);
   return MI355_OK;
 }
 
@@ -143,14 +186,13 @@ extern "C" int mi355_gemm_i8_scaled(mi355_dev *dev, const int8_t *A, uint64_t ld
   MI355_REQUIRE(dev, (uintptr_t)bias % 4u == 0, "%s: the bias is not aligned to its elements", what);
   if (int rc = check_matrix(dev, what, "C", C, ldc, N, type == MI355_TYPE_F32 ? 4 : 2)) return rc;
   MI355_REQUIRE(dev, ((uintptr_t)workspace & 15u) == 0, "%s: the workspace must be 16-byte aligned", what);
-  (void)workspace_bytes;
   MI355_SET_DEVICE(dev);
   FfnProduct p{};
   p.a = (const uint8_t *)A; p.b = (const uint8_t *)B;
   p.lda = lda; p.ldb = ldb;
   p.m = M; p.n = N; p.k_bytes = K;
   p.out.c = C; p.out.ldc = ldc; p.out.sa = scale_a; p.out.sb = scale_b; p.out.bias = bias; p.out.type = type;
-  return mi355_ffn_product(dev, kQuadI8, kEpiScaled, what, p);
+  return mi355_ffn_product(dev, kQuadI8, kEpiScaled, what, p, workspace, workspace_bytes);
 }
 
 extern "C" int mi355_glu_i8(mi355_dev *dev, int act, const int8_t *A, uint64_t lda, const int8_t *Bg, const int8_t *Bu, uint64_t ldb,
@@ -176,5 +218,5 @@ extern "C" int mi355_glu_i8(mi355_dev *dev, int act, const int8_t *A, uint64_t l
   p.lda = lda; p.ldb = ldb;
   p.m = M; p.n = F; p.k_bytes = K;
   p.out.c = H; p.out.ldc = ldh; p.out.sa = scale_a; p.out.sb = scale_g; p.out.sb2 = scale_u; p.out.type = type; p.out.act = act;
-  return mi355_ffn_product(dev, kQuadI8, kEpiGatedScaled, what, p);
+  return mi355_ffn_product(dev, kQuadI8, kEpiGatedScaled, what, p, nullptr, 0);
 }

@@ -170,7 +170,7 @@ int mi355_launch_glu_backward(mi355_dev *dev, int type, int act, const void *dH,
     q.b = ws + p.wt; q.ldb = 4 * p.fk;
     q.m = T; q.n = D; q.k_bytes = (uint32_t)(4 * p.fk);
     q.out.c = dX; q.out.ldc = lddx;
-    if (int rc = mi355_ffn_product(dev, op, kEpiPlain, "glu_backward (dX)", q)) return rc;
+    if (int rc = mi355_ffn_product(dev, op, kEpiPlain, "glu_backward (dX)", q, nullptr, 0)) return rc;
   }
   if (dWg) {
     if (int rc = turn(dev, X, ldx, ws + p.xt, p.tp, T, p.tp, D)) return rc;
@@ -181,7 +181,7 @@ int mi355_launch_glu_backward(mi355_dev *dev, int type, int act, const void *dH,
     for (int half = 0; half < 2; half++) {
       q.a = ws + p.cols + half * p.fp * p.tp * 2;
       q.out.c = half ? dWu : dWg;
-      if (int rc = mi355_ffn_product(dev, op, kEpiPlain, "glu_backward (dW)", q)) return rc;
+      if (int rc = mi355_ffn_product(dev, op, kEpiPlain, "glu_backward (dW)", q, nullptr, 0)) return rc;
     }
   }
   return MI355_OK;

@@ -1,0 +1,193 @@
+// The feed-forward products on the schedule of gemm_small.hip: a workgroup of four waves and one 128x128 tile of sums, for
+// products that have too few 256x256 ones.  Operands may end inside a tile (ffn_quad.hip says how), and for the gated
+// projection the tile's rows of B are 32 of the gate's weights, the same 32 of the other projection's, and again 32 and 32:
+// a wave fetches one matrix's and owns 32 channels of both.
+//
+// Where even these tiles are few and K is long, K is cut into slices, a workgroup for each tile and slice; the sums of a
+// slice go to the workspace as they are and a second launch adds the slices in their order and finishes (int8 sums are
+// exact however they are cut).
+#include "ffn.h"
+#include "gemm_small_step.h"
+
+namespace {
+
+template <int OP, int EPI, int I, int JP>
+__device__ __forceinline__ void finish_tiles(const FfnProduct &p, uint32_t row0, uint32_t col0, uint32_t lane, const FfnColumns<EPI> &c) {
+  const uint32_t row = row0 + 16u * I;
+  float sa = 0.0f;
+  if constexpr (EPI == kEpiScaled || EPI == kEpiGatedScaled) sa = p.out.sa[min(row, p.m - 1u)];
+  const i32x4v s[2] = {small_take_tile<I * 4 + JP>(), small_take_tile<I * 4 + JP + 1>()};
+  if constexpr (epi_is_gated(EPI)) {
+    const i32x4v s2[2] = {small_take_tile<I * 4 + 2>(), small_take_tile<I * 4 + 3>()};
+    ffn_finish_pair<OP, EPI>(p.out, row, col0, lane, p.m, p.n, sa, c, s, s2);
+  } else {
+    ffn_finish_pair<OP, EPI>(p.out, row, col0 + 16u * JP, lane, p.m, p.n, sa, c, s, s);
+  }
+}
+template <int OP, int EPI, int JP>
+__device__ __forceinline__ void finish_columns(const FfnProduct &p, uint32_t row0, uint32_t col0, uint32_t lane) {
+  FfnColumns<EPI> c;
+  c.load(p.out, col0 + 16u * JP, lane, p.n);
+  finish_tiles<OP, EPI, 0, JP>(p, row0, col0, lane, c);
+  finish_tiles<OP, EPI, 1, JP>(p, row0, col0, lane, c);
+  finish_tiles<OP, EPI, 2, JP>(p, row0, col0, lane, c);
+  finish_tiles<OP, EPI, 3, JP>(p, row0, col0, lane, c);
+}
+
+// Slice blockIdx.y of p.slices of K; its sums go to p.out.c as matrix number blockIdx.y there (kEpiPartial).
+template <int OP, int EPI>
+__global__ void __launch_bounds__(kSmallThreads) ffn_small_kernel(FfnProduct p, uint32_t tiles_m, uint32_t tiles_n) {
+  constexpr bool kGated = epi_is_gated(EPI);
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  const uint32_t tid = threadIdx.x, lane = tid % 64;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid / 64);
+  const uint32_t wm = wave / 2, wn = wave % 2;
+  TileGrid grid;
+  grid.tiles_m = tiles_m; grid.tiles_n = tiles_n; grid.total = tiles_m * tiles_n;
+  grid.first = blockIdx.x; grid.stride = gridDim.x; grid.mine = 1;
+  uint32_t tm, tn;
+  tile_at(grid, 0, tm, tn);
+  uint32_t steps = p.k_bytes / kRowBytes, k0 = 0;
+  if constexpr (EPI == kEpiPartial) {
+    const uint32_t all = steps;
+    k0 = (uint32_t)((uint64_t)all * blockIdx.y / gridDim.y);
+    steps = (uint32_t)((uint64_t)all * (blockIdx.y + 1u) / gridDim.y) - k0;
+  }
+  const uint32_t lda = (uint32_t)p.lda, ldb = (uint32_t)p.ldb;
+  constexpr uint32_t kRing = kSmallSlots * kSmallSlot;
+  auto after = [](uint32_t slot_off) { return slot_off + kSmallSlot == kRing ? 0u : slot_off + kSmallSlot; };
+
+  // global -> LDS: wave w fills rows [32w, 32w+32) of the A slab and of the B slab, 8 rows per instruction; lane i is
+  // position i%8 of row i/8, which holds logical chunk (i%8) ^ (i/8)
+  const uint32_t lds_base = (uint32_t)(uintptr_t)lds;
+  const uint32_t dst_wave = __builtin_amdgcn_readfirstlane(lds_base + wave * 32u * (uint32_t)kRowBytes);
+  SmallEdgeWalk w;
+  const uint32_t a_row = min(tm * 128u + wave * 32u, p.m - 1u);
+  const uint32_t b_row = min(kGated ? tn * 64u + wave / 2u * 32u : tn * 128u + wave * 32u, p.n - 1u);
+  const uint8_t *b = kGated && (wave & 1u) ? p.b2 : p.b;
+#pragma unroll
+  for (uint32_t q = 0; q < 4; q++) {
+    const uint32_t chunk = ((lane % 8u) ^ (lane / 8u)) * 16u;
+    w.voff[q] = min(lane / 8u + 8u * q, p.m - 1u - a_row) * lda + chunk;
+    w.voff_b[q] = min(lane / 8u + 8u * q, p.n - 1u - b_row) * ldb + chunk;
+  }
+  w.ga = (uint64_t)(uintptr_t)(p.a + (uint64_t)a_row * lda + (uint64_t)k0 * kRowBytes);
+  w.gb = (uint64_t)(uintptr_t)(b + (uint64_t)b_row * ldb + (uint64_t)k0 * kRowBytes);
+  uint32_t fetch_left = steps, fill = 0, look = 0;   // slot offsets: the one to fill, the one to read
+  auto fetched = [&]() {                             // on to the next slab; past the last one: the first again
+    w.ga += kRowBytes;
+    w.gb += kRowBytes;
+    if (--fetch_left == 0u) { w.ga -= (uint64_t)steps * kRowBytes; w.gb -= (uint64_t)steps * kRowBytes; fetch_left = steps; }
+    fill = after(fill);
+  };
+  const uint32_t swz0 = ((lane / 16u) ^ (lane & 7u)) << 4;
+  const uint32_t lane_a = lds_base + (wm * 64u + lane % 16u) * kRowBytes + swz0;
+  const uint32_t lane_b = lds_base + kSmallSlab + (wn * 64u + lane % 16u) * kRowBytes + swz0;
+  auto place = [&]() {
+    w.a0 = lane_a + look; w.a1 = w.a0 ^ 64u;
+    w.b0 = lane_b + look; w.b1 = w.b0 ^ 64u;
+    w.dst = dst_wave + fill;
+  };
+
+  small_claim_accumulators();
+  small_zero_accumulators(std::make_integer_sequence<int, 64>{});
+
+  // slabs 0..3 into slots 0..3; the fragments of slab 0
+  for (uint32_t d = 0; d < kSmallAhead; d++) {
+    place();
+    small_load<0>(w); small_load<1>(w); small_load<2>(w); small_load<3>(w);
+    small_load<4>(w); small_load<5>(w); small_load<6>(w); small_load<7>(w);
+    fetched();
+  }
+  asm volatile("s_waitcnt vmcnt(%0)\n s_barrier" :: "n"(8 * (kSmallAhead - 1)) : "memory");
+  SmallFrags f0, f1;
+  place();
+  small_read<0>(f0, w); small_read<1>(f0, w); small_read<2>(f0, w); small_read<3>(f0, w);
+  small_read<4>(f0, w); small_read<5>(f0, w); small_read<6>(f0, w); small_read<7>(f0, w);
+  small_read<8>(f0, w); small_read<9>(f0, w); small_read<10>(f0, w); small_read<11>(f0, w);
+  small_read<12>(f0, w); small_read<13>(f0, w); small_read<14>(f0, w); small_read<15>(f0, w);
+  small_arrived(f0);
+
+  constexpr auto kSlots = std::make_integer_sequence<int, 32>{};
+  uint32_t s = 0;
+  for (; s + 2 < steps; s += 2) {
+    look = after(look); place();
+    small_step<OP, false>(kSlots, f0, f1, w);
+    fetched();
+    look = after(look); place();
+    small_step<OP, false>(kSlots, f1, f0, w);
+    fetched();
+  }
+  if (s + 2 == steps) {
+    look = after(look); place();
+    small_step<OP, false>(kSlots, f0, f1, w);
+    small_step<OP, true>(kSlots, f1, f0, w);
+  } else {
+    small_step<OP, true>(kSlots, f0, f1, w);
+  }
+  // the wait states between the last matrix instruction and the first read of its result; the fetches that ran
+  // ahead of the last step still write LDS
+  asm volatile("s_nop 15\n s_nop 15\n s_waitcnt vmcnt(0)" ::: "memory");
+  const uint32_t row0 = tm * 128u + wm * 64u + lane % 16u, col0 = tn * (kGated ? 64u : 128u) + wn * (kGated ? 32u : 64u);
+  if constexpr (EPI == kEpiPartial) p.out.c = static_cast<float *>(p.out.c) + (uint64_t)blockIdx.y * p.m * p.out.ldc;
+  finish_columns<OP, EPI, 0>(p, row0, col0, lane);
+  if constexpr (!kGated) finish_columns<OP, EPI, 2>(p, row0, col0, lane);
+}
+
+// The slices of four neighbouring columns added up and finished.  Bound by the workspace it reads, 4 bytes per slice and output.
+template <int OP, int EPI>
+__global__ void __launch_bounds__(256) ffn_join_kernel(FfnOut o, const float *partial, uint32_t slices, uint64_t ldp, uint32_t m, uint32_t n) {
+  const uint64_t quads = (n + 3u) / 4u, at = (uint64_t)blockIdx.x * 256u + threadIdx.x;
+  if (at >= quads * m) return;
+  const uint32_t row = (uint32_t)(at / quads), col = (uint32_t)(at % quads) * 4u;
+  const float *from = partial + (uint64_t)row * ldp + col;
+  i32x4v s = *reinterpret_cast<const i32x4v *>(from);
+  for (uint32_t k = 1; k < slices; k++) {
+    const i32x4v t = *reinterpret_cast<const i32x4v *>(from + (uint64_t)k * m * ldp);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const int32_t x = s[e], y = t[e];
+      if constexpr (OP == kQuadI8) s[e] = x + y;
+      else s[e] = __builtin_bit_cast(int32_t, __builtin_bit_cast(float, x) + __builtin_bit_cast(float, y));
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; e++)
+    if (col + e < n) ffn_finish1<EPI>(o, row, col + e, s[e], 0);
+}
+
+template <int OP, int EPI>
+int launch_tiles(mi355_dev *dev, const char *what, const FfnProduct &p, uint32_t slices) {
+  if (int rc = allow_full_lds(dev, &ffn_small_kernel<OP, EPI>, kLdsFfnSmall0 + ffn_kind(OP, EPI))) return rc;
+  const uint32_t cols = epi_is_gated(EPI) ? 64 : 128;
+  const uint64_t tiles_m = (p.m + 127ull) / 128u, tiles_n = (p.n + cols - 1ull) / cols;
+  MI355_REQUIRE(dev, tiles_m * tiles_n <= 0x3fffffffull, "%s: %u x %u outputs are more than one launch takes", what, p.m, p.n);
+  ffn_small_kernel<OP, EPI><<<dim3((uint32_t)(tiles_m * tiles_n), slices), kSmallThreads, kRingBytes, dev->stream>>>(p, (uint32_t)tiles_m, (uint32_t)tiles_n);
+  MI355_LAUNCH_CHECK(dev, what);
+  return MI355_OK;
+}
+template <int OP, int EPI>
+int launch(mi355_dev *dev, const char *what, const FfnProduct &p, uint32_t slices, void *workspace) {
+  if constexpr (EPI == kEpiPlain || EPI == kEpiScaled) {
+    if (slices > 1) {
+      FfnProduct q = p;
+      q.out.c = workspace;
+      q.out.ldc = mi355_ffn_slice_row(p.n);
+      q.out.type = MI355_TYPE_F32;
+      if (int rc = launch_tiles<OP, kEpiPartial>(dev, what, q, slices)) return rc;
+      const uint64_t blocks = ((uint64_t)((p.n + 3u) / 4u) * p.m + 255u) / 256u;
+      ffn_join_kernel<OP, EPI><<<(uint32_t)blocks, 256, 0, dev->stream>>>(p.out, (const float *)workspace, slices, q.out.ldc, p.m, p.n);
+      MI355_LAUNCH_CHECK(dev, what);
+      return MI355_OK;
+    }
+  }
+  return launch_tiles<OP, EPI>(dev, what, p, 1);
+}
+
+}  // namespace
+
+int mi355_launch_ffn_small(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p, uint32_t slices, void *workspace) {
+  if (op == kQuadI8) return epi == kEpiScaled ? launch<kQuadI8, kEpiScaled>(dev, what, p, slices, workspace) : launch<kQuadI8, kEpiGatedScaled>(dev, what, p, 1, nullptr);
+  if (op == kQuadBf16) return epi == kEpiPlain ? launch<kQuadBf16, kEpiPlain>(dev, what, p, slices, workspace) : launch<kQuadBf16, kEpiGated>(dev, what, p, 1, nullptr);
+  return epi == kEpiPlain ? launch<kQuadF16, kEpiPlain>(dev, what, p, slices, workspace) : launch<kQuadF16, kEpiGated>(dev, what, p, 1, nullptr);
+}

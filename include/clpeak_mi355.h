@@ -288,7 +288,9 @@ int mi355_gemm_fp8_e5m2(mi355_dev *dev, const uint8_t *A, const uint8_t *B, uint
  * workgroup per 128x128 tile, four times as many workgroups at half the arithmetic per operand byte.  AUTO (the
  * default of a new handle): 128 when the product has at most half a 256x256 tile per CU (2048 cubed: 64 tiles on
  * 256 CUs), 256 otherwise.  The 256 tiling needs M and N to be multiples of 256: a product with a multiple of 128 only
- * runs on the 128 tiling under AUTO and is refused under 256.  Results of the two agree within rounding (int8 exactly). */
+ * runs on the 128 tiling under AUTO and is refused under 256.  Results of the two agree within rounding (int8 exactly).
+ * The feed-forward operators further down, whose sizes need not be multiples of anything, take it too: under AUTO they
+ * choose by the work of either tiling, and a product of up to 64 rows runs on neither. */
 #define MI355_GEMM_TILING_AUTO 0
 #define MI355_GEMM_TILING_256  1
 #define MI355_GEMM_TILING_128  2

@@ -32,6 +32,14 @@ def dv():
     d.close()
 
 
+@pytest.fixture(params=["auto", "256", "128"])
+def tiled(dv, request):
+    """The library's own choice of kernel (few rows, 256x256 tiles, 128x128 tiles) and either tiling pinned."""
+    dv.gemm_tiling({"auto": capi.GEMM_TILING_AUTO, "256": capi.GEMM_TILING_256, "128": capi.GEMM_TILING_128}[request.param])
+    yield dv
+    dv.gemm_tiling(capi.GEMM_TILING_AUTO)
+
+
 def gen(seed):
     g = torch.Generator(device="cuda")
     g.manual_seed(seed)
@@ -115,7 +123,8 @@ SIZES = [  # T, F, D: one token, around the edges of 16-, 64-, 128- and 256-row 
 
 @pytest.mark.parametrize("type", [capi.TYPE_BF16, capi.TYPE_F16])
 @pytest.mark.parametrize("T, F, D", SIZES)
-def test_glu_forward(dv, type, T, F, D):
+def test_glu_forward(tiled, type, T, F, D):
+    dv = tiled
     dt, act = TYPES[type], ACTS[(T + F) % 4]
     g = gen(T * 7 + F)
     ldx, ldw, ldh, ldg = D + 8 * (T % 3), D + 8 * (F % 5), F + T % 4, F + F % 3
@@ -142,8 +151,9 @@ def test_glu_forward(dv, type, T, F, D):
             assert bool((gb == -7.0).all())
 
 
-def test_glu_forward_keeps_what_is_not_finite_in_its_row(dv):
+def test_glu_forward_keeps_what_is_not_finite_in_its_row(tiled):
     """An infinity or NaN in a row of X shows in that row of H and nowhere else; one in a row of a weight in that column."""
+    dv = tiled
     T, F, D = 70, 150, 128
     g = gen(3)
     x, wg, wu = (operand(g, n, D, D, torch.bfloat16, s) for n, s in ((T, 1.0), (F, 0.1), (F, 0.1)))
@@ -159,8 +169,9 @@ def test_glu_forward_keeps_what_is_not_finite_in_its_row(dv):
 
 
 @pytest.mark.parametrize("act", ACTS)
-def test_glu_activations_over_the_whole_range(dv, act):
+def test_glu_activations_over_the_whole_range(tiled, act):
     """G is one product of a value and 1 and U is 1, so H is the activation itself, at every bf16 value there is."""
+    dv = tiled
     D = 64
     bits = torch.arange(0, 1 << 16, device="cuda", dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
     vals = bits[torch.isfinite(bits)]
@@ -187,7 +198,8 @@ def test_glu_activations_over_the_whole_range(dv, act):
 
 @pytest.mark.parametrize("type", [capi.TYPE_BF16, capi.TYPE_F16])
 @pytest.mark.parametrize("T, F, D", SIZES)
-def test_glu_backward(dv, type, T, F, D):
+def test_glu_backward(tiled, type, T, F, D):
+    dv = tiled
     dt, act = TYPES[type], ACTS[(T + F + 1) % 4]
     g = gen(T * 11 + F)
     ldx, ldw, ldd, ldg, lddx, lddw = D + 8 * (T % 3), D + 8 * (F % 5), F + T % 4, F + F % 3, D + T % 3, D + F % 7
@@ -348,7 +360,8 @@ def i8_problem(M, N, K, seed, ws=1):
 
 @pytest.mark.parametrize("type", list(TYPES))
 @pytest.mark.parametrize("M, N, K", I8_SIZES)
-def test_gemm_i8_scaled(dv, type, M, N, K):
+def test_gemm_i8_scaled(tiled, type, M, N, K):
+    dv = tiled
     dt = TYPES[type]
     g, a, lda, (b,), ldb, sa, (sb,) = i8_problem(M, N, K, M + 3 * N + K)
     bias = torch.randn(N, generator=g, device="cuda")
@@ -369,8 +382,9 @@ def test_gemm_i8_scaled(dv, type, M, N, K):
         assert torch.equal(outs[0], outs[1])      # the sums are exact, however K is split
 
 
-def test_gemm_i8_scaled_the_deepest_sum(dv):
+def test_gemm_i8_scaled_the_deepest_sum(tiled):
     """K = 130944 of (-128)^2: the sum is 2^31 - 2^21, and its rounding to fp32 the only one before the scales."""
+    dv = tiled
     K, N = 130944, 5
     for M in (1, 70):
         a, b = (torch.full((r, K), -128, dtype=torch.int8, device="cuda") for r in (M, N))
@@ -380,8 +394,9 @@ def test_gemm_i8_scaled_the_deepest_sum(dv):
         assert bool((c == float(K * 16384)).all())
 
 
-def test_gemm_i8_scaled_scales_that_are_extreme(dv):
+def test_gemm_i8_scaled_scales_that_are_extreme(tiled):
     """A zero scale gives zeros, a NaN its row or column; a large scale against a small one stays in range."""
+    dv = tiled
     M, N, K = 40, 50, 256
     g, a, lda, (b,), ldb, sa, (sb,) = i8_problem(M, N, K, 9)
     sa[3], sa[4], sb[7], sa[5], sb[9] = 0.0, math.nan, math.nan, 1e-36, 1e36
@@ -397,7 +412,8 @@ def test_gemm_i8_scaled_scales_that_are_extreme(dv):
 
 @pytest.mark.parametrize("type", list(TYPES))
 @pytest.mark.parametrize("M, F, K", I8_SIZES)
-def test_glu_i8(dv, type, M, F, K):
+def test_glu_i8(tiled, type, M, F, K):
+    dv = tiled
     dt, act = TYPES[type], ACTS[(M + F) % 4]
     g, a, lda, (bg, bu), ldb, sa, (sg, su) = i8_problem(M, F, K, M + 5 * F + K, ws=2)
     ldh = F + M % 3
@@ -425,10 +441,11 @@ def test_no_rows_is_a_call_that_writes_nothing(dv):
 
 
 @pytest.mark.parametrize("T", [1, 19, 200, 600])
-def test_an_8bit_feed_forward_layer(dv, T):
+def test_an_8bit_feed_forward_layer(tiled, T):
     """Activations quantised for each token, the gated projection, its result quantised, the projection back: the layer
     as a server runs it, against the same steps in 64 bits on what each step was given, and as a whole against the
     unquantised layer (whose distance is that of the two 8-bit roundings, a percent or so)."""
+    dv = tiled
     D, F = 500, 700
     g = gen(T)
     Dp, Fp = 512, 768
