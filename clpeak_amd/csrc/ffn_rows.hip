@@ -27,34 +27,50 @@ __device__ __forceinline__ i32x4v rows_mfma(const i32x4v &b, const i32x4v &a, co
   }
 }
 
-// One window: the fragments of both K halves (16 bytes at 16 * (lane / 16), and 64 bytes on).
-template <int OP, int MT, int NB>
-struct RowWindow {
-  i32x4v a[MT][2], b[NB][2];
-  __device__ __forceinline__ void load(const uint8_t *const (&pa)[MT], const uint8_t *const (&pb)[NB], uint64_t at) {
+// U windows: the fragments of both K halves (16 bytes at 16 * (lane / 16), and 64 bytes on).
+template <int OP, int MT, int NB, int U>
+struct RowStage {
+  i32x4v a[U][MT][2], b[U][NB][2];
+  // `at`: byte offset along K of window number i of this wave
+  template <class At>
+  __device__ __forceinline__ void load(const uint8_t *const (&pa)[MT], const uint8_t *const (&pb)[NB], uint32_t i, At at) {
 #pragma unroll
-    for (int j = 0; j < NB; j++)
+    for (int k = 0; k < U; k++) {
+      const uint32_t o = at(i + k);
 #pragma unroll
-      for (int h = 0; h < 2; h++) b[j][h] = *reinterpret_cast<const i32x4v *>(pb[j] + at + 64 * h);
+      for (int j = 0; j < NB; j++)
 #pragma unroll
-    for (int i = 0; i < MT; i++)
+        for (int h = 0; h < 2; h++) b[k][j][h] = *reinterpret_cast<const i32x4v *>(pb[j] + o + 64 * h);
 #pragma unroll
-      for (int h = 0; h < 2; h++) a[i][h] = *reinterpret_cast<const i32x4v *>(pa[i] + at + 64 * h);
+      for (int t = 0; t < MT; t++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) a[k][t][h] = *reinterpret_cast<const i32x4v *>(pa[t] + o + 64 * h);
+    }
+    __builtin_amdgcn_sched_barrier(0);   // (the loads go out here, not where their values are needed)
   }
-  __device__ __forceinline__ void multiply(i32x4v (&acc)[MT][NB]) const {
+  __device__ __forceinline__ void multiply(i32x4v (&acc)[MT][NB], uint32_t windows = U) const {
 #pragma unroll
-    for (int h = 0; h < 2; h++)
+    for (int k = 0; k < U; k++) {
+      if ((uint32_t)k >= windows) break;
 #pragma unroll
-      for (int i = 0; i < MT; i++)
+      for (int h = 0; h < 2; h++)
 #pragma unroll
-        for (int j = 0; j < NB; j++) acc[i][j] = rows_mfma<OP>(b[j][h], a[i][h], acc[i][j]);
+        for (int t = 0; t < MT; t++)
+#pragma unroll
+          for (int j = 0; j < NB; j++) acc[t][j] = rows_mfma<OP>(b[k][j][h], a[k][t][h], acc[t][j]);
+    }
   }
 };
+
+#ifndef MI355_ROWS_UNROLL
+// Windows per stage, two stages in flight: as many as leave room for the sums.
+constexpr int rows_unroll(int mt, int nb) { return mt == 1 && nb == 1 ? 4 : mt * nb <= 4 && mt < 4 ? 2 : mt == 4 && nb == 1 ? 2 : 1; }
+#endif
 
 template <int OP, int EPI, int MT>
 __global__ void __launch_bounds__(kRowThreads) ffn_rows_kernel(FfnProduct p, uint32_t tiles_n) {
   constexpr int NB = epi_is_gated(EPI) ? 2 : 1;
-  constexpr int kUnroll = MT == 4 ? 2 : 4;   // 64 KiB in flight per workgroup, what the registers of 8 waves hold
+  constexpr int U = rows_unroll(MT, NB);
   __shared__ int32_t sums[kRowWaves][MT][NB][16][16];   // [row][column]
   const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t r = lane % 16, g = lane / 16;
@@ -75,19 +91,33 @@ __global__ void __launch_bounds__(kRowThreads) ffn_rows_kernel(FfnProduct p, uin
 #pragma unroll
     for (int j = 0; j < NB; j++) acc[i][j] = (i32x4v){0, 0, 0, 0};
 
-  const uint32_t windows = p.k_bytes / 128u;
-  uint32_t w = wave;
-  for (; w + kRowWaves * (kUnroll - 1) < windows; w += kRowWaves * kUnroll) {
-    RowWindow<OP, MT, NB> win[kUnroll];
-#pragma unroll
-    for (int k = 0; k < kUnroll; k++) win[k].load(pa, pb, (uint64_t)(w + kRowWaves * k) * 128u);
-#pragma unroll
-    for (int k = 0; k < kUnroll; k++) win[k].multiply(acc);
-  }
-  for (; w < windows; w += kRowWaves) {
-    RowWindow<OP, MT, NB> win;
-    win.load(pa, pb, (uint64_t)w * 128u);
-    win.multiply(acc);
+  // This wave's windows are numbers wave, wave + 8, .. of a walk over K that starts at a place of the workgroup's own: rows
+  // are a power of two apart as a rule, and workgroups that all read the same few columns of their rows would all read
+  // from the same few memory channels.
+  const uint32_t windows = p.k_bytes / 128u, begin = (tn / 8u * kRowWaves + tn % 8u * (windows / 8u)) % windows;
+  const uint32_t mine = wave < windows ? (windows - wave - 1u) / kRowWaves + 1u : 0u;
+  auto at = [&](uint32_t i) {
+    const uint32_t w = min(wave + kRowWaves * i, windows - 1u) + begin;   // (past the end: a window that is not multiplied)
+    return (w >= windows ? w - windows : w) * 128u;
+  };
+  // Two stages of U windows, one in flight while the other is multiplied.
+  RowStage<OP, MT, NB, U> s0, s1;
+  if (mine > 0) {
+    s0.load(pa, pb, 0, at);
+    uint32_t i = 0;
+    for (; i + 2 * U < mine; i += 2 * U) {
+      s1.load(pa, pb, i + U, at);
+      s0.multiply(acc);
+      s0.load(pa, pb, i + 2 * U, at);
+      s1.multiply(acc);
+    }
+    if (i + U < mine) {
+      s1.load(pa, pb, i + U, at);
+      s0.multiply(acc);
+      s1.multiply(acc, mine - i - U);
+    } else {
+      s0.multiply(acc, mine - i);
+    }
   }
 
 #pragma unroll
@@ -126,6 +156,7 @@ template <int OP, int EPI>
 int launch_by_rows(mi355_dev *dev, const char *what, const FfnProduct &p) {
   if (p.m <= 16u) return launch<OP, EPI, 1>(dev, what, p);
   if (p.m <= 32u) return launch<OP, EPI, 2>(dev, what, p);
+  if (p.m <= 48u) return launch<OP, EPI, 3>(dev, what, p);
   return launch<OP, EPI, 4>(dev, what, p);
 }
 

@@ -603,3 +603,45 @@ def test_a_borrowed_stream_survives_its_handle():
         d.close()
         st.synchronize()
         assert torch.equal(q.double(), quantized(x)[0])
+
+
+@pytest.mark.parametrize("type", list(TYPES))
+def test_quantize_rows_whose_largest_is_a_multiple_of_127(dv, type):
+    """amax = 127 c 2^n: there whole families of values lie exactly on a border, and 127 / amax is exact for powers of two c
+    only.  Every value of the type up to amax is tried (fp32: a step of 2^-10 of amax)."""
+    dt = TYPES[type]
+    for c in range(1, 17):
+        for n in (-9, 0, 5):
+            top = 127 * c * 2.0 ** n
+            if float(torch.tensor(top).to(dt)) != top:
+                continue
+            if dt == torch.float32:
+                x = torch.arange(0, 1025, dtype=torch.float64) * top / 1024
+            else:
+                x = torch.arange(0, 1 << 15, dtype=torch.int32).to(torch.int16).view(dt).double()
+                x = x[x <= top]
+            x = torch.cat((x, -x)).to(dt)[None].cuda()
+            K = x.shape[1]
+            q, s = torch.empty(1, K, dtype=torch.int8, device="cuda"), torch.empty(1, device="cuda")
+            dv.quantize_i8(type, x, K, q, K, s, 1, K, K)
+            rq, rs = quantized(x)
+            assert torch.equal(q.double(), rq) and torch.equal(s, rs), (c, n)
+
+
+@pytest.mark.parametrize("type", [capi.TYPE_BF16, capi.TYPE_F16])
+def test_quantize_every_value_against_every_mantissa(dv, type):
+    """Every mantissa amax can have (128 of bf16, every fifth of the 1024 of fp16) against every value of the type that is
+    no larger and no smaller than amax / 512."""
+    dt = TYPES[type]
+    bits = torch.arange(0, 1 << 15, dtype=torch.int32, device="cuda").to(torch.int16).view(dt)
+    vals = bits[torch.isfinite(bits)]
+    tops = vals[(vals >= 16.0) & (vals < 32.0)][:: 1 if type == capi.TYPE_BF16 else 5]
+    vals = vals[(vals >= 1 / 32) & (vals < 32.0)]
+    x = torch.where(vals[None] <= tops[:, None], vals[None], torch.zeros_like(vals)[None]).contiguous()
+    x[:, 1::2] *= -1
+    x = torch.cat((x, tops[:, None]), 1).contiguous()
+    M, K = x.shape
+    q, s = torch.empty(M, K, dtype=torch.int8, device="cuda"), torch.empty(M, device="cuda")
+    dv.quantize_i8(type, x, K, q, K, s, M, K, K)
+    rq, rs = quantized(x)
+    assert torch.equal(q.double(), rq) and torch.equal(s, rs)
