@@ -40,12 +40,24 @@ int mi355_launch_ffn_rows(mi355_dev *dev, int op, int epi, const char *what, con
 
 // ffn_quad.hip / ffn_small.hip: on 256x256 and on 128x128 tiles of sums (gated: of 256x128 / 128x64 outputs).
 int mi355_launch_ffn_quad(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p);
+// ffn_mid.hip: on 64x64 tiles of sums (gated: of 64x32 outputs), for some dozens of rows.
 // slices > 1 (one product, not gated): K is cut into so many, `workspace` holds `slices` matrices of m rows of
 // mi355_ffn_slice_row(n) 32-bit sums, on 16 bytes.
 int mi355_launch_ffn_small(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p, uint32_t slices, void *workspace);
+int mi355_launch_ffn_mid(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p, uint32_t slices, void *workspace);
+// ffn_join.hip: the second launch of a product in slices.
+int mi355_launch_ffn_join(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p, uint32_t slices, const void *workspace);
 inline uint64_t mi355_ffn_slice_row(uint32_t n) { return (n + 3ull) / 4u * 4u; }
+// The product whose outputs are the sums of the slices, in the workspace.
+inline FfnProduct mi355_ffn_slices_of(const FfnProduct &p, void *workspace) {
+  FfnProduct q = p;
+  q.out.c = workspace;
+  q.out.ldc = mi355_ffn_slice_row(p.n);
+  q.out.type = MI355_TYPE_F32;
+  return q;
+}
 // Bits of mi355_dev::full_lds_allowed: three operand types with up to three kinds of product each.
-enum { kLdsFfnQuad0 = 24, kLdsFfnSmall0 = 36 };
+enum { kLdsFfnQuad0 = 24, kLdsFfnSmall0 = 33, kLdsFfnMid0 = 42 };
 constexpr int ffn_kind(int op, int epi) { return (op - kQuadBf16) * 3 + (epi == kEpiPartial ? 2 : epi_is_gated(epi) ? 1 : 0); }
 
 // ffn.hip: the product on the kernel that suits it, and the workspace that it can use.
@@ -54,7 +66,7 @@ size_t mi355_ffn_workspace(const mi355_dev *dev, int epi, uint32_t m, uint32_t n
 
 // ffn_backward.hip (arguments checked by the caller).
 int mi355_glu_backward_limits(mi355_dev *dev, const char *what, uint32_t T, uint32_t F);
-size_t mi355_glu_backward_bytes(uint32_t T, uint32_t F, uint32_t D);
+size_t mi355_glu_backward_bytes(const mi355_dev *dev, uint32_t T, uint32_t F, uint32_t D);
 int mi355_launch_glu_backward(mi355_dev *dev, int type, int act, const void *dH, uint64_t lddh, const void *X, uint64_t ldx, const void *Wg,
                               const void *Wu, uint64_t ldw, const void *G, const void *U, uint64_t ldg, void *dX, uint64_t lddx, void *dWg,
                               void *dWu, uint64_t lddw, uint32_t T, uint32_t F, uint32_t D, uint8_t *workspace);
@@ -186,6 +198,47 @@ __device__ __forceinline__ void ffn_store_pair(void *base, uint64_t ld, int type
   }
 }
 
+// Four neighbouring elements (the first `count` of them).
+__device__ __forceinline__ void ffn_store4(void *base, uint64_t at, int type, const float (&x)[4], uint32_t count) {
+  if (type == MI355_TYPE_F32) {
+    float *to = static_cast<float *>(base) + at;
+    if (count >= 4u) {
+      __builtin_memcpy(__builtin_assume_aligned(to, 4), x, 16);
+    } else {
+#pragma unroll
+      for (uint32_t e = 0; e < 3; e++)
+        if (e < count) to[e] = x[e];
+    }
+    return;
+  }
+  uint32_t w[2];
+#pragma unroll
+  for (int h = 0; h < 2; h++) w[h] = type == MI355_TYPE_F16 ? mi355_pack_f16x2(x[2 * h], x[2 * h + 1]) : mi355_pack_bf16x2(x[2 * h], x[2 * h + 1]);
+  uint16_t *to = static_cast<uint16_t *>(base) + at;
+  if (count >= 4u) {
+    __builtin_memcpy(__builtin_assume_aligned(to, 2), w, 8);
+  } else {
+#pragma unroll
+    for (uint32_t e = 0; e < 3; e++)
+      if (e < count) to[e] = (uint16_t)(w[e / 2] >> (16 * (e % 2)));
+  }
+}
+
+// One matrix instruction on 16-byte fragments, K half by K half; issued transposed (B first): a lane then holds 4
+// consecutive columns of one row.
+template <int OP>
+__device__ __forceinline__ i32x4v ffn_mfma(const i32x4v &b, const i32x4v &a, const i32x4v &c) {
+  if constexpr (OP == kQuadI8) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(b, a, c, 0, 0, 0);
+  } else if constexpr (OP == kQuadBf16) {
+    return __builtin_bit_cast(i32x4v, __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8v, b), __builtin_bit_cast(bf16x8v, a),
+                                                                           __builtin_bit_cast(f32x4v, c), 0, 0, 0));
+  } else {
+    return __builtin_bit_cast(i32x4v, __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8v, b), __builtin_bit_cast(half8v, a),
+                                                                          __builtin_bit_cast(f32x4v, c), 0, 0, 0));
+  }
+}
+
 // What a lane needs for its columns of a pair of tiles, and for a row.
 template <int EPI>
 struct FfnColumns {
@@ -248,6 +301,39 @@ __device__ __forceinline__ void ffn_finish_pair(const FfnOut &o, uint32_t row, u
     }
   }
   ffn_store_pair(o.c, o.ldc, type, row, col0, lane, m, n, a);
+}
+
+// Four neighbouring columns of one row (of them, those below n) from their sums (gated: from both sums each).
+template <int OP, int EPI>
+__device__ __forceinline__ void ffn_finish4(const FfnOut &o, uint32_t row, uint32_t col, uint32_t n, const i32x4v &s, const i32x4v &s2) {
+  if (col >= n) return;
+  const int type = EPI == kEpiPartial ? MI355_TYPE_F32 : OP == kQuadBf16 ? MI355_TYPE_BF16 : OP == kQuadF16 ? MI355_TYPE_F16 : o.type;
+  float x[4], y[4];
+  const float sa = EPI == kEpiScaled || EPI == kEpiGatedScaled ? o.sa[row] : 0.0f;
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const int32_t v = s[e], v2 = s2[e];   // (through a scalar: __builtin_bit_cast of a vector's element reads element 0)
+    const uint32_t c = min(col + e, n - 1u);
+    if constexpr (EPI == kEpiScaled) {
+      x[e] = o.bias ? ffn_scaled_plus(v, sa, o.sb[c], o.bias[c]) : ffn_scaled(v, sa, o.sb[c]);
+    } else if constexpr (EPI == kEpiGatedScaled) {
+      x[e] = ffn_scaled(v, sa, o.sb[c]);
+      y[e] = ffn_scaled(v2, sa, o.sb2[c]);
+    } else {
+      x[e] = __builtin_bit_cast(float, v);
+      y[e] = __builtin_bit_cast(float, v2);
+    }
+  }
+  if constexpr (EPI == kEpiGated)
+    if (o.g) {
+      ffn_store4(o.g, (uint64_t)row * o.ldg + col, type, x, n - col);
+      ffn_store4(o.u, (uint64_t)row * o.ldg + col, type, y, n - col);
+    }
+  if constexpr (epi_is_gated(EPI)) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) x[e] = ffn_act(o.act, x[e]) * y[e];
+  }
+  ffn_store4(o.c, (uint64_t)row * o.ldc + col, type, x, n - col);
 }
 
 // One element of the output from its sum (gated: from its two sums), as raw bits of fp32 or int32.

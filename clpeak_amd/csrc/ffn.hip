@@ -1,5 +1,7 @@
 // The entry points of the feed-forward products: their checks, and which kernel a product runs on.
 #include "ffn.h"
+#include <algorithm>
+#include <cmath>
 
 namespace {
 
@@ -41,51 +43,125 @@ int check_sizes(mi355_dev *dev, const char *what, uint32_t rows, uint32_t cols, 
 
 }  // namespace
 
-// Which kernel.  Up to 64 rows the weights' bytes are the time: ffn_rows.hip.  Above, the two tilings by their measured
-// time per step of K (0.85 us for a 256x256 tile of sums, 0.40 us for a 128x128 one, and some 5 us around the walk) and
-// the rounds of tiles that the CUs have to make; slices of K where those leave CUs idle, at the price of a second launch
-// and of the sums' way through memory.
+// Which kernel: the one whose time, by what was measured of it, is least.  Each has its own limit.
+//   rows   everything the workgroups read, the weights once and the rows of A once for each workgroup, at 8.4 TB/s through
+//          the vector caches, the weights at 5.5 TB/s from memory;
+//   tiles  of 64x64, 128x128 or 256x256 sums: rounds of tiles over the CUs, each the steps of K (128 bytes) times a step's
+//          time and what surrounds the walk (the 256x256 tiles' workgroups go on to their next tile without a break).  A
+//          step takes longer as the part fills up and its clock falls.  At least the time of the weights, more where CUs
+//          are idle and fewer bytes are in flight.
+// K in slices where the tiles leave CUs idle: shorter walks, for a second launch and the sums' way through memory.
+// Rows that would make the CUs go round once more for a few tiles are a product of their own: 4099 x 8190 x 8192 int8 as
+// 4096 rows in two full rounds of 256x256 tiles and 3 rows by themselves.
+// mi355_gemm_tiling pins a tiling, whatever the number of rows.
 namespace {
 
+enum Kernel { kOnRows, kOn64, kOn128, kOn256 };
 struct Choice {
-  enum { kRows, kQuad, kSmall } kernel;
-  uint32_t slices;
+  Kernel kernel = kOn256;
+  uint32_t slices = 1;
+  double us = 1e30;
 };
+struct Tiling {
+  Kernel kernel;
+  int pin;
+  double edge, step_us, full_step_us, round_us, once_us, weights;   // (the weights' bytes per us)
+};
+constexpr Tiling kTilings[] = {{kOn64, MI355_GEMM_TILING_64, 64, 0.20, 0.32, 4.0, 1.0, 5.5e6},
+                               {kOn128, MI355_GEMM_TILING_128, 128, 0.30, 0.47, 5.0, 0.0, 4.5e6},
+                               {kOn256, MI355_GEMM_TILING_256, 256, 0.85, 1.40, 2.0, 4.0, 4.5e6}};
+
+double count_of_cus(const mi355_dev *dev) { return dev->props.num_cus > 0 ? dev->props.num_cus : 1; }
+double columns_of_sums(int epi, uint32_t n) { return epi_is_gated(epi) ? 2.0 * n : (double)n; }
+
+double tiling_us(const Tiling &t, double cus, uint32_t m, uint32_t n, double sums_n, uint32_t k_bytes, uint32_t slices) {
+  const double steps = std::ceil(k_bytes / 128u / (double)slices), weights_us = sums_n * k_bytes / t.weights;
+  const double tiles = std::ceil(m / t.edge) * std::ceil(sums_n / t.edge) * slices;
+  const double busy = std::min(1.0, tiles / cus), rounds = std::ceil(tiles / cus);
+  const double step = t.step_us + (t.full_step_us - t.step_us) * busy;
+  double us = t.once_us + std::max(weights_us * (1.6 - 0.6 * busy) + t.round_us, rounds * (steps * step + t.round_us));
+  if (slices > 1) us += 4.0 + (double)m * n * (slices * 8.0 + 2.0) / 4e6;
+  return us;
+}
+
 Choice choose(const mi355_dev *dev, int epi, uint32_t m, uint32_t n, uint32_t k_bytes, bool can_slice) {
-  if (dev->gemm_tiling == MI355_GEMM_TILING_256) return {Choice::kQuad, 1};
-  const bool pinned = dev->gemm_tiling == MI355_GEMM_TILING_128;
-  if (m <= 64u && !pinned) return {Choice::kRows, 1};
-  const uint64_t cus = dev->props.num_cus > 0 ? (uint64_t)dev->props.num_cus : 1u, steps = k_bytes / 128u;
-  const uint64_t sums_n = epi_is_gated(epi) ? 2ull * n : n;
-  const uint64_t big = ((m + 255ull) / 256u) * ((sums_n + 255u) / 256u), small = ((m + 127ull) / 128u) * ((sums_n + 127u) / 128u);
-  auto rounds = [&](uint64_t tiles) { return (double)((tiles + cus - 1u) / cus); };
-  const double big_us = rounds(big) * (double)steps * 0.85 + 6.0;
-  double best = rounds(small) * (double)steps * 0.40 + 5.0;
-  Choice c{Choice::kSmall, 1};
-  if (can_slice && !epi_is_gated(epi)) {
-    for (uint32_t s = 2; s <= 16u && s * 4u <= steps; s++) {
-      const double us = rounds(small * s) * (double)((steps + s - 1u) / s) * 0.40 + 5.0 + 4.0 + (double)m * n * (s * 8.0 + 2.0) / 4e6;
-      if (us < best) { best = us; c.slices = s; }
-    }
+  const double cus = count_of_cus(dev), sums_n = columns_of_sums(epi, n);
+  Choice best;
+  auto take = [&](Kernel k, uint32_t slices, double us) {
+    if (us < best.us) { best.kernel = k; best.slices = slices; best.us = us; }
+  };
+  const int pin = dev->gemm_tiling;
+  if (pin == MI355_GEMM_TILING_AUTO && m <= 64u) {
+    const double a_rows = m <= 16u ? m : (m + 15u) / 16u * 16u;
+    take(kOnRows, 1, 2.5 + std::max(sums_n * k_bytes / 5.5e6, (sums_n + (n + 15u) / 16u * a_rows) * k_bytes / 8.4e6));
   }
-  if (big_us < best && !pinned) return {Choice::kQuad, 1};
-  return c;
+  for (const Tiling &t : kTilings) {
+    if (pin != MI355_GEMM_TILING_AUTO && pin != t.pin) continue;
+    const uint32_t most = can_slice && !epi_is_gated(epi) && t.kernel != kOn256 ? 16 : 1;
+    for (uint32_t s = 1; s <= most && (s == 1 || s * 4u <= k_bytes / 128u); s++) take(t.kernel, s, tiling_us(t, cus, m, n, sums_n, k_bytes, s));
+  }
+  return best;
+}
+
+// A product as one launch, or (main_rows > 0) as two by rows.
+struct Division {
+  Choice whole, rest;
+  uint32_t main_rows = 0;
+};
+Division divide(const mi355_dev *dev, int epi, uint32_t m, uint32_t n, uint32_t k_bytes, bool can_slice) {
+  Division d;
+  d.whole = choose(dev, epi, m, n, k_bytes, can_slice);
+  if (d.whole.kernel != kOn256 || dev->gemm_tiling != MI355_GEMM_TILING_AUTO) return d;
+  const double cus = count_of_cus(dev), sums_n = columns_of_sums(epi, n), tiles_n = std::ceil(sums_n / 256.0);
+  const double rounds = std::ceil(std::ceil(m / 256.0) * tiles_n / cus);
+  const double rows = std::floor((rounds - 1.0) * cus / tiles_n) * 256.0;   // in one round less
+  if (rows < 256.0 || rows >= m) return d;
+  const uint32_t main_rows = (uint32_t)rows;
+  const Choice rest = choose(dev, epi, m - main_rows, n, k_bytes, can_slice);
+  const double us = tiling_us(kTilings[2], cus, main_rows, n, sums_n, k_bytes, 1) + rest.us;
+  if (us < d.whole.us) { d.main_rows = main_rows; d.rest = rest; d.whole.slices = 1; }
+  return d;
+}
+
+size_t slices_bytes(const Choice &c, uint32_t m, uint32_t n) {
+  return c.slices > 1 ? (size_t)(c.slices * (uint64_t)m * mi355_ffn_slice_row(n) * 4u) : 0;
+}
+size_t division_bytes(const Division &d, uint32_t m, uint32_t n) {
+  return d.main_rows ? slices_bytes(d.rest, m - d.main_rows, n) : slices_bytes(d.whole, m, n);
+}
+
+int launch(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p, const Choice &c, void *workspace) {
+  if (c.kernel == kOnRows) return mi355_launch_ffn_rows(dev, op, epi, what, p);
+  if (c.kernel == kOn64) return mi355_launch_ffn_mid(dev, op, epi, what, p, c.slices, workspace);
+  if (c.kernel == kOn128) return mi355_launch_ffn_small(dev, op, epi, what, p, c.slices, workspace);
+  return mi355_launch_ffn_quad(dev, op, epi, what, p);
 }
 
 }  // namespace
 
 size_t mi355_ffn_workspace(const mi355_dev *dev, int epi, uint32_t m, uint32_t n, uint32_t k_bytes) {
-  const Choice c = choose(dev, epi, m, n, k_bytes, true);
-  return c.slices > 1 ? (size_t)(c.slices * (uint64_t)m * mi355_ffn_slice_row(n) * 4u) : 0;
+  return division_bytes(divide(dev, epi, m, n, k_bytes, true), m, n);
 }
 
 // The caller has checked everything.
 int mi355_ffn_product(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p, void *workspace, size_t workspace_bytes) {
-  Choice c = choose(dev, epi, p.m, p.n, p.k_bytes, true);
-  if (c.slices > 1 && (!workspace || workspace_bytes < mi355_ffn_workspace(dev, epi, p.m, p.n, p.k_bytes))) c = choose(dev, epi, p.m, p.n, p.k_bytes, false);
-  if (c.kernel == Choice::kRows) return mi355_launch_ffn_rows(dev, op, epi, what, p);
-  if (c.kernel == Choice::kQuad) return mi355_launch_ffn_quad(dev, op, epi, what, p);
-  return mi355_launch_ffn_small(dev, op, epi, what, p, c.slices, workspace);
+  Division d = divide(dev, epi, p.m, p.n, p.k_bytes, true);
+  const size_t need = division_bytes(d, p.m, p.n);
+  if (need > 0 && (!workspace || workspace_bytes < need)) d = divide(dev, epi, p.m, p.n, p.k_bytes, false);
+  if (d.main_rows == 0) return launch(dev, op, epi, what, p, d.whole, workspace);
+  FfnProduct first = p, rest = p;
+  first.m = d.main_rows;
+  const uint64_t elem = p.out.type == MI355_TYPE_F32 ? 4 : 2;
+  rest.m = p.m - d.main_rows;
+  rest.a += (uint64_t)d.main_rows * p.lda;
+  rest.out.c = static_cast<uint8_t *>(p.out.c) + d.main_rows * p.out.ldc * elem;
+  if (p.out.sa) rest.out.sa += d.main_rows;
+  if (p.out.g) {
+    rest.out.g = static_cast<uint8_t *>(p.out.g) + d.main_rows * p.out.ldg * elem;
+    rest.out.u = static_cast<uint8_t *>(p.out.u) + d.main_rows * p.out.ldg * elem;
+  }
+  if (int rc = launch(dev, op, epi, what, first, d.whole, nullptr)) return rc;
+  return launch(dev, op, epi, what, rest, d.rest, workspace);
 }
 
 extern "C" int mi355_glu_forward(mi355_dev *dev, int type, int act, const void *X, uint64_t ldx, const void *Wg, const void *Wu, uint64_t ldw,
@@ -119,7 +195,7 @@ extern "C" int mi355_glu_backward_workspace(mi355_dev *dev, uint32_t T, uint32_t
   *bytes = 0;
   if (int rc = check_sizes(dev, "glu_backward_workspace", T, F, D, 2)) return rc;
   if (int rc = mi355_glu_backward_limits(dev, "glu_backward_workspace", T, F)) return rc;
-  *bytes = mi355_glu_backward_bytes(T, F, D);
+  *bytes = mi355_glu_backward_bytes(dev, T, F, D);
   return MI355_OK;
 }
 
@@ -152,7 +228,7 @@ extern "C" int mi355_glu_backward(mi355_dev *dev, int type, int act, const void 
   if (T == 0) dX = nullptr;   // no rows
   if (!dX && !dWg) return MI355_OK;
   MI355_REQUIRE(dev, workspace && ((uintptr_t)workspace & 255u) == 0, "%s: the workspace is null or not aligned to 256 bytes", what);
-  const size_t need = mi355_glu_backward_bytes(T, F, D);
+  const size_t need = mi355_glu_backward_bytes(dev, T, F, D);
   MI355_REQUIRE(dev, workspace_bytes >= need, "%s: a workspace of %zu bytes, %zu are needed", what, workspace_bytes, need);
   MI355_SET_DEVICE(dev);
   return mi355_launch_glu_backward(dev, type, act, dH, lddh, X, ldx, Wg, Wu, ldw, G, U, ldg, dX, lddx, dWg, dWu, lddw, T, F, D, (uint8_t *)workspace);

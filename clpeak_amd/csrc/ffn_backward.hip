@@ -12,12 +12,13 @@ constexpr int kTileEdge = 64, kThreads = 256, kVec = 8;
 
 __host__ __device__ constexpr uint64_t round_up(uint64_t x, uint64_t to) { return (x + to - 1) / to * to; }
 
-// The workspace: dG | dU by rows [T][2 Fk], by columns 2 x [Fp][Tp], the weights turned [D][2 Fk], X turned [D][Tp].
+// The workspace: dG | dU by rows [T][2 Fk], by columns 2 x [Fp][Tp], the weights turned [D][2 Fk], X turned [D][Tp], and what
+// the products use of it where they are cut along their sums.
 struct Plan {
-  uint64_t fk, fp, tp;                      // F padded to a row of a product, F padded to whole tiles, T padded to a row
-  uint64_t rows, cols, wt, xt, bytes;       // offsets
+  uint64_t fk, fp, tp;                            // F padded to a row of a product, F padded to whole tiles, T padded to a row
+  uint64_t rows, cols, wt, xt, sums, bytes;       // offsets
 };
-Plan plan_of(uint32_t T, uint32_t F, uint32_t D) {
+Plan plan_of(const mi355_dev *dev, uint32_t T, uint32_t F, uint32_t D) {
   Plan p;
   p.fk = round_up(F, 64);
   p.fp = round_up(F, 256);
@@ -26,7 +27,10 @@ Plan plan_of(uint32_t T, uint32_t F, uint32_t D) {
   p.cols = round_up(p.rows + (uint64_t)T * 2 * p.fk * 2, 256);
   p.wt = round_up(p.cols + 2 * p.fp * p.tp * 2, 256);
   p.xt = round_up(p.wt + (uint64_t)D * 2 * p.fk * 2, 256);
-  p.bytes = round_up(p.xt + (uint64_t)D * p.tp * 2, 256);
+  p.sums = round_up(p.xt + (uint64_t)D * p.tp * 2, 256);
+  const uint64_t dx = T ? mi355_ffn_workspace(dev, kEpiPlain, T, D, (uint32_t)(4 * p.fk)) : 0;
+  const uint64_t dw = mi355_ffn_workspace(dev, kEpiPlain, F, D, (uint32_t)(2 * p.tp));
+  p.bytes = round_up(p.sums + (dx > dw ? dx : dw), 256);
   return p;
 }
 
@@ -67,32 +71,50 @@ __device__ __forceinline__ void store_column(const Tile &t, uint32_t c, uint32_t
   *reinterpret_cast<uint4 *>(dst) = __builtin_bit_cast(uint4, x);
 }
 
-// dG and dU of a 64x64 tile: by rows (dG at column f, dU at column fk + f of a row of 2 fk; zeros from F to fk) and by
-// columns (row f of [fp][tp], dU fp rows on; zeros from T to tp).
+// What precedes the products, all of it one launch: the workgroups are tiles of 64x64 values, first those of dG and dU, then
+// those of the matrices to be turned.
+struct Turn {               // dst[c][r] = src[r][c]: R rows of C values, rows of dst padded with zeros from R to a multiple of 64
+  const uint16_t *src;
+  uint16_t *dst;
+  uint64_t ld, ld_dst;
+  uint32_t R, tiles_c, tiles;   // C / 64 (C is a multiple of 64), tiles in all
+};
+struct Gate {
+  const uint16_t *dH, *G, *U;
+  uint64_t lddh, ldg;
+  uint16_t *rows, *cols;
+  uint32_t T, F, fk, tp;
+  uint64_t fp;
+  int act;
+  uint32_t tiles_f, tiles;
+  bool by_rows, by_columns;
+};
+
+// dG and dU of a tile: by rows (dG at column f, dU at column fk + f of a row of 2 fk; zeros from F to fk) and by columns
+// (row f of [fp][tp], dU fp rows on; zeros from T to tp).
 template <int TYPE>
-__global__ void __launch_bounds__(kThreads)
-glu_gate_grad_kernel(const uint16_t *dH, uint64_t lddh, const uint16_t *G, const uint16_t *U, uint64_t ldg, uint16_t *rows, uint16_t *cols,
-                     uint32_t T, uint32_t F, uint32_t fk, uint64_t fp, uint32_t tp, int act, uint32_t tiles_f) {
-  __shared__ Tile tg, tu;
-  const uint32_t f0 = blockIdx.x % tiles_f * kTileEdge, t0 = blockIdx.x / tiles_f * kTileEdge;
+__device__ __forceinline__ void gate_tile(const Gate &p, uint32_t tile, Tile &tg, Tile &tu) {
+  const uint32_t f0 = tile % p.tiles_f * kTileEdge, t0 = tile / p.tiles_f * kTileEdge;
   const uint32_t c = threadIdx.x % 8u * kVec, r0 = threadIdx.x / 8u;
 #pragma unroll
   for (uint32_t r = r0; r < kTileEdge; r += kThreads / 8) {
     const uint32_t t = t0 + r, f = f0 + c;
     Vec8 dg{}, du{};
-    if (t < T) {
-      const Vec8 h = load8(dH + (uint64_t)t * lddh, f, F), g = load8(G + (uint64_t)t * ldg, f, F), u = load8(U + (uint64_t)t * ldg, f, F);
+    if (t < p.T) {
+      const Vec8 h = load8(p.dH + (uint64_t)t * p.lddh, f, p.F), g = load8(p.G + (uint64_t)t * p.ldg, f, p.F), u = load8(p.U + (uint64_t)t * p.ldg, f, p.F);
 #pragma unroll
       for (int e = 0; e < kVec; e++) {
         float a, da;
-        ffn_act_grad(act, widen<TYPE>(g.v[e]), a, da);
+        ffn_act_grad(p.act, widen<TYPE>(g.v[e]), a, da);
         const float d = widen<TYPE>(h.v[e]);
         dg.v[e] = narrow<TYPE>(d * widen<TYPE>(u.v[e]) * da);   // (past F: 0 * 0)
         du.v[e] = narrow<TYPE>(d * a);
       }
-      uint16_t *to = rows + (uint64_t)t * 2u * fk + f;
-      *reinterpret_cast<uint4 *>(to) = __builtin_bit_cast(uint4, dg);
-      *reinterpret_cast<uint4 *>(to + fk) = __builtin_bit_cast(uint4, du);
+      if (p.by_rows) {
+        uint16_t *to = p.rows + (uint64_t)t * 2u * p.fk + f;
+        *reinterpret_cast<uint4 *>(to) = __builtin_bit_cast(uint4, dg);
+        *reinterpret_cast<uint4 *>(to + p.fk) = __builtin_bit_cast(uint4, du);
+      }
     }
 #pragma unroll
     for (int e = 0; e < kVec; e++) {
@@ -100,40 +122,51 @@ glu_gate_grad_kernel(const uint16_t *dH, uint64_t lddh, const uint16_t *G, const
       tu.at[r][c + e] = du.v[e];
     }
   }
+  if (!p.by_columns) return;
   __syncthreads();
 #pragma unroll
   for (uint32_t r = r0; r < kTileEdge; r += kThreads / 8) {   // r: a column of the tile, c: 8 of its rows
-    if (f0 + r < F) {
-      uint16_t *to = cols + (uint64_t)(f0 + r) * tp + t0 + c;
+    if (f0 + r < p.F) {
+      uint16_t *to = p.cols + (uint64_t)(f0 + r) * p.tp + t0 + c;
       store_column(tg, r, c, to);
-      store_column(tu, r, c, to + fp * tp);
+      store_column(tu, r, c, to + p.fp * p.tp);
     }
   }
 }
 
-// dst[c][r] = src[r][c], rows of dst padded with zeros from R to rp.  C and rp are multiples of 64; src rows on 16 bytes.
-__global__ void __launch_bounds__(kThreads) turn_kernel(const uint16_t *src, uint64_t ld, uint16_t *dst, uint64_t ld_dst, uint32_t R, uint32_t tiles_c) {
-  __shared__ Tile tile;
-  const uint32_t c0 = blockIdx.x % tiles_c * kTileEdge, r0 = blockIdx.x / tiles_c * kTileEdge;
+__device__ __forceinline__ void turn_tile(const Turn &p, uint32_t number, Tile &tile) {
+  const uint32_t c0 = number % p.tiles_c * kTileEdge, r0 = number / p.tiles_c * kTileEdge;
   const uint32_t c = threadIdx.x % 8u * kVec;
 #pragma unroll
   for (uint32_t r = threadIdx.x / 8u; r < kTileEdge; r += kThreads / 8) {
     Vec8 x{};
-    if (r0 + r < R) x = __builtin_bit_cast(Vec8, *reinterpret_cast<const uint4 *>(src + (uint64_t)(r0 + r) * ld + c0 + c));
+    if (r0 + r < p.R) x = __builtin_bit_cast(Vec8, *reinterpret_cast<const uint4 *>(p.src + (uint64_t)(r0 + r) * p.ld + c0 + c));
 #pragma unroll
     for (int e = 0; e < kVec; e++) tile.at[r][c + e] = x.v[e];
   }
   __syncthreads();
 #pragma unroll
-  for (uint32_t r = threadIdx.x / 8u; r < kTileEdge; r += kThreads / 8) store_column(tile, r, c, dst + (uint64_t)(c0 + r) * ld_dst + r0 + c);
+  for (uint32_t r = threadIdx.x / 8u; r < kTileEdge; r += kThreads / 8) store_column(tile, r, c, p.dst + (uint64_t)(c0 + r) * p.ld_dst + r0 + c);
 }
 
-int turn(mi355_dev *dev, const void *src, uint64_t ld, uint8_t *dst, uint64_t ld_dst, uint32_t R, uint64_t rp, uint32_t C) {
-  const uint64_t tiles = (uint64_t)(C / 64u) * (rp / 64u);
-  MI355_REQUIRE(dev, tiles <= 0x7fffffffull, "glu_backward: %u x %u values are more than one launch takes", R, C);
-  turn_kernel<<<(uint32_t)tiles, kThreads, 0, dev->stream>>>((const uint16_t *)src, ld, (uint16_t *)dst, ld_dst, R, C / 64u);
-  MI355_LAUNCH_CHECK(dev, "glu_backward (turn)");
-  return MI355_OK;
+template <int TYPE>
+__global__ void __launch_bounds__(kThreads) glu_backward_prepare_kernel(Gate gate, Turn t0, Turn t1, Turn t2) {
+  __shared__ Tile a, b;
+  uint32_t i = blockIdx.x;
+  if (i < gate.tiles) return gate_tile<TYPE>(gate, i, a, b);
+  i -= gate.tiles;
+  if (i < t0.tiles) return turn_tile(t0, i, a);
+  i -= t0.tiles;
+  if (i < t1.tiles) return turn_tile(t1, i, a);
+  turn_tile(t2, i - t1.tiles, a);
+}
+
+Turn turn(const void *src, uint64_t ld, uint8_t *dst, uint64_t ld_dst, uint32_t R, uint64_t rp, uint32_t C) {
+  Turn t;
+  t.src = (const uint16_t *)src; t.dst = (uint16_t *)dst;
+  t.ld = ld; t.ld_dst = ld_dst;
+  t.R = R; t.tiles_c = C / 64u; t.tiles = (uint32_t)((uint64_t)t.tiles_c * (rp / 64u));
+  return t;
 }
 
 }  // namespace
@@ -144,36 +177,42 @@ int mi355_glu_backward_limits(mi355_dev *dev, const char *what, uint32_t T, uint
   return MI355_OK;
 }
 
-size_t mi355_glu_backward_bytes(uint32_t T, uint32_t F, uint32_t D) { return (size_t)plan_of(T, F, D).bytes; }
+size_t mi355_glu_backward_bytes(const mi355_dev *dev, uint32_t T, uint32_t F, uint32_t D) { return (size_t)plan_of(dev, T, F, D).bytes; }
 
 int mi355_launch_glu_backward(mi355_dev *dev, int type, int act, const void *dH, uint64_t lddh, const void *X, uint64_t ldx, const void *Wg,
                               const void *Wu, uint64_t ldw, const void *G, const void *U, uint64_t ldg, void *dX, uint64_t lddx, void *dWg,
                               void *dWu, uint64_t lddw, uint32_t T, uint32_t F, uint32_t D, uint8_t *ws) {
-  const Plan p = plan_of(T, F, D);
+  const Plan p = plan_of(dev, T, F, D);
   const int op = type == MI355_TYPE_BF16 ? kQuadBf16 : kQuadF16;
-  const uint64_t tiles = p.fk / 64u * (p.tp / 64u);
-  MI355_REQUIRE(dev, tiles <= 0x7fffffffull, "glu_backward: %u x %u values are more than one launch takes", T, F);
-  auto *rows = (uint16_t *)(ws + p.rows), *cols = (uint16_t *)(ws + p.cols);
-#define GO(TYPE)                                                                                                             \
-  glu_gate_grad_kernel<TYPE><<<(uint32_t)tiles, kThreads, 0, dev->stream>>>((const uint16_t *)dH, lddh, (const uint16_t *)G,   \
-      (const uint16_t *)U, ldg, rows, cols, T, F, (uint32_t)p.fk, p.fp, (uint32_t)p.tp, act, (uint32_t)(p.fk / 64u))
-  if (type == MI355_TYPE_BF16) GO(MI355_TYPE_BF16);
-  else GO(MI355_TYPE_F16);
-#undef GO
-  MI355_LAUNCH_CHECK(dev, "glu_backward (gate)");
+  const uint64_t tiles = p.fk / 64u * (p.tp / 64u) + (uint64_t)(D / 64u) * (2u * (p.fk / 64u) + p.tp / 64u);
+  MI355_REQUIRE(dev, tiles <= 0x7fffffffull, "glu_backward: T = %u, F = %u, D = %u are more than one launch takes", T, F, D);
+  Gate gate;
+  gate.dH = (const uint16_t *)dH; gate.G = (const uint16_t *)G; gate.U = (const uint16_t *)U;
+  gate.lddh = lddh; gate.ldg = ldg;
+  gate.rows = (uint16_t *)(ws + p.rows); gate.cols = (uint16_t *)(ws + p.cols);
+  gate.T = T; gate.F = F; gate.fk = (uint32_t)p.fk; gate.fp = p.fp; gate.tp = (uint32_t)p.tp; gate.act = act;
+  gate.tiles_f = (uint32_t)(p.fk / 64u); gate.tiles = (uint32_t)(p.fk / 64u * (p.tp / 64u));
+  gate.by_rows = dX != nullptr; gate.by_columns = dWg != nullptr;
+  Turn wg{}, wu{}, x{};
+  if (dX) {
+    wg = turn(Wg, ldw, ws + p.wt, 2 * p.fk, F, p.fk, D);
+    wu = turn(Wu, ldw, ws + p.wt + p.fk * 2, 2 * p.fk, F, p.fk, D);
+  }
+  if (dWg) x = turn(X, ldx, ws + p.xt, p.tp, T, p.tp, D);
+  const uint32_t grid = gate.tiles + wg.tiles + wu.tiles + x.tiles;
+  if (type == MI355_TYPE_BF16) glu_backward_prepare_kernel<MI355_TYPE_BF16><<<grid, kThreads, 0, dev->stream>>>(gate, wg, wu, x);
+  else glu_backward_prepare_kernel<MI355_TYPE_F16><<<grid, kThreads, 0, dev->stream>>>(gate, wg, wu, x);
+  MI355_LAUNCH_CHECK(dev, "glu_backward (prepare)");
   FfnProduct q{};
   q.out.type = type;
   if (dX) {
-    if (int rc = turn(dev, Wg, ldw, ws + p.wt, 2 * p.fk, F, p.fk, D)) return rc;
-    if (int rc = turn(dev, Wu, ldw, ws + p.wt + p.fk * 2, 2 * p.fk, F, p.fk, D)) return rc;
     q.a = ws + p.rows; q.lda = 4 * p.fk;
     q.b = ws + p.wt; q.ldb = 4 * p.fk;
     q.m = T; q.n = D; q.k_bytes = (uint32_t)(4 * p.fk);
     q.out.c = dX; q.out.ldc = lddx;
-    if (int rc = mi355_ffn_product(dev, op, kEpiPlain, "glu_backward (dX)", q, nullptr, 0)) return rc;
+    if (int rc = mi355_ffn_product(dev, op, kEpiPlain, "glu_backward (dX)", q, ws + p.sums, p.bytes - p.sums)) return rc;
   }
   if (dWg) {
-    if (int rc = turn(dev, X, ldx, ws + p.xt, p.tp, T, p.tp, D)) return rc;
     q.lda = q.ldb = 2 * p.tp;
     q.b = ws + p.xt;
     q.m = F; q.n = D; q.k_bytes = (uint32_t)(2 * p.tp);
@@ -181,7 +220,7 @@ int mi355_launch_glu_backward(mi355_dev *dev, int type, int act, const void *dH,
     for (int half = 0; half < 2; half++) {
       q.a = ws + p.cols + half * p.fp * p.tp * 2;
       q.out.c = half ? dWu : dWg;
-      if (int rc = mi355_ffn_product(dev, op, kEpiPlain, "glu_backward (dW)", q, nullptr, 0)) return rc;
+      if (int rc = mi355_ffn_product(dev, op, kEpiPlain, "glu_backward (dW)", q, ws + p.sums, p.bytes - p.sums)) return rc;
     }
   }
   return MI355_OK;

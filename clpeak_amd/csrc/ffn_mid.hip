@@ -1,0 +1,132 @@
+// Products of some dozens of rows: too many to read every operand straight into registers (ffn_rows.hip: there each group of
+// 16 rows of A is read again by every workgroup, at the rate of the vector cache), too few to keep the matrix pipe busy.
+// The time is still that of reading the weights, so the kernel is built to keep as much of them in flight as LDS holds:
+// a workgroup of four waves owns a 64x64 tile of sums (gated: 32 channels of both matrices) and the whole LDS of a CU, ten
+// slots of 16 KiB (64 rows of A and 64 of B, 128 bytes of K), nine of them being filled while the tenth is read.  That is
+// 72 KiB of weights on their way to each CU, 18 MiB to the part, twice what its memory delivers in a trip.
+//
+// A step: wait for this wave's four loads of the slab (they complete in order, eight younger slabs may be in flight) and
+// for its own reads of the slab before; barrier; four loads into the slot that everybody has read; eight fragment reads,
+// eight matrix instructions.  Slab rows are swizzled as in the other kernels (chunk c of row r at position c ^ (r & 7)).
+#include "ffn.h"
+#include "gemm_ring.h"
+
+namespace {
+
+constexpr uint32_t kMidTile = 64, kMidThreads = 256;
+constexpr uint32_t kMidSlab = kMidTile * kRowBytes, kMidSlot = 2 * kMidSlab, kMidSlots = 10, kMidAhead = 9;
+static_assert(kMidSlots * kMidSlot == kRingBytes && kMidAhead + 1 == kMidSlots, "the ring is the whole LDS of a CU");
+
+// Slice blockIdx.y of gridDim.y of K (kEpiPartial: its sums go to p.out.c as matrix number blockIdx.y there).
+template <int OP, int EPI>
+__global__ void __launch_bounds__(kMidThreads) ffn_mid_kernel(FfnProduct p, uint32_t tiles_n) {
+  constexpr bool kGated = epi_is_gated(EPI);
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const uint32_t wm = wave / 2, wn = wave % 2;
+  const uint32_t tn = blockIdx.x % tiles_n, tm = blockIdx.x / tiles_n;
+  const uint32_t all = p.k_bytes / kRowBytes;
+  const uint32_t k0 = EPI == kEpiPartial ? (uint32_t)((uint64_t)all * blockIdx.y / gridDim.y) : 0u;
+  const uint32_t steps = EPI == kEpiPartial ? (uint32_t)((uint64_t)all * (blockIdx.y + 1u) / gridDim.y) - k0 : all;
+  const uint32_t lda = (uint32_t)p.lda, ldb = (uint32_t)p.ldb;
+
+  // global -> LDS: wave w fills rows [16w, 16w+16) of the A slab and of the B slab, 8 rows per instruction (rows past the
+  // last one: the last one); lane i is position i%8 of row i/8, which holds logical chunk (i%8) ^ (i/8)
+  const uint32_t lds_base = (uint32_t)(uintptr_t)lds;
+  const uint32_t dst_wave = __builtin_amdgcn_readfirstlane(lds_base + wave * 16u * (uint32_t)kRowBytes);
+  const uint32_t a_row = min(tm * kMidTile + wave * 16u, p.m - 1u);
+  const uint32_t b_row = min(kGated ? tn * 32u + wave / 2u * 16u : tn * kMidTile + wave * 16u, p.n - 1u);
+  const uint32_t chunk = ((lane % 8u) ^ (lane / 8u)) * 16u;
+  uint32_t va[2], vb[2];
+#pragma unroll
+  for (uint32_t q = 0; q < 2; q++) {
+    va[q] = min(lane / 8u + 8u * q, p.m - 1u - a_row) * lda + chunk;
+    vb[q] = min(lane / 8u + 8u * q, p.n - 1u - b_row) * ldb + chunk;
+  }
+  // the walk over K starts at a place of the workgroup's own (ffn_rows.hip says why) and wraps around; past its end it
+  // runs on, fetches that nobody reads, so that every step is the same code
+  const uint8_t *a0 = p.a + (uint64_t)a_row * lda + (uint64_t)k0 * kRowBytes;
+  const uint8_t *b0 = (kGated && (wave & 1u) ? p.b2 : p.b) + (uint64_t)b_row * ldb + (uint64_t)k0 * kRowBytes;
+  uint32_t at = (tn / 8u * 8u + tn % 8u * (steps / 8u)) % steps, fill = 0;
+  auto fetch = [&]() {
+    const uint64_t ga = (uint64_t)(uintptr_t)(a0 + (uint64_t)at * kRowBytes), gb = (uint64_t)(uintptr_t)(b0 + (uint64_t)at * kRowBytes);
+    MI355_LOAD_LDS(vb[0], gb, dst_wave + fill + kMidSlab);
+    MI355_LOAD_LDS(vb[1], gb, dst_wave + fill + kMidSlab + 1024u);
+    MI355_LOAD_LDS(va[0], ga, dst_wave + fill);
+    MI355_LOAD_LDS(va[1], ga, dst_wave + fill + 1024u);
+    at = at + 1u == steps ? 0u : at + 1u;
+    fill = fill + kMidSlot == kRingBytes ? 0u : fill + kMidSlot;
+  };
+  // LDS -> fragments: row lane%16 of the wave's part, chunk lane/16 (+4 for the second K half: bit 6 of the address)
+  const uint32_t swz = ((lane / 16u) ^ (lane & 7u)) << 4;
+  const uint32_t lane_a = (wm * 32u + lane % 16u) * kRowBytes + swz, lane_b = kMidSlab + (wn * 32u + lane % 16u) * kRowBytes + swz;
+
+  i32x4v acc[2][2];
+#pragma unroll
+  for (int i = 0; i < 4; i++) acc[i / 2][i % 2] = (i32x4v){0, 0, 0, 0};
+  for (uint32_t d = 0; d < kMidAhead; d++) fetch();
+  uint32_t look = 0;
+  for (uint32_t s = 0; s < steps; s++) {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n s_barrier" :: "n"(4 * (kMidAhead - 1)) : "memory");
+    fetch();
+    i32x4v a[2][2], b[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        a[i][h] = *reinterpret_cast<const i32x4v *>(lds + look + ((lane_a + i * 16 * kRowBytes) ^ (h * 64u)));
+        b[i][h] = *reinterpret_cast<const i32x4v *>(lds + look + ((lane_b + i * 16 * kRowBytes) ^ (h * 64u)));
+      }
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) acc[i][j] = ffn_mfma<OP>(b[j][h], a[i][h], acc[i][j]);
+    look = look + kMidSlot == kRingBytes ? 0u : look + kMidSlot;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the fetches that ran ahead still write LDS
+
+  FfnOut o = p.out;
+  if constexpr (EPI == kEpiPartial) o.c = static_cast<float *>(o.c) + (uint64_t)blockIdx.y * p.m * o.ldc;
+  const uint32_t g4 = 4u * (lane / 16u);
+#pragma unroll
+  for (uint32_t i = 0; i < 2; i++) {
+    const uint32_t row = tm * kMidTile + wm * 32u + 16u * i + lane % 16u;
+    if (row >= p.m) continue;
+    if constexpr (kGated) {
+      ffn_finish4<OP, EPI>(o, row, tn * 32u + wn * 16u + g4, p.n, acc[i][0], acc[i][1]);
+    } else {
+      ffn_finish4<OP, EPI>(o, row, tn * kMidTile + wn * 32u + g4, p.n, acc[i][0], acc[i][0]);
+      ffn_finish4<OP, EPI>(o, row, tn * kMidTile + wn * 32u + 16u + g4, p.n, acc[i][1], acc[i][1]);
+    }
+  }
+}
+
+template <int OP, int EPI>
+int launch_tiles(mi355_dev *dev, const char *what, const FfnProduct &p, uint32_t slices) {
+  if (int rc = allow_full_lds(dev, &ffn_mid_kernel<OP, EPI>, kLdsFfnMid0 + ffn_kind(OP, EPI))) return rc;
+  const uint32_t cols = epi_is_gated(EPI) ? 32 : 64;
+  const uint64_t tiles_m = (p.m + 63ull) / 64u, tiles_n = (p.n + cols - 1ull) / cols;
+  MI355_REQUIRE(dev, tiles_m * tiles_n <= 0x3fffffffull, "%s: %u x %u outputs are more than one launch takes", what, p.m, p.n);
+  ffn_mid_kernel<OP, EPI><<<dim3((uint32_t)(tiles_m * tiles_n), slices), kMidThreads, kRingBytes, dev->stream>>>(p, (uint32_t)tiles_n);
+  MI355_LAUNCH_CHECK(dev, what);
+  return MI355_OK;
+}
+template <int OP, int EPI>
+int launch(mi355_dev *dev, const char *what, const FfnProduct &p, uint32_t slices, void *workspace) {
+  if constexpr (EPI == kEpiPlain || EPI == kEpiScaled)
+    if (slices > 1) {
+      if (int rc = launch_tiles<OP, kEpiPartial>(dev, what, mi355_ffn_slices_of(p, workspace), slices)) return rc;
+      return mi355_launch_ffn_join(dev, OP, EPI, what, p, slices, workspace);
+    }
+  return launch_tiles<OP, EPI>(dev, what, p, 1);
+}
+
+}  // namespace
+
+int mi355_launch_ffn_mid(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p, uint32_t slices, void *workspace) {
+  if (op == kQuadI8) return epi == kEpiScaled ? launch<kQuadI8, kEpiScaled>(dev, what, p, slices, workspace) : launch<kQuadI8, kEpiGatedScaled>(dev, what, p, 1, nullptr);
+  if (op == kQuadBf16) return epi == kEpiPlain ? launch<kQuadBf16, kEpiPlain>(dev, what, p, slices, workspace) : launch<kQuadBf16, kEpiGated>(dev, what, p, 1, nullptr);
+  return epi == kEpiPlain ? launch<kQuadF16, kEpiPlain>(dev, what, p, slices, workspace) : launch<kQuadF16, kEpiGated>(dev, what, p, 1, nullptr);
+}

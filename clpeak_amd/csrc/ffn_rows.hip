@@ -13,20 +13,6 @@ namespace {
 
 constexpr int kRowWaves = 8, kRowThreads = 64 * kRowWaves;
 
-template <int OP>
-__device__ __forceinline__ i32x4v rows_mfma(const i32x4v &b, const i32x4v &a, const i32x4v &c) {
-  // the product is issued transposed (B first): a lane then holds 4 consecutive columns of one row
-  if constexpr (OP == kQuadI8) {
-    return __builtin_amdgcn_mfma_i32_16x16x64_i8(b, a, c, 0, 0, 0);
-  } else if constexpr (OP == kQuadBf16) {
-    return __builtin_bit_cast(i32x4v, __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8v, b), __builtin_bit_cast(bf16x8v, a),
-                                                                           __builtin_bit_cast(f32x4v, c), 0, 0, 0));
-  } else {
-    return __builtin_bit_cast(i32x4v, __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8v, b), __builtin_bit_cast(half8v, a),
-                                                                          __builtin_bit_cast(f32x4v, c), 0, 0, 0));
-  }
-}
-
 // U windows: the fragments of both K halves (16 bytes at 16 * (lane / 16), and 64 bytes on).
 template <int OP, int MT, int NB, int U>
 struct RowStage {
@@ -57,7 +43,7 @@ struct RowStage {
 #pragma unroll
         for (int t = 0; t < MT; t++)
 #pragma unroll
-          for (int j = 0; j < NB; j++) acc[t][j] = rows_mfma<OP>(b[k][j][h], a[k][t][h], acc[t][j]);
+          for (int j = 0; j < NB; j++) acc[t][j] = ffn_mfma<OP>(b[k][j][h], a[k][t][h], acc[t][j]);
     }
   }
 };

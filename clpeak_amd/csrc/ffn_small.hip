@@ -4,8 +4,7 @@
 // a wave fetches one matrix's and owns 32 channels of both.
 //
 // Where even these tiles are few and K is long, K is cut into slices, a workgroup for each tile and slice; the sums of a
-// slice go to the workspace as they are and a second launch adds the slices in their order and finishes (int8 sums are
-// exact however they are cut).
+// slice go to the workspace as they are and a second launch (ffn_join.hip) adds the slices and finishes.
 #include "ffn.h"
 #include "gemm_small_step.h"
 
@@ -34,7 +33,7 @@ __device__ __forceinline__ void finish_columns(const FfnProduct &p, uint32_t row
   finish_tiles<OP, EPI, 3, JP>(p, row0, col0, lane, c);
 }
 
-// Slice blockIdx.y of p.slices of K; its sums go to p.out.c as matrix number blockIdx.y there (kEpiPartial).
+// Slice blockIdx.y of gridDim.y of K (kEpiPartial: its sums go to p.out.c as matrix number blockIdx.y there).
 template <int OP, int EPI>
 __global__ void __launch_bounds__(kSmallThreads) ffn_small_kernel(FfnProduct p, uint32_t tiles_m, uint32_t tiles_n) {
   constexpr bool kGated = epi_is_gated(EPI);
@@ -134,28 +133,6 @@ __global__ void __launch_bounds__(kSmallThreads) ffn_small_kernel(FfnProduct p, 
   if constexpr (!kGated) finish_columns<OP, EPI, 2>(p, row0, col0, lane);
 }
 
-// The slices of four neighbouring columns added up and finished.  Bound by the workspace it reads, 4 bytes per slice and output.
-template <int OP, int EPI>
-__global__ void __launch_bounds__(256) ffn_join_kernel(FfnOut o, const float *partial, uint32_t slices, uint64_t ldp, uint32_t m, uint32_t n) {
-  const uint64_t quads = (n + 3u) / 4u, at = (uint64_t)blockIdx.x * 256u + threadIdx.x;
-  if (at >= quads * m) return;
-  const uint32_t row = (uint32_t)(at / quads), col = (uint32_t)(at % quads) * 4u;
-  const float *from = partial + (uint64_t)row * ldp + col;
-  i32x4v s = *reinterpret_cast<const i32x4v *>(from);
-  for (uint32_t k = 1; k < slices; k++) {
-    const i32x4v t = *reinterpret_cast<const i32x4v *>(from + (uint64_t)k * m * ldp);
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const int32_t x = s[e], y = t[e];
-      if constexpr (OP == kQuadI8) s[e] = x + y;
-      else s[e] = __builtin_bit_cast(int32_t, __builtin_bit_cast(float, x) + __builtin_bit_cast(float, y));
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < 4; e++)
-    if (col + e < n) ffn_finish1<EPI>(o, row, col + e, s[e], 0);
-}
-
 template <int OP, int EPI>
 int launch_tiles(mi355_dev *dev, const char *what, const FfnProduct &p, uint32_t slices) {
   if (int rc = allow_full_lds(dev, &ffn_small_kernel<OP, EPI>, kLdsFfnSmall0 + ffn_kind(OP, EPI))) return rc;
@@ -168,19 +145,11 @@ int launch_tiles(mi355_dev *dev, const char *what, const FfnProduct &p, uint32_t
 }
 template <int OP, int EPI>
 int launch(mi355_dev *dev, const char *what, const FfnProduct &p, uint32_t slices, void *workspace) {
-  if constexpr (EPI == kEpiPlain || EPI == kEpiScaled) {
+  if constexpr (EPI == kEpiPlain || EPI == kEpiScaled)
     if (slices > 1) {
-      FfnProduct q = p;
-      q.out.c = workspace;
-      q.out.ldc = mi355_ffn_slice_row(p.n);
-      q.out.type = MI355_TYPE_F32;
-      if (int rc = launch_tiles<OP, kEpiPartial>(dev, what, q, slices)) return rc;
-      const uint64_t blocks = ((uint64_t)((p.n + 3u) / 4u) * p.m + 255u) / 256u;
-      ffn_join_kernel<OP, EPI><<<(uint32_t)blocks, 256, 0, dev->stream>>>(p.out, (const float *)workspace, slices, q.out.ldc, p.m, p.n);
-      MI355_LAUNCH_CHECK(dev, what);
-      return MI355_OK;
+      if (int rc = launch_tiles<OP, kEpiPartial>(dev, what, mi355_ffn_slices_of(p, workspace), slices)) return rc;
+      return mi355_launch_ffn_join(dev, OP, EPI, what, p, slices, workspace);
     }
-  }
   return launch_tiles<OP, EPI>(dev, what, p, 1);
 }
 

@@ -203,7 +203,7 @@ int launch_quad(mi355_dev *dev, int op, const char *what, const void *A, const v
                 "gemm: M (%u) and N (%u) must be multiples of 256 on the 256x256 tiles this handle is set to", M, N);
   const uint64_t tiles = (uint64_t)(M / kTile) * (N / kTile);
   const bool small = !big_fits || dev->gemm_tiling == MI355_GEMM_TILING_128 ||
-                     (dev->gemm_tiling == MI355_GEMM_TILING_AUTO && 2u * tiles <= (uint64_t)(dev->props.num_cus > 0 ? dev->props.num_cus : 1));
+                     (dev->gemm_tiling != MI355_GEMM_TILING_256 && 2u * tiles <= (uint64_t)(dev->props.num_cus > 0 ? dev->props.num_cus : 1));
   if (small) return mi355_launch_gemm_small(dev, op, what, A, B, C, M, N, K * elem, scale);
   return mi355_launch_gemm_quad(dev, op, what, A, B, C, M, N, K * elem, scale);
 }
@@ -212,7 +212,7 @@ int launch_quad(mi355_dev *dev, int op, const char *what, const void *A, const v
 
 extern "C" int mi355_gemm_tiling(mi355_dev *dev, int tiling) {
   if (!dev) return mi355_fail(nullptr, MI355_ERR_ARG, "null device handle");
-  MI355_REQUIRE(dev, tiling == MI355_GEMM_TILING_AUTO || tiling == MI355_GEMM_TILING_256 || tiling == MI355_GEMM_TILING_128,
+  MI355_REQUIRE(dev, tiling == MI355_GEMM_TILING_AUTO || tiling == MI355_GEMM_TILING_256 || tiling == MI355_GEMM_TILING_128 || tiling == MI355_GEMM_TILING_64,
                 "gemm_tiling: unknown tiling %d", tiling);
   dev->gemm_tiling = tiling;
   return MI355_OK;

@@ -290,10 +290,12 @@ int mi355_gemm_fp8_e5m2(mi355_dev *dev, const uint8_t *A, const uint8_t *B, uint
  * 256 CUs), 256 otherwise.  The 256 tiling needs M and N to be multiples of 256: a product with a multiple of 128 only
  * runs on the 128 tiling under AUTO and is refused under 256.  Results of the two agree within rounding (int8 exactly).
  * The feed-forward operators further down, whose sizes need not be multiples of anything, take it too: under AUTO they
- * choose by the work of either tiling, and a product of up to 64 rows runs on neither. */
+ * choose by the time each tiling is measured to need, among them one of 64x64 tiles (64: pinned; the five calls above,
+ * which have no such tiling, take it as AUTO) and a kernel for few rows that has none. */
 #define MI355_GEMM_TILING_AUTO 0
 #define MI355_GEMM_TILING_256  1
 #define MI355_GEMM_TILING_128  2
+#define MI355_GEMM_TILING_64   3
 int mi355_gemm_tiling(mi355_dev *dev, int tiling);
 /*   "fp32" of runRocblas (src/rocm/rocblas.cpp:246-254, rocblas_sgemm): fp32 operands, accumulation
  *          and output, on the fp32 matrix instruction; M, N multiples of 256, K a multiple of 32;
@@ -379,7 +381,8 @@ int mi355_glu_forward(mi355_dev *dev, int type, int act, const void *X, uint64_t
  *     dG = dH * U * act'(G),  dU = dH * act(G)      (fp32, rounded to `type` for the products that follow)
  *     dX[T][D] = dG Wg + dU Wu,   dWg[F][D] = dG^T X,   dWu[F][D] = dU^T X      (fp32 sums, rounded once to `type`)
  * dX NULL, or dWg and dWu NULL: that part is left out (a frozen weight, a first layer); its operand (Wg and Wu, or X)
- * may then be NULL too.  `workspace` holds what mi355_glu_backward_workspace says, on 256 bytes.  T up to 2^25, F up to
+ * may then be NULL too.  `workspace` holds what mi355_glu_backward_workspace says (for this handle, as its
+ * tiling is set), on 256 bytes.  T up to 2^25, F up to
  * 2^24 - 64. */
 int mi355_glu_backward_workspace(mi355_dev *dev, uint32_t T, uint32_t F, uint32_t D, size_t *bytes);
 int mi355_glu_backward(mi355_dev *dev, int type, int act, const void *dH, uint64_t lddh, const void *X, uint64_t ldx,
