@@ -56,9 +56,11 @@ inline FfnProduct mi355_ffn_slices_of(const FfnProduct &p, void *workspace) {
   q.out.type = MI355_TYPE_F32;
   return q;
 }
-// Bits of mi355_dev::full_lds_allowed: three operand types with up to three kinds of product each.
-enum { kLdsFfnQuad0 = 24, kLdsFfnSmall0 = 33, kLdsFfnMid0 = 42 };
-constexpr int ffn_kind(int op, int epi) { return (op - kQuadBf16) * 3 + (epi == kEpiPartial ? 2 : epi_is_gated(epi) ? 1 : 0); }
+// Bits of mi355_dev::full_lds_allowed: the kernels of each tiling (the 256x256 one has one for each output type).
+constexpr int ffn_kind(int op, int epi, int type = 0) {
+  return op != kQuadI8 ? (op - kQuadBf16) * 3 + (epi == kEpiPartial ? 2 : epi_is_gated(epi) ? 1 : 0) : epi == kEpiPartial ? 12 : 6 + 3 * epi_is_gated(epi) + type;
+}
+enum { kLdsFfnQuad0 = 24, kLdsFfnSmall0 = 37, kLdsFfnMid0 = 50 };   // 13 each
 
 // ffn.hip: the product on the kernel that suits it, and the workspace that it can use.
 int mi355_ffn_product(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p, void *workspace, size_t workspace_bytes);
