@@ -69,7 +69,7 @@ struct Tiling {
 };
 constexpr Tiling kTilings[] = {{kOn64, MI355_GEMM_TILING_64, 64, 0.20, 0.32, 4.0, 1.0, 5.5e6},
                                {kOn128, MI355_GEMM_TILING_128, 128, 0.30, 0.47, 5.0, 0.0, 4.5e6},
-                               {kOn256, MI355_GEMM_TILING_256, 256, 0.85, 1.40, 2.0, 4.0, 4.5e6}};
+                               {kOn256, MI355_GEMM_TILING_256, 256, 0.85, 1.30, 4.0, 10.0, 4.5e6}};
 
 double count_of_cus(const mi355_dev *dev) { return dev->props.num_cus > 0 ? dev->props.num_cus : 1; }
 double columns_of_sums(int epi, uint32_t n) { return epi_is_gated(epi) ? 2.0 * n : (double)n; }
