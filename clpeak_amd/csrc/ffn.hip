@@ -139,6 +139,10 @@ int launch(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &
 
 }  // namespace
 
+bool mi355_ffn_on_256(const mi355_dev *dev, uint32_t m, uint32_t n, uint32_t k_bytes) {
+  return choose(dev, kEpiPlain, m, n, k_bytes, true).kernel == kOn256;
+}
+
 size_t mi355_ffn_workspace(const mi355_dev *dev, int epi, uint32_t m, uint32_t n, uint32_t k_bytes) {
   return division_bytes(divide(dev, epi, m, n, k_bytes, true), m, n);
 }

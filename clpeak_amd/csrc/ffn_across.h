@@ -1,0 +1,21 @@
+// ffn_across.hip: products whose sum runs over the rows of B, and of A too where that is asked for.
+#pragma once
+#include "ffn.h"
+
+// C[m][n] = sum over k of A * B[k][n], k = 0 .. 64 steps - 1, 16-bit operands, 256x256 tiles of sums.
+//   B: up to four stretches of rows, one behind the other along k, each a multiple of 64 rows.
+//   A: [m][k] (a row of k lda bytes apart from the next), or across: [k][parts x part], parts times m columns, each part
+//      padded to `part` columns (a multiple of 64); part 0 is C's, part 1 that of c2.
+// n is a multiple of 64; addresses and strides (bytes) are multiples of 16, strides at most 64 MiB.
+struct FfnAcross {
+  const uint8_t *a;
+  uint64_t lda;
+  uint32_t m, n, steps, parts, part, stretches;
+  struct Stretch {
+    const uint8_t *rows;
+    uint32_t ld, slabs;   // (slabs of 64 rows)
+  } b[4];
+  FfnOut out;             // c, ldc, type
+  void *c2;
+};
+int mi355_launch_ffn_across(mi355_dev *dev, int op, bool across_a, const char *what, const FfnAcross &p);

@@ -1,10 +1,13 @@
-// The gradients of the gated projection.  dG and dU are one elementwise pass; what follows are products whose operands
-// have the sum's index on the outside (dX sums over F, the rows of the weights; dW over T, the rows of X and of dG, dU),
-// while the product kernels want it innermost.  So the pass that makes dG and dU writes them both ways, and X and the
-// weights are turned once into the workspace: per product of 2 T F D operations a few bytes of T F + F D + T D, some
-// percent of the products' time at the sizes of a training batch.  Rows of the turned copies are padded with zeros to
-// the product kernels' 128 bytes, which is what lets T and F be anything.
+// The gradients of the gated projection.  dG and dU are one elementwise pass, the rest are products whose sums run over the
+// rows of their operands: dX over F, the rows of the weights, dW over T, the rows of X and of dG, dU.
+//
+// Products of many tiles read such operands as they are (ffn_across.hip).  The others run on the kernels that want the
+// sum's index innermost, for which the pass that makes dG and dU writes them both ways and X and the weights are turned
+// once into the workspace.  Which of the two is each product's own choice: turning costs the products of a training batch
+// (8192x8192x4096) 145 of 1640 us.  Either way the workspace's copies are padded with zeros to the kernels' 64 values of
+// the sum, which is what lets T and F be anything.
 #include "ffn.h"
+#include "ffn_across.h"
 
 namespace {
 
@@ -12,24 +15,28 @@ constexpr int kTileEdge = 64, kThreads = 256, kVec = 8;
 
 __host__ __device__ constexpr uint64_t round_up(uint64_t x, uint64_t to) { return (x + to - 1) / to * to; }
 
-// The workspace: dG | dU by rows [T][2 Fk], by columns 2 x [Fp][Tp], the weights turned [D][2 Fk], X turned [D][Tp], and what
-// the products use of it where they are cut along their sums.
+// The workspace: dG | dU by rows [Tp][2 Fk]; by columns 2 x [Fp][Tp] where dW wants that; the weights turned [D][2 Fk], or
+// their last rows 2 x [64][D]; X turned [D][Tp], or its last rows [64][D]; and what the products use of it where they are
+// cut along their sums.
 struct Plan {
-  uint64_t fk, fp, tp;                            // F padded to a row of a product, F padded to whole tiles, T padded to a row
-  uint64_t rows, cols, wt, xt, sums, bytes;       // offsets
+  uint64_t fk, fp, tp;                         // F padded to a row of a product, F padded to whole tiles, T padded to a row
+  bool dx_across, dw_across;
+  uint64_t rows, cols, w, x, sums, bytes;      // offsets
 };
 Plan plan_of(const mi355_dev *dev, uint32_t T, uint32_t F, uint32_t D) {
   Plan p;
   p.fk = round_up(F, 64);
   p.fp = round_up(F, 256);
   p.tp = T ? round_up(T, 64) : 64;
+  p.dx_across = T && mi355_ffn_on_256(dev, T, D, (uint32_t)(4 * p.fk));
+  p.dw_across = mi355_ffn_on_256(dev, F, D, (uint32_t)(2 * p.tp));
   p.rows = 0;
-  p.cols = round_up(p.rows + (uint64_t)T * 2 * p.fk * 2, 256);
-  p.wt = round_up(p.cols + 2 * p.fp * p.tp * 2, 256);
-  p.xt = round_up(p.wt + (uint64_t)D * 2 * p.fk * 2, 256);
-  p.sums = round_up(p.xt + (uint64_t)D * p.tp * 2, 256);
-  const uint64_t dx = T ? mi355_ffn_workspace(dev, kEpiPlain, T, D, (uint32_t)(4 * p.fk)) : 0;
-  const uint64_t dw = mi355_ffn_workspace(dev, kEpiPlain, F, D, (uint32_t)(2 * p.tp));
+  p.cols = round_up(p.rows + p.tp * 2 * p.fk * 2, 256);
+  p.w = round_up(p.cols + (p.dw_across ? 0 : 2 * p.fp * p.tp * 2), 256);
+  p.x = round_up(p.w + (p.dx_across ? 2 * 64 * (uint64_t)D * 2 : (uint64_t)D * 2 * p.fk * 2), 256);
+  p.sums = round_up(p.x + (p.dw_across ? 64 * (uint64_t)D * 2 : (uint64_t)D * p.tp * 2), 256);
+  const uint64_t dx = T && !p.dx_across ? mi355_ffn_workspace(dev, kEpiPlain, T, D, (uint32_t)(4 * p.fk)) : 0;
+  const uint64_t dw = p.dw_across ? 0 : mi355_ffn_workspace(dev, kEpiPlain, F, D, (uint32_t)(2 * p.tp));
   p.bytes = round_up(p.sums + (dx > dw ? dx : dw), 256);
   return p;
 }
@@ -72,12 +79,13 @@ __device__ __forceinline__ void store_column(const Tile &t, uint32_t c, uint32_t
 }
 
 // What precedes the products, all of it one launch: the workgroups are tiles of 64x64 values, first those of dG and dU, then
-// those of the matrices to be turned.
-struct Turn {               // dst[c][r] = src[r][c]: R rows of C values, rows of dst padded with zeros from R to a multiple of 64
-  const uint16_t *src;
-  uint16_t *dst;
+// those of the matrices to be turned or whose last rows are to be copied.
+struct Layout {
+  const uint16_t *src;          // R rows of C values (C a multiple of 64), ld apart
+  uint16_t *dst;                // turned: C rows of R values; otherwise R rows of C; zeros behind R, up to a multiple of 64
   uint64_t ld, ld_dst;
-  uint32_t R, tiles_c, tiles;   // C / 64 (C is a multiple of 64), tiles in all
+  uint32_t R, tiles_c, tiles;   // C / 64, tiles in all
+  bool turned;
 };
 struct Gate {
   const uint16_t *dH, *G, *U;
@@ -90,8 +98,8 @@ struct Gate {
   bool by_rows, by_columns;
 };
 
-// dG and dU of a tile: by rows (dG at column f, dU at column fk + f of a row of 2 fk; zeros from F to fk) and by columns
-// (row f of [fp][tp], dU fp rows on; zeros from T to tp).
+// dG and dU of a tile: by rows (dG at column f, dU at column fk + f of a row of 2 fk; zeros from F to fk and in the rows
+// from T to tp) and by columns (row f of [fp][tp], dU fp rows on; zeros from T to tp).
 template <int TYPE>
 __device__ __forceinline__ void gate_tile(const Gate &p, uint32_t tile, Tile &tg, Tile &tu) {
   const uint32_t f0 = tile % p.tiles_f * kTileEdge, t0 = tile / p.tiles_f * kTileEdge;
@@ -110,12 +118,13 @@ __device__ __forceinline__ void gate_tile(const Gate &p, uint32_t tile, Tile &tg
         dg.v[e] = narrow<TYPE>(d * widen<TYPE>(u.v[e]) * da);   // (past F: 0 * 0)
         du.v[e] = narrow<TYPE>(d * a);
       }
-      if (p.by_rows) {
-        uint16_t *to = p.rows + (uint64_t)t * 2u * p.fk + f;
-        *reinterpret_cast<uint4 *>(to) = __builtin_bit_cast(uint4, dg);
-        *reinterpret_cast<uint4 *>(to + p.fk) = __builtin_bit_cast(uint4, du);
-      }
     }
+    if (p.by_rows) {
+      uint16_t *to = p.rows + (uint64_t)t * 2u * p.fk + f;
+      *reinterpret_cast<uint4 *>(to) = __builtin_bit_cast(uint4, dg);
+      *reinterpret_cast<uint4 *>(to + p.fk) = __builtin_bit_cast(uint4, du);
+    }
+    if (!p.by_columns) continue;
 #pragma unroll
     for (int e = 0; e < kVec; e++) {
       tg.at[r][c + e] = dg.v[e];
@@ -134,39 +143,59 @@ __device__ __forceinline__ void gate_tile(const Gate &p, uint32_t tile, Tile &tg
   }
 }
 
-__device__ __forceinline__ void turn_tile(const Turn &p, uint32_t number, Tile &tile) {
+__device__ __forceinline__ void layout_tile(const Layout &p, uint32_t number, Tile &tile) {
   const uint32_t c0 = number % p.tiles_c * kTileEdge, r0 = number / p.tiles_c * kTileEdge;
   const uint32_t c = threadIdx.x % 8u * kVec;
 #pragma unroll
   for (uint32_t r = threadIdx.x / 8u; r < kTileEdge; r += kThreads / 8) {
     Vec8 x{};
     if (r0 + r < p.R) x = __builtin_bit_cast(Vec8, *reinterpret_cast<const uint4 *>(p.src + (uint64_t)(r0 + r) * p.ld + c0 + c));
+    if (!p.turned) {
+      *reinterpret_cast<uint4 *>(p.dst + (uint64_t)(r0 + r) * p.ld_dst + c0 + c) = __builtin_bit_cast(uint4, x);
+      continue;
+    }
 #pragma unroll
     for (int e = 0; e < kVec; e++) tile.at[r][c + e] = x.v[e];
   }
+  if (!p.turned) return;
   __syncthreads();
 #pragma unroll
   for (uint32_t r = threadIdx.x / 8u; r < kTileEdge; r += kThreads / 8) store_column(tile, r, c, p.dst + (uint64_t)(c0 + r) * p.ld_dst + r0 + c);
 }
 
 template <int TYPE>
-__global__ void __launch_bounds__(kThreads) glu_backward_prepare_kernel(Gate gate, Turn t0, Turn t1, Turn t2) {
+__global__ void __launch_bounds__(kThreads) glu_backward_prepare_kernel(Gate gate, Layout l0, Layout l1, Layout l2) {
   __shared__ Tile a, b;
   uint32_t i = blockIdx.x;
   if (i < gate.tiles) return gate_tile<TYPE>(gate, i, a, b);
   i -= gate.tiles;
-  if (i < t0.tiles) return turn_tile(t0, i, a);
-  i -= t0.tiles;
-  if (i < t1.tiles) return turn_tile(t1, i, a);
-  turn_tile(t2, i - t1.tiles, a);
+  if (i < l0.tiles) return layout_tile(l0, i, a);
+  i -= l0.tiles;
+  if (i < l1.tiles) return layout_tile(l1, i, a);
+  layout_tile(l2, i - l1.tiles, a);
 }
 
-Turn turn(const void *src, uint64_t ld, uint8_t *dst, uint64_t ld_dst, uint32_t R, uint64_t rp, uint32_t C) {
-  Turn t;
+Layout turned(const void *src, uint64_t ld, uint8_t *dst, uint64_t ld_dst, uint32_t R, uint64_t rp, uint32_t C) {
+  Layout t;
   t.src = (const uint16_t *)src; t.dst = (uint16_t *)dst;
   t.ld = ld; t.ld_dst = ld_dst;
   t.R = R; t.tiles_c = C / 64u; t.tiles = (uint32_t)((uint64_t)t.tiles_c * (rp / 64u));
+  t.turned = true;
   return t;
+}
+// The rows of [R][C] behind the last whole 64 (R = 0: none, 64 rows of zeros; no such rows: nothing to do).
+Layout last_rows(const void *src, uint64_t ld, uint8_t *dst, uint32_t R, uint32_t C) {
+  Layout t{};
+  if (R > 0 && R % 64u == 0u) return t;
+  t.src = (const uint16_t *)src + (uint64_t)(R / 64u * 64u) * ld; t.dst = (uint16_t *)dst;
+  t.ld = ld; t.ld_dst = C;
+  t.R = R % 64u; t.tiles_c = t.tiles = C / 64u;
+  return t;
+}
+// The same rows as stretches of B: the whole 64s where they are, then the copy.
+void add_stretches(FfnAcross &q, const void *src, uint64_t ld, const uint8_t *copy, uint32_t R, uint32_t C) {
+  if (R >= 64u) q.b[q.stretches++] = {(const uint8_t *)src, (uint32_t)(ld * 2u), R / 64u};
+  if (R == 0 || R % 64u) q.b[q.stretches++] = {copy, C * 2u, 1};
 }
 
 }  // namespace
@@ -186,35 +215,54 @@ int mi355_launch_glu_backward(mi355_dev *dev, int type, int act, const void *dH,
   const int op = type == MI355_TYPE_BF16 ? kQuadBf16 : kQuadF16;
   const uint64_t tiles = p.fk / 64u * (p.tp / 64u) + (uint64_t)(D / 64u) * (2u * (p.fk / 64u) + p.tp / 64u);
   MI355_REQUIRE(dev, tiles <= 0x7fffffffull, "glu_backward: T = %u, F = %u, D = %u are more than one launch takes", T, F, D);
+  uint8_t *const wu_copy = ws + p.w + (p.dx_across ? 64 * (uint64_t)D * 2 : p.fk * 2);
   Gate gate;
   gate.dH = (const uint16_t *)dH; gate.G = (const uint16_t *)G; gate.U = (const uint16_t *)U;
   gate.lddh = lddh; gate.ldg = ldg;
   gate.rows = (uint16_t *)(ws + p.rows); gate.cols = (uint16_t *)(ws + p.cols);
   gate.T = T; gate.F = F; gate.fk = (uint32_t)p.fk; gate.fp = p.fp; gate.tp = (uint32_t)p.tp; gate.act = act;
   gate.tiles_f = (uint32_t)(p.fk / 64u); gate.tiles = (uint32_t)(p.fk / 64u * (p.tp / 64u));
-  gate.by_rows = dX != nullptr; gate.by_columns = dWg != nullptr;
-  Turn wg{}, wu{}, x{};
-  if (dX) {
-    wg = turn(Wg, ldw, ws + p.wt, 2 * p.fk, F, p.fk, D);
-    wu = turn(Wu, ldw, ws + p.wt + p.fk * 2, 2 * p.fk, F, p.fk, D);
+  gate.by_rows = dX || (dWg && p.dw_across); gate.by_columns = dWg && !p.dw_across;
+  Layout wg{}, wu{}, x{};
+  if (dX && p.dx_across) {
+    wg = last_rows(Wg, ldw, ws + p.w, F, D);
+    wu = last_rows(Wu, ldw, wu_copy, F, D);
+  } else if (dX) {
+    wg = turned(Wg, ldw, ws + p.w, 2 * p.fk, F, p.fk, D);
+    wu = turned(Wu, ldw, wu_copy, 2 * p.fk, F, p.fk, D);
   }
-  if (dWg) x = turn(X, ldx, ws + p.xt, p.tp, T, p.tp, D);
+  if (dWg) x = p.dw_across ? last_rows(X, ldx, ws + p.x, T, D) : turned(X, ldx, ws + p.x, p.tp, T, p.tp, D);
   const uint32_t grid = gate.tiles + wg.tiles + wu.tiles + x.tiles;
   if (type == MI355_TYPE_BF16) glu_backward_prepare_kernel<MI355_TYPE_BF16><<<grid, kThreads, 0, dev->stream>>>(gate, wg, wu, x);
   else glu_backward_prepare_kernel<MI355_TYPE_F16><<<grid, kThreads, 0, dev->stream>>>(gate, wg, wu, x);
   MI355_LAUNCH_CHECK(dev, "glu_backward (prepare)");
+  FfnAcross c{};
+  c.a = ws + p.rows; c.lda = 4 * p.fk;
+  c.n = D;
+  c.out.type = type;
   FfnProduct q{};
   q.out.type = type;
-  if (dX) {
+  if (dX && p.dx_across) {
+    c.m = T; c.steps = (uint32_t)(2 * p.fk / 64u); c.parts = 1; c.stretches = 0;
+    add_stretches(c, Wg, ldw, ws + p.w, F, D);
+    add_stretches(c, Wu, ldw, wu_copy, F, D);
+    c.out.c = dX; c.out.ldc = lddx;
+    if (int rc = mi355_launch_ffn_across(dev, op, false, "glu_backward (dX)", c)) return rc;
+  } else if (dX) {
     q.a = ws + p.rows; q.lda = 4 * p.fk;
-    q.b = ws + p.wt; q.ldb = 4 * p.fk;
+    q.b = ws + p.w; q.ldb = 4 * p.fk;
     q.m = T; q.n = D; q.k_bytes = (uint32_t)(4 * p.fk);
     q.out.c = dX; q.out.ldc = lddx;
     if (int rc = mi355_ffn_product(dev, op, kEpiPlain, "glu_backward (dX)", q, ws + p.sums, p.bytes - p.sums)) return rc;
   }
-  if (dWg) {
+  if (dWg && p.dw_across) {
+    c.m = F; c.steps = (uint32_t)(p.tp / 64u); c.parts = 2; c.part = (uint32_t)p.fk; c.stretches = 0;
+    add_stretches(c, X, ldx, ws + p.x, T, D);
+    c.out.c = dWg; c.c2 = dWu; c.out.ldc = lddw;
+    if (int rc = mi355_launch_ffn_across(dev, op, true, "glu_backward (dW)", c)) return rc;
+  } else if (dWg) {
     q.lda = q.ldb = 2 * p.tp;
-    q.b = ws + p.xt;
+    q.b = ws + p.x;
     q.m = F; q.n = D; q.k_bytes = (uint32_t)(2 * p.tp);
     q.out.ldc = lddw;
     for (int half = 0; half < 2; half++) {
