@@ -65,8 +65,7 @@ enum { kLdsFfnQuad0 = 24, kLdsFfnSmall0 = 37, kLdsFfnMid0 = 50 };   // 13 each
 // ffn.hip: the product on the kernel that suits it, and the workspace that it can use.
 int mi355_ffn_product(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p, void *workspace, size_t workspace_bytes);
 size_t mi355_ffn_workspace(const mi355_dev *dev, int epi, uint32_t m, uint32_t n, uint32_t k_bytes);
-// Whether a plain product of that size is one for 256x256 tiles.
-bool mi355_ffn_on_256(const mi355_dev *dev, uint32_t m, uint32_t n, uint32_t k_bytes);
+double mi355_ffn_expected_us(const mi355_dev *dev, int epi, uint32_t m, uint32_t n, uint32_t k_bytes);
 
 // ffn_backward.hip (arguments checked by the caller).
 int mi355_glu_backward_limits(mi355_dev *dev, const char *what, uint32_t T, uint32_t F);

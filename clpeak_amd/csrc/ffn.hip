@@ -1,5 +1,6 @@
 // The entry points of the feed-forward products: their checks, and which kernel a product runs on.
 #include "ffn.h"
+#include "ffn_across.h"
 #include <algorithm>
 #include <cmath>
 
@@ -97,6 +98,7 @@ Choice choose(const mi355_dev *dev, int epi, uint32_t m, uint32_t n, uint32_t k_
   }
   for (const Tiling &t : kTilings) {
     if (pin != MI355_GEMM_TILING_AUTO && pin != t.pin) continue;
+    if (epi == kEpiPlain && t.kernel == kOn256) continue;   // (those are ffn_across.hip's)
     const uint32_t most = can_slice && !epi_is_gated(epi) && t.kernel != kOn256 ? 16 : 1;
     for (uint32_t s = 1; s <= most && (s == 1 || s * 4u <= k_bytes / 128u); s++) take(t.kernel, s, tiling_us(t, cus, m, n, sums_n, k_bytes, s));
   }
@@ -107,10 +109,12 @@ Choice choose(const mi355_dev *dev, int epi, uint32_t m, uint32_t n, uint32_t k_
 struct Division {
   Choice whole, rest;
   uint32_t main_rows = 0;
+  double us = 0.0;
 };
 Division divide(const mi355_dev *dev, int epi, uint32_t m, uint32_t n, uint32_t k_bytes, bool can_slice) {
   Division d;
   d.whole = choose(dev, epi, m, n, k_bytes, can_slice);
+  d.us = d.whole.us;
   if (d.whole.kernel != kOn256 || dev->gemm_tiling != MI355_GEMM_TILING_AUTO) return d;
   const double cus = count_of_cus(dev), sums_n = columns_of_sums(epi, n), tiles_n = std::ceil(sums_n / 256.0);
   const double rounds = std::ceil(std::ceil(m / 256.0) * tiles_n / cus);
@@ -119,7 +123,7 @@ Division divide(const mi355_dev *dev, int epi, uint32_t m, uint32_t n, uint32_t 
   const uint32_t main_rows = (uint32_t)rows;
   const Choice rest = choose(dev, epi, m - main_rows, n, k_bytes, can_slice);
   const double us = tiling_us(kTilings[2], cus, main_rows, n, sums_n, k_bytes, 1) + rest.us;
-  if (us < d.whole.us) { d.main_rows = main_rows; d.rest = rest; d.whole.slices = 1; }
+  if (us < d.us) { d.main_rows = main_rows; d.rest = rest; d.us = us; }
   return d;
 }
 
@@ -139,8 +143,33 @@ int launch(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &
 
 }  // namespace
 
-bool mi355_ffn_on_256(const mi355_dev *dev, uint32_t m, uint32_t n, uint32_t k_bytes) {
-  return choose(dev, kEpiPlain, m, n, k_bytes, true).kernel == kOn256;
+double mi355_ffn_expected_us(const mi355_dev *dev, int epi, uint32_t m, uint32_t n, uint32_t k_bytes) {
+  return divide(dev, epi, m, n, k_bytes, true).us;
+}
+
+AcrossChoice mi355_choose_ffn_across(const mi355_dev *dev, uint32_t m, uint32_t parts, uint32_t n, uint32_t steps) {
+  const double cus = count_of_cus(dev);
+  const Tiling &t = kTilings[2];
+  auto best = [&](uint32_t rows, uint32_t &slices) {
+    double least = 1e30;
+    for (uint32_t s = 1; s <= 16u && (s == 1 || s * 4u <= steps); s++) {
+      // (the parts' tiles side by side; rows of a tile that do not exist cost as much as others, but not the join)
+      const double all = parts * std::ceil(rows / 256.0) * 256.0;
+      const double us = tiling_us(t, cus, (uint32_t)all, n, n, steps * 128u, s) - (s > 1 ? (all - parts * (double)rows) * n * (s * 8.0 + 2.0) / 4e6 : 0.0);
+      if (us < least) { least = us; slices = s; }
+    }
+    return least;
+  };
+  AcrossChoice c{0, 1, 1, 0.0};
+  c.us = best(m, c.slices);
+  const double tiles_n = std::ceil(n / 256.0), rounds = std::ceil(std::ceil(m / 256.0) * tiles_n / cus);
+  const double rows = std::floor((rounds - 1.0) * cus / tiles_n) * 256.0;
+  if (parts == 1 && rows >= 256.0 && rows < m) {
+    uint32_t main_slices = 1, rest_slices = 1;
+    const double us = best((uint32_t)rows, main_slices) + best(m - (uint32_t)rows, rest_slices);
+    if (us < c.us) c = {(uint32_t)rows, main_slices, rest_slices, us};
+  }
+  return c;
 }
 
 size_t mi355_ffn_workspace(const mi355_dev *dev, int epi, uint32_t m, uint32_t n, uint32_t k_bytes) {

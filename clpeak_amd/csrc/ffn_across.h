@@ -18,4 +18,13 @@ struct FfnAcross {
   FfnOut out;             // c, ldc, type
   void *c2;
 };
-int mi355_launch_ffn_across(mi355_dev *dev, int op, bool across_a, const char *what, const FfnAcross &p);
+// slices > 1: the sum is cut into so many, `workspace` holds slices x parts matrices of m rows of n 32-bit sums, on 16 bytes.
+int mi355_launch_ffn_across(mi355_dev *dev, int op, bool across_a, const char *what, const FfnAcross &p, uint32_t slices, uint8_t *workspace);
+
+// How such a product is best launched (ffn.hip), and the time expected of it: the rows behind main_rows (if that is not 0)
+// are a launch of their own; each launch in slices.
+struct AcrossChoice {
+  uint32_t main_rows, slices, rest_slices;
+  double us;
+};
+AcrossChoice mi355_choose_ffn_across(const mi355_dev *dev, uint32_t m, uint32_t parts, uint32_t n, uint32_t steps);

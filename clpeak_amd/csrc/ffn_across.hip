@@ -124,14 +124,17 @@ __device__ __forceinline__ void across_step(std::integer_sequence<int, Ps...>, A
 }
 
 // ACROSS_A: A is [k][columns], in parts of p.part columns each (a product for each, B shared); otherwise [rows][k].
-template <int OP, bool ACROSS_A, int TYPE>
+// Slice blockIdx.y of gridDim.y of the sum (kEpiPartial: the sums go to p.out.c, p.c2 as matrix number blockIdx.y there).
+template <int OP, bool ACROSS_A, int EPI, int TYPE>
 __global__ void __launch_bounds__(kQuadThreads) ffn_across_kernel(FfnAcross p, uint32_t tiles_m, uint32_t tiles_n) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const uint32_t tid = threadIdx.x, lane = tid % 64;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const uint32_t wm = wave / 2, wn = wave % 2;
   const TileGrid grid = tiles_of_workgroup(tiles_m, tiles_n);
-  const uint32_t steps = p.steps, lda = (uint32_t)p.lda;
+  const uint32_t k0 = EPI == kEpiPartial ? (uint32_t)((uint64_t)p.steps * blockIdx.y / gridDim.y) : 0u;
+  const uint32_t steps = EPI == kEpiPartial ? (uint32_t)((uint64_t)p.steps * (blockIdx.y + 1u) / gridDim.y) - k0 : p.steps;
+  const uint32_t lda = (uint32_t)p.lda;
   const uint32_t lds_base = (uint32_t)(uintptr_t)lds;
   const uint32_t tiles_part = ACROSS_A ? tiles_m / p.parts : tiles_m;
 
@@ -159,18 +162,19 @@ __global__ void __launch_bounds__(kQuadThreads) ffn_across_kernel(FfnAcross p, u
   auto place = [&](uint32_t rnd, uint32_t pos) __attribute__((always_inline)) {   // the stream stands on slab `pos` of the tile of round `rnd`
     uint32_t tm, tn;
     tile_at(grid, rnd, tm, tn);
+    const uint32_t slab = k0 + pos;
     if constexpr (ACROSS_A) {
       const uint32_t part = tm / tiles_part, col0 = (tm - part * tiles_part) * 256u;
-      w.ga = in_scalars((uint64_t)(uintptr_t)(p.a + (uint64_t)part * p.part * 2u + ((uint64_t)pos * 64u + wave * 16u) * lda));
+      w.ga = in_scalars((uint64_t)(uintptr_t)(p.a + (uint64_t)part * p.part * 2u + ((uint64_t)slab * 64u + wave * 16u) * lda));
 #pragma unroll
       for (uint32_t q = 0; q < 8; q++) w.voff[q] = (2u * q + lane / 32u) * lda + 2u * min(col0 + across_column(q), p.part - 8u);
     } else {
       const uint32_t a_row = min(tm * 256u + wave * 64u, p.m - 1u);
-      w.ga = in_scalars((uint64_t)(uintptr_t)(p.a + (uint64_t)a_row * lda + (uint64_t)pos * kRowBytes));
+      w.ga = in_scalars((uint64_t)(uintptr_t)(p.a + (uint64_t)a_row * lda + (uint64_t)slab * kRowBytes));
 #pragma unroll
       for (uint32_t q = 0; q < 8; q++) w.voff[q] = min(lane / 8u + 8u * q, p.m - 1u - a_row) * lda + chunk;
     }
-    uint32_t at = pos, slabs = p.b[0].slabs, ldb = p.b[0].ld;
+    uint32_t at = slab, slabs = p.b[0].slabs, ldb = p.b[0].ld;
     const uint8_t *rows = p.b[0].rows;
 #pragma unroll
     for (uint32_t s = 1; s < 4; s++) {   // (no index that varies: the addresses have to stay in scalar registers)
@@ -180,7 +184,7 @@ __global__ void __launch_bounds__(kQuadThreads) ffn_across_kernel(FfnAcross p, u
       ldb = on ? p.b[s].ld : ldb;
       slabs = on ? p.b[s].slabs : slabs;
     }
-    stretch_left = slabs - at;
+    stretch_left = min(slabs - at, steps - pos);   // (a slice may end inside a stretch)
     w.gb = in_scalars((uint64_t)(uintptr_t)(rows + ((uint64_t)at * 64u + wave * 16u) * ldb));
     w.step_b = 64ull * ldb;
 #pragma unroll
@@ -252,7 +256,8 @@ __global__ void __launch_bounds__(kQuadThreads) ffn_across_kernel(FfnAcross p, u
         row_tile = tm - part * tiles_part;
         if (part) o.out.c = p.c2;
       }
-      Finish<OP, kEpiPlain, TYPE>{o, row_tile * 256u + wm * 128u + lane % 16u, tn * 256u + wn * 128u, lane}.run();
+      if constexpr (EPI == kEpiPartial) o.out.c = static_cast<float *>(o.out.c) + (uint64_t)blockIdx.y * p.m * p.out.ldc;
+      Finish<OP, EPI, TYPE>{o, row_tile * 256u + wm * 128u + lane % 16u, tn * 256u + wn * 128u, lane}.run();
       left = steps;
       w.first = 1;
       done = ++round == grid.mine;
@@ -271,20 +276,39 @@ __global__ void __launch_bounds__(kQuadThreads) ffn_across_kernel(FfnAcross p, u
   MI355_DRAIN_RING();
 }
 
-template <int OP, bool ACROSS_A, int TYPE>
-int launch(mi355_dev *dev, const char *what, const FfnAcross &p, int bit) {
-  if (int rc = allow_full_lds(dev, &ffn_across_kernel<OP, ACROSS_A, TYPE>, bit)) return rc;
+template <int OP, bool ACROSS_A, int EPI, int TYPE>
+int launch(mi355_dev *dev, const char *what, const FfnAcross &p, uint32_t slices) {
+  // bits 1 to 8 of mi355_dev::full_lds_allowed
+  if (int rc = allow_full_lds(dev, &ffn_across_kernel<OP, ACROSS_A, EPI, TYPE>, 1 + (OP == kQuadF16) * 4 + ACROSS_A * 2 + (EPI == kEpiPartial))) return rc;
   const uint64_t tiles_m = (uint64_t)p.parts * ((p.m + 255u) / 256u), tiles_n = (p.n + 255u) / 256u;
   MI355_REQUIRE(dev, tiles_m * tiles_n <= 0x3fffffffull, "%s: %u x %u outputs are more than one launch takes", what, p.m, p.n);
-  ffn_across_kernel<OP, ACROSS_A, TYPE><<<gemm_workgroups(dev, (uint32_t)(tiles_m * tiles_n)), kQuadThreads, kRingBytes, dev->stream>>>(p, (uint32_t)tiles_m, (uint32_t)tiles_n);
+  const dim3 grid(slices > 1 ? (uint32_t)(tiles_m * tiles_n) : gemm_workgroups(dev, (uint32_t)(tiles_m * tiles_n)), slices);
+  ffn_across_kernel<OP, ACROSS_A, EPI, TYPE><<<grid, kQuadThreads, kRingBytes, dev->stream>>>(p, (uint32_t)tiles_m, (uint32_t)tiles_n);
   MI355_LAUNCH_CHECK(dev, what);
+  return MI355_OK;
+}
+template <int OP, bool ACROSS_A, int TYPE>
+int launch_slices(mi355_dev *dev, const char *what, const FfnAcross &p, uint32_t slices, uint8_t *workspace) {
+  if (slices <= 1) return launch<OP, ACROSS_A, kEpiPlain, TYPE>(dev, what, p, 1);
+  const uint64_t part = slices * (uint64_t)p.m * p.n * 4u;
+  FfnAcross q = p;
+  q.out.c = workspace;
+  q.c2 = workspace + part;
+  q.out.ldc = p.n;
+  if (int rc = launch<OP, ACROSS_A, kEpiPartial, MI355_TYPE_F32>(dev, what, q, slices)) return rc;
+  for (uint32_t i = 0; i < p.parts; i++) {
+    FfnProduct o{};
+    o.m = p.m; o.n = p.n;
+    o.out = p.out;
+    if (i) o.out.c = p.c2;
+    if (int rc = mi355_launch_ffn_join(dev, OP, kEpiPlain, what, o, slices, workspace + i * part)) return rc;
+  }
   return MI355_OK;
 }
 
 }  // namespace
 
-int mi355_launch_ffn_across(mi355_dev *dev, int op, bool across_a, const char *what, const FfnAcross &p) {
-  enum { kLdsAcross0 = 1 };   // bits of mi355_dev::full_lds_allowed: 1 to 4
-  if (op == kQuadBf16) return across_a ? launch<kQuadBf16, true, MI355_TYPE_BF16>(dev, what, p, kLdsAcross0) : launch<kQuadBf16, false, MI355_TYPE_BF16>(dev, what, p, kLdsAcross0 + 1);
-  return across_a ? launch<kQuadF16, true, MI355_TYPE_F16>(dev, what, p, kLdsAcross0 + 2) : launch<kQuadF16, false, MI355_TYPE_F16>(dev, what, p, kLdsAcross0 + 3);
+int mi355_launch_ffn_across(mi355_dev *dev, int op, bool across_a, const char *what, const FfnAcross &p, uint32_t slices, uint8_t *workspace) {
+  if (op == kQuadBf16) return across_a ? launch_slices<kQuadBf16, true, MI355_TYPE_BF16>(dev, what, p, slices, workspace) : launch_slices<kQuadBf16, false, MI355_TYPE_BF16>(dev, what, p, slices, workspace);
+  return across_a ? launch_slices<kQuadF16, true, MI355_TYPE_F16>(dev, what, p, slices, workspace) : launch_slices<kQuadF16, false, MI355_TYPE_F16>(dev, what, p, slices, workspace);
 }

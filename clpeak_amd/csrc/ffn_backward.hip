@@ -3,11 +3,12 @@
 //
 // Products of many tiles read such operands as they are (ffn_across.hip).  The others run on the kernels that want the
 // sum's index innermost, for which the pass that makes dG and dU writes them both ways and X and the weights are turned
-// once into the workspace.  Which of the two is each product's own choice: turning costs the products of a training batch
-// (8192x8192x4096) 145 of 1640 us.  Either way the workspace's copies are padded with zeros to the kernels' 64 values of
+// once into the workspace.  Which of the two goes by the expected times, for each product by itself: turning costs the
+// products of a training batch (8192x8192x4096) 106 of 1585 us.  Either way the workspace's copies are padded with zeros to the kernels' 64 values of
 // the sum, which is what lets T and F be anything.
 #include "ffn.h"
 #include "ffn_across.h"
+#include <algorithm>
 
 namespace {
 
@@ -21,6 +22,7 @@ __host__ __device__ constexpr uint64_t round_up(uint64_t x, uint64_t to) { retur
 struct Plan {
   uint64_t fk, fp, tp;                         // F padded to a row of a product, F padded to whole tiles, T padded to a row
   bool dx_across, dw_across;
+  AcrossChoice dx, dw;
   uint64_t rows, cols, w, x, sums, bytes;      // offsets
 };
 Plan plan_of(const mi355_dev *dev, uint32_t T, uint32_t F, uint32_t D) {
@@ -28,15 +30,28 @@ Plan plan_of(const mi355_dev *dev, uint32_t T, uint32_t F, uint32_t D) {
   p.fk = round_up(F, 64);
   p.fp = round_up(F, 256);
   p.tp = T ? round_up(T, 64) : 64;
-  p.dx_across = T && mi355_ffn_on_256(dev, T, D, (uint32_t)(4 * p.fk));
-  p.dw_across = mi355_ffn_on_256(dev, F, D, (uint32_t)(2 * p.tp));
+  // across, or turned at the price of the copies' way through memory (4.5 bytes a picosecond)
+  const uint32_t dx_k = (uint32_t)(4 * p.fk), dw_k = (uint32_t)(2 * p.tp);
+  p.dx = mi355_choose_ffn_across(dev, T ? T : 1, 1, D, dx_k / 128u);
+  p.dw = mi355_choose_ffn_across(dev, F, 2, D, dw_k / 128u);
+  const double turn_dx = 8.0 * F * D / 4.5e6, turn_dw = (4.0 * T * F + 4.0 * T * D) / 4.5e6;
+  p.dx_across = T && p.dx.us < mi355_ffn_expected_us(dev, kEpiPlain, T, D, dx_k) + turn_dx;
+  p.dw_across = p.dw.us < 2.0 * mi355_ffn_expected_us(dev, kEpiPlain, F, D, dw_k) + turn_dw;
+  if (dev->gemm_tiling != MI355_GEMM_TILING_AUTO) {
+    p.dw_across = dev->gemm_tiling == MI355_GEMM_TILING_256;
+    p.dx_across = T && p.dw_across;
+  }
   p.rows = 0;
   p.cols = round_up(p.rows + p.tp * 2 * p.fk * 2, 256);
   p.w = round_up(p.cols + (p.dw_across ? 0 : 2 * p.fp * p.tp * 2), 256);
   p.x = round_up(p.w + (p.dx_across ? 2 * 64 * (uint64_t)D * 2 : (uint64_t)D * 2 * p.fk * 2), 256);
   p.sums = round_up(p.x + (p.dw_across ? 64 * (uint64_t)D * 2 : (uint64_t)D * p.tp * 2), 256);
-  const uint64_t dx = T && !p.dx_across ? mi355_ffn_workspace(dev, kEpiPlain, T, D, (uint32_t)(4 * p.fk)) : 0;
-  const uint64_t dw = p.dw_across ? 0 : mi355_ffn_workspace(dev, kEpiPlain, F, D, (uint32_t)(2 * p.tp));
+  auto sums = [&](uint32_t slices, uint64_t rows) { return slices > 1 ? slices * rows * D * 4 : 0; };
+  uint64_t dx = 0, dw = 0;
+  if (p.dx_across) dx = std::max(sums(p.dx.slices, p.dx.main_rows ? p.dx.main_rows : T), sums(p.dx.rest_slices, T - p.dx.main_rows));
+  else if (T) dx = mi355_ffn_workspace(dev, kEpiPlain, T, D, dx_k);
+  if (p.dw_across) dw = sums(p.dw.slices, 2 * (uint64_t)F);
+  else dw = mi355_ffn_workspace(dev, kEpiPlain, F, D, dw_k);
   p.bytes = round_up(p.sums + (dx > dw ? dx : dw), 256);
   return p;
 }
@@ -243,11 +258,17 @@ int mi355_launch_glu_backward(mi355_dev *dev, int type, int act, const void *dH,
   FfnProduct q{};
   q.out.type = type;
   if (dX && p.dx_across) {
-    c.m = T; c.steps = (uint32_t)(2 * p.fk / 64u); c.parts = 1; c.stretches = 0;
+    c.m = p.dx.main_rows ? p.dx.main_rows : T; c.steps = (uint32_t)(2 * p.fk / 64u); c.parts = 1; c.stretches = 0;
     add_stretches(c, Wg, ldw, ws + p.w, F, D);
     add_stretches(c, Wu, ldw, wu_copy, F, D);
     c.out.c = dX; c.out.ldc = lddx;
-    if (int rc = mi355_launch_ffn_across(dev, op, false, "glu_backward (dX)", c)) return rc;
+    if (int rc = mi355_launch_ffn_across(dev, op, false, "glu_backward (dX)", c, p.dx.slices, ws + p.sums)) return rc;
+    if (p.dx.main_rows) {
+      c.a += p.dx.main_rows * c.lda;
+      c.m = T - p.dx.main_rows;
+      c.out.c = (uint16_t *)dX + p.dx.main_rows * lddx;
+      if (int rc = mi355_launch_ffn_across(dev, op, false, "glu_backward (dX)", c, p.dx.rest_slices, ws + p.sums)) return rc;
+    }
   } else if (dX) {
     q.a = ws + p.rows; q.lda = 4 * p.fk;
     q.b = ws + p.w; q.ldb = 4 * p.fk;
@@ -256,10 +277,11 @@ int mi355_launch_glu_backward(mi355_dev *dev, int type, int act, const void *dH,
     if (int rc = mi355_ffn_product(dev, op, kEpiPlain, "glu_backward (dX)", q, ws + p.sums, p.bytes - p.sums)) return rc;
   }
   if (dWg && p.dw_across) {
+    c.a = ws + p.rows;
     c.m = F; c.steps = (uint32_t)(p.tp / 64u); c.parts = 2; c.part = (uint32_t)p.fk; c.stretches = 0;
     add_stretches(c, X, ldx, ws + p.x, T, D);
     c.out.c = dWg; c.c2 = dWu; c.out.ldc = lddw;
-    if (int rc = mi355_launch_ffn_across(dev, op, true, "glu_backward (dW)", c)) return rc;
+    if (int rc = mi355_launch_ffn_across(dev, op, true, "glu_backward (dW)", c, p.dw.slices, ws + p.sums)) return rc;
   } else if (dWg) {
     q.lda = q.ldb = 2 * p.tp;
     q.b = ws + p.x;

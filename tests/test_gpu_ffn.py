@@ -243,6 +243,23 @@ def test_glu_backward(tiled, type, T, F, D):
     assert bool((room[ws.data_ptr() - room.data_ptr() + n:] == 0xFF).all())
 
 
+@pytest.mark.parametrize("T, F, D", [(4200, 320, 4096), (600, 4096, 512), (2048, 2752, 1024), (130, 8192, 256), (3000, 70, 2048)])
+def test_glu_backward_larger(tiled, T, F, D):
+    """Sizes at which the products are cut along their sums, go round the CUs more than once, and have rows left over for a
+    launch of their own."""
+    test_glu_backward(tiled, capi.TYPE_BF16, T, F, D)
+
+
+@pytest.mark.parametrize("T, F, D", [(4200, 1100, 128), (2176, 2100, 64), (513, 20000, 64)])
+def test_glu_forward_larger(tiled, T, F, D):
+    """More tiles than CUs, and rows left over for a launch of their own."""
+    test_glu_forward(tiled, capi.TYPE_F16, T, F, D)
+
+
+def test_nothing_is_summed_over_no_rows_on_any_tiling(tiled):
+    test_glu_backward_without_rows_clears_the_weights_gradients(tiled)
+
+
 def test_glu_backward_without_rows_clears_the_weights_gradients(dv):
     F, D = 100, 128
     n = dv.glu_backward_workspace(0, F, D)
