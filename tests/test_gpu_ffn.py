@@ -662,3 +662,128 @@ def test_quantize_every_value_against_every_mantissa(dv, type):
     dv.quantize_i8(type, x, K, q, K, s, M, K, K)
     rq, rs = quantized(x)
     assert torch.equal(q.double(), rq) and torch.equal(s, rs)
+
+
+# ---- where offsets, values and calls are unusual ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("M", [3, 70])
+def test_operands_whose_rows_are_far_apart(tiled, M):
+    """Rows 64 MiB apart, the most that is taken: the last of 70 is more than 4 GiB behind the first."""
+    dv = tiled
+    N, K, far = 70, 256, 64 << 20
+    g = gen(M)
+    a, b, b2 = (torch.randint(-128, 128, (r, K), generator=g, device="cuda").to(torch.int8) for r in (M, N, N))
+    big = torch.empty((N - 1) * far + 2 * K, dtype=torch.int8, device="cuda")
+    rows, rows2 = big.as_strided((N, K), (far, 1)), big.as_strided((N, K), (far, 1), K)
+    rows.copy_(b)
+    rows2.copy_(b2)
+    one = torch.ones(N, device="cuda")
+    c = torch.empty(M, N, device="cuda")
+    dv.gemm_i8_scaled(a, K, rows, far, one, one, None, capi.TYPE_F32, c, N, M, N, K)
+    assert torch.equal(c.double(), a.double() @ b.double().T)
+    dv.glu_i8(capi.GLU_RELU, a, K, rows, rows2, far, one, one, one, capi.TYPE_F32, c, N, M, N, K)
+    want = (a.double() @ b.double().T).clamp(min=0) * (a.double() @ b2.double().T)
+    within(c, want, 4 * E * want.abs(), torch.float32)
+    dv.gemm_i8_scaled(rows, far, a, K, one, one, None, capi.TYPE_F32, c.view(N, M), M, N, M, K)
+    assert torch.equal(c.view(N, M).double(), b.double() @ a.double().T)
+    D = 64
+    x = (torch.randn(N, D, generator=g, device="cuda")).bfloat16()
+    w = (torch.randn(2, M, D, generator=g, device="cuda") / 8).bfloat16()
+    xs = big.view(torch.bfloat16).as_strided((N, D), (far // 2, 1))
+    xs.copy_(x)
+    h, G, U = (torch.empty(N, M, dtype=torch.bfloat16, device="cuda") for _ in range(3))
+    dv.glu_forward(capi.TYPE_BF16, capi.GLU_RELU, xs, far // 2, w[0], w[1], D, h, M, G, U, M, N, M, D)
+    g64, u64 = x.double() @ w[0].double().T, x.double() @ w[1].double().T
+    s = 2 * D * E * (x.double().abs() @ w.double().abs().amax(0).T)
+    within(h, g64.clamp(min=0) * u64, s * (g64.abs() + u64.abs()), torch.bfloat16)
+    n = dv.glu_backward_workspace(N, M, D)
+    dw = torch.empty(2, M, D, dtype=torch.bfloat16, device="cuda")
+    dv.glu_backward(capi.TYPE_BF16, capi.GLU_RELU, h, M, xs, far // 2, None, None, D, G, U, M, None, D, dw[0], dw[1], D, N, M, D,
+                    torch.empty(n, dtype=torch.uint8, device="cuda"), n)
+    dU = h.double() * G.double().clamp(min=0)
+    within(dw[1], dU.T @ x.double(), (UNIT[torch.bfloat16] + 2 * N * E) * (dU.abs().T @ x.double().abs()), torch.bfloat16)
+
+
+def test_outputs_whose_rows_are_far_apart(tiled):
+    """Rows of 2^31 elements: the second one's bytes are past 32 bits."""
+    dv = tiled
+    M, N, K, far = 3, 40, 128, 1 << 31
+    g = gen(2)
+    a, b = (torch.randint(-128, 128, (r, K), generator=g, device="cuda").to(torch.int8) for r in (M, N))
+    one = torch.ones(N, device="cuda")
+    big = torch.empty((M - 1) * far + 64, dtype=torch.bfloat16, device="cuda")
+    c = big.as_strided((M, N), (far, 1))
+    c.zero_()
+    dv.gemm_i8_scaled(a, K, b, K, one, one, None, capi.TYPE_BF16, c, far, M, N, K)
+    ref = a.double() @ b.double().T
+    within(c, ref, 4 * E * ref.abs(), torch.bfloat16)
+    c.zero_()
+    dv.glu_i8(capi.GLU_RELU, a, K, b, b, K, one, one, one, capi.TYPE_BF16, c, far, M, N, K)     # (the same weights twice)
+    want = ref.clamp(min=0) * ref
+    within(c, want, 4 * E * want.abs(), torch.bfloat16)
+    # as inputs of the quantiser and of the gradients
+    q, s = torch.empty(M, N, dtype=torch.int8, device="cuda"), torch.empty(M, device="cuda")
+    dv.quantize_i8(capi.TYPE_BF16, c, far, q, N, s, M, N, N)
+    assert torch.equal(q.double(), quantized(c)[0])
+    c.copy_(torch.randn(M, N, generator=g, device="cuda"))
+    D = 64
+    w = torch.randn(N, D, generator=g, device="cuda").bfloat16()
+    dx = torch.empty(M, D, dtype=torch.bfloat16, device="cuda")
+    n = dv.glu_backward_workspace(M, N, D)
+    dv.glu_backward(capi.TYPE_BF16, capi.GLU_RELU, c, far, None, D, w, w, D, c, c, far, dx, D, None, None, D, M, N, D, torch.empty(n, dtype=torch.uint8, device="cuda"), n)
+    v = c.double()
+    d = torch.where(v > 0, v * v, 0.0)                       # dG and dU of relu with dH = G = U
+    within(dx, 2 * d @ w.double(), 2 * (UNIT[torch.bfloat16] + 4 * N * E) * (d.abs() @ w.double().abs()), torch.bfloat16)
+
+
+def test_a_product_out_of_the_types_range_is_infinite(tiled):
+    """fp16 holds 65504: what is past half a step above is infinity, with its sign, and nothing else changes."""
+    dv = tiled
+    T, F, D = 80, 90, 64
+    x = torch.zeros(T, D, dtype=torch.float16, device="cuda")
+    x[:, 0] = torch.linspace(-300, 300, T, device="cuda")
+    wg, wu = torch.zeros(F, D, dtype=torch.float16, device="cuda"), torch.zeros(F, D, dtype=torch.float16, device="cuda")
+    wg[:, 0] = 1.0
+    wu[:, 0] = torch.linspace(-2, 2, F, device="cuda")
+    h = torch.empty(T, F, dtype=torch.float16, device="cuda")
+    dv.glu_forward(capi.TYPE_F16, capi.GLU_RELU, x, D, wg, wu, D, h, F, None, None, 0, T, F, D)
+    g64 = x.double()[:, :1]
+    ref = g64.clamp(min=0) * (g64 * wu.double()[:, 0][None])
+    assert bool(torch.isinf(h).any())
+    assert torch.equal(h, ref.to(torch.float16))             # two roundings in fp32, exact here: 11-bit factors
+
+
+def test_a_refused_call_leaves_the_handle_usable(dv):
+    x = torch.randn(4, 256, device="cuda")
+    q, s = torch.full((4, 256), 5, dtype=torch.int8, device="cuda"), torch.zeros(4, device="cuda")
+    with pytest.raises(capi.Mi355Error) as e:
+        dv.quantize_i8(capi.TYPE_F32, x, 100, q, 256, s, 4, 256, 256)
+    assert e.value.code == capi.ERR_ARG and "do not fit" in str(e.value)
+    assert bool((q == 5).all())
+    dv.quantize_i8(capi.TYPE_F32, x, 256, q, 256, s, 4, 256, 256)
+    assert torch.equal(q.double(), quantized(x)[0])
+    n = dv.glu_backward_workspace(300, 400, 128)
+    with pytest.raises(capi.Mi355Error) as e:
+        dv.glu_backward(capi.TYPE_BF16, 0, x, 400, x, 128, x, x, 128, x, x, 400, x, 128, x, x, 128, 300, 400, 128, torch.empty(n, dtype=torch.uint8, device="cuda"), n - 1)
+    assert "are needed" in str(e.value)
+
+
+def test_the_handles_own_stream():
+    """A handle that owns its stream: its calls are in order among themselves and wait for mi355_sync."""
+    d = capi.Device(0)
+    M, K = 33, 512
+    x = torch.randn(M, K, device="cuda")
+    torch.cuda.synchronize()
+    w = torch.randint(-127, 128, (40, K), device="cuda").to(torch.int8)
+    q, s, one, c = d.alloc(M * K), d.alloc(M * 4), torch.ones(40, device="cuda"), d.alloc(M * 40 * 4)
+    torch.cuda.synchronize()
+    d.quantize_i8(capi.TYPE_F32, x, K, q, K, s, M, K, K)
+    d.gemm_i8_scaled(q, K, w, K, s, one, None, capi.TYPE_F32, c, 40, M, 40, K)
+    d.sync()
+    got = torch.from_numpy(c.download(np.float32, M * 40)).view(M, 40).cuda()
+    rq, rs = quantized(x)
+    ref = (rq @ w.double().T) * rs.double()[:, None]
+    within(got, ref, 4 * E * ref.abs(), torch.float32)
+    for b in (q, s, c):
+        b.free()
+    d.close()
