@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(kQuadThreads) ffn_across_kernel(FfnAcross p, u
         if (part) o.out.c = p.c2;
       }
       if constexpr (EPI == kEpiPartial) o.out.c = static_cast<float *>(o.out.c) + (uint64_t)blockIdx.y * p.m * p.out.ldc;
-      Finish<OP, EPI, TYPE>{o, row_tile * 256u + wm * 128u + lane % 16u, tn * 256u + wn * 128u, lane}.run();
+      Finish<OP, EPI, TYPE>{o, row_tile * 256u + wm * 128u + lane % 16u, tn * 256u + wn * 128u, lane, false}.run();
       left = steps;
       w.first = 1;
       done = ++round == grid.mine;

@@ -26,6 +26,7 @@ __global__ void __launch_bounds__(kQuadThreads) ffn_quad_kernel(FfnProduct p, ui
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const uint32_t wm = wave / 2, wn = wave % 2;
   const TileGrid grid = tiles_of_workgroup(tiles_m, tiles_n);
+  const bool many_rounds = grid.total >= Finish<OP, EPI, TYPE>::kManyRounds * grid.stride;
   const uint32_t k_bytes = p.k_bytes, steps = k_bytes / kRowBytes;
   const uint32_t lda = (uint32_t)p.lda, ldb = (uint32_t)p.ldb;
   const uint32_t lds_base = (uint32_t)(uintptr_t)lds;
@@ -115,7 +116,7 @@ __global__ void __launch_bounds__(kQuadThreads) ffn_quad_kernel(FfnProduct p, ui
     if (left == 0u) {
       uint32_t tm, tn;
       tile_at(grid, round, tm, tn);
-      Finish<OP, EPI, TYPE>{p, tm * 256u + wm * 128u + lane % 16u, tn * kCols + wn * (kCols / 2u), lane}.run();
+      Finish<OP, EPI, TYPE>{p, tm * 256u + wm * 128u + lane % 16u, tn * kCols + wn * (kCols / 2u), lane, many_rounds}.run();
       left = steps;
       w.first = 1;
       done = ++round == grid.mine;

@@ -23,7 +23,8 @@ struct PairOut {
   }
   // `whole`: the row exists and so do all of the lane's columns; `some`: the row exists and only the columns below `rem` do
   // (rem counts from the lane's first column).
-  __device__ __forceinline__ void store(const float (&x)[2][4], bool whole, bool edge, bool some, int32_t rem) {
+  // streams: past the caches.
+  __device__ __forceinline__ void store(const float (&x)[2][4], bool whole, bool edge, bool some, int32_t rem, bool streams) {
     if constexpr (TYPE == MI355_TYPE_F32) {
       if (whole) {
         __builtin_memcpy(__builtin_assume_aligned(at, 4), x[0], 16);
@@ -46,7 +47,13 @@ struct PairOut {
       const auto q01 = __builtin_amdgcn_permlane16_swap(p[0][0], p[1][0], false, false);
       const auto q23 = __builtin_amdgcn_permlane16_swap(p[0][1], p[1][1], false, false);
       const uint32_t w[4] = {q01[0], q23[0], q01[1], q23[1]};
-      if (whole) __builtin_memcpy(__builtin_assume_aligned(at, 2), w, 16);
+      if (whole) {
+        // (as text: the compiler merges the two arms of a branch that differ only in the cache policy of a store; the wait
+        // state keeps a following write to its data registers off, which the compiler sees to for its own stores)
+        const i32x4v bits = {(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+        if (streams) asm volatile("global_store_dwordx4 %0, %1, off nt\n s_nop 0" :: "v"(at), "v"(bits) : "memory");
+        else __builtin_memcpy(__builtin_assume_aligned(at, 2), w, 16);
+      }
       if (__builtin_expect(edge, 0)) {
         if (some) {   // (a loop, so that this rare case stays short code)
           uint64_t lo = (uint64_t)w[1] << 32 | w[0], hi = (uint64_t)w[3] << 32 | w[2];
@@ -91,8 +98,14 @@ struct PairScales {
 
 template <int OP, int EPI, int TYPE>
 struct Finish {
+  static constexpr uint32_t kManyRounds = 4;
   const FfnProduct &p;
   uint32_t row0, col0, lane;   // the lane's first row, the wave's first column
+  // The outputs of a gated 16-bit product of many rounds go past the caches, where up to three of them would only push out
+  // operands that later rounds read again (glu 8192x8192x4096 with G and U, 8 rounds: 743 -> 718 us; 2048 rows, 2 rounds:
+  // 177 -> 186 us, the last round's stores being all that is left to wait for; int8, whose operands are half as large:
+  // 2 % slower)
+  bool many_rounds;
   float sa[8];
   PairOut<TYPE> c, g, u;
 
@@ -123,8 +136,8 @@ struct Finish {
         }
       if constexpr (EPI == kEpiGated)
         if (p.out.g) {
-          g.store(x, whole, edge, row && !whole, rem);
-          u.store(y, whole, edge, row && !whole, rem);
+          g.store(x, whole, edge, row && !whole, rem, EPI == kEpiGated && many_rounds);
+          u.store(y, whole, edge, row && !whole, rem, EPI == kEpiGated && many_rounds);
         }
       // one branch on the activation for the 8 values
       auto gate = [&](int act) {
@@ -136,7 +149,7 @@ struct Finish {
       else if (p.out.act == MI355_GLU_GELU) gate(MI355_GLU_GELU);
       else gate(MI355_GLU_RELU);
     }
-    c.store(x, whole, edge, row && !whole, rem);
+    c.store(x, whole, edge, row && !whole, rem, EPI == kEpiGated && many_rounds);
     __builtin_amdgcn_sched_barrier(0);   // few tiles at a time: the fragment registers stay live, few are free
   }
   template <int JP, int... Is>
