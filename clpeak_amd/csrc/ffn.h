@@ -130,12 +130,6 @@ __device__ __forceinline__ void ffn_store1(void *base, uint64_t at, int type, fl
   const uint32_t p = type == MI355_TYPE_F16 ? mi355_pack_f16x2(x, 0.0f) : mi355_pack_bf16x2(x, 0.0f);
   static_cast<uint16_t *>(base)[at] = (uint16_t)p;
 }
-__device__ __forceinline__ float ffn_load1(const void *base, uint64_t at, int type) {
-  if (type == MI355_TYPE_F32) return static_cast<const float *>(base)[at];
-  if (type == MI355_TYPE_F16) return (float)static_cast<const _Float16 *>(base)[at];
-  const uint32_t bits = (uint32_t)static_cast<const uint16_t *>(base)[at] << 16;
-  return __builtin_bit_cast(float, bits);
-}
 
 // int32 sum -> value.  The sum is rounded to fp32 (exact below 2^24), then multiplied by the two scales in turn, so that
 // neither product of a small and a large scale leaves the range before the sum is in it.
@@ -143,7 +137,7 @@ __device__ __forceinline__ float ffn_scaled(int32_t sum, float sa, float sb) { r
 // (the addition as one operation with the second product, in every kernel alike)
 __device__ __forceinline__ float ffn_scaled_plus(int32_t sum, float sa, float sb, float bias) { return fmaf((float)sum * sa, sb, bias); }
 
-// ---- finished tiles of the tile kernels --------------------------------------------------------------------------------
+// ---- finished tiles --------------------------------------------------------------------------------
 // A wave's sums are tiles of 16x16, and a lane holds 4 consecutive columns of one row of a tile: row lane % 16, columns
 // 4 (lane / 16) on (the products are issued transposed).  Two neighbouring tiles are finished together: of 16-bit
 // outputs the two first trade halves (v_permlane16_swap exchanges the odd lane groups of the first tile with the even

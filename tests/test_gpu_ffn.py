@@ -256,6 +256,23 @@ def test_glu_forward_larger(tiled, T, F, D):
     test_glu_forward(tiled, capi.TYPE_F16, T, F, D)
 
 
+def test_glu_forward_many_rounds(dv):
+    """More than four rounds of 256x256 tiles over the CUs, where the outputs are stored past the caches: an odd number of
+    channels, both sums kept, whole outputs."""
+    T, F, D, dt = 8200, 4131, 64, torch.bfloat16
+    g = gen(77)
+    x, wg, wu = operand(g, T, D, D, dt), operand(g, F, D, D, dt, 0.25), operand(g, F, D, D, dt, 0.25)
+    (hb, h), (gb, G), (ub, U) = (padded(T, F, F + 2, dt, -7.0) for _ in range(3))
+    assert ((T + 255) // 256) * ((F + 127) // 128) >= 4 * dv.props.num_cus
+    dv.glu_forward(capi.TYPE_BF16, capi.GLU_RELU, x, D, wg, wu, D, h, F + 2, G, U, F + 2, T, F, D)
+    G64, U64 = x.double() @ wg.double().T, x.double() @ wu.double().T
+    sg, su = 2 * D * E * (x.double().abs() @ wg.double().abs().T), 2 * D * E * (x.double().abs() @ wu.double().abs().T)
+    within(G, G64, sg, dt)
+    within(U, U64, su, dt)
+    within(h, G64.clamp(min=0) * U64, sg * U64.abs() + G64.abs() * su + 4 * E * (G64 * U64).abs(), dt)
+    assert untouched(hb, h, F + 2, -7.0) and untouched(gb, G, F + 2, -7.0) and untouched(ub, U, F + 2, -7.0)
+
+
 def test_nothing_is_summed_over_no_rows_on_any_tiling(tiled):
     test_glu_backward_without_rows_clears_the_weights_gradients(tiled)
 
