@@ -46,7 +46,7 @@ int check_sizes(mi355_dev *dev, const char *what, uint32_t rows, uint32_t cols, 
 
 // Which kernel: the one whose time, by what was measured of it, is least.  Each has its own limit.
 //   rows   everything the workgroups read, the weights once and the rows of A once for each workgroup, at 8.4 TB/s through
-//          the vector caches, the weights at 5.5 TB/s from memory;
+//          the vector caches of all CUs, the weights at 5.5 TB/s from memory;
 //   tiles  of 64x64, 128x128 or 256x256 sums: rounds of tiles over the CUs, each the steps of K (128 bytes) times a step's
 //          time and what surrounds the walk (the 256x256 tiles' workgroups go on to their next tile without a break).  A
 //          step takes longer as the part fills up and its clock falls.  At least the time of the weights, more where CUs
@@ -94,7 +94,8 @@ Choice choose(const mi355_dev *dev, int epi, uint32_t m, uint32_t n, uint32_t k_
   const int pin = dev->gemm_tiling;
   if (pin == MI355_GEMM_TILING_AUTO && m <= 64u) {
     const double a_rows = m <= 16u ? m : (m + 15u) / 16u * 16u;
-    take(kOnRows, 1, 2.5 + std::max(sums_n * k_bytes / 5.5e6, (sums_n + (n + 15u) / 16u * a_rows) * k_bytes / 8.4e6));
+    const double groups = (n + 15u) / 16u, all_read = (sums_n + groups * a_rows) * k_bytes;
+    take(kOnRows, 1, 2.5 + std::max(sums_n * k_bytes / 5.5e6, all_read / (8.4e6 * std::min(1.0, groups / cus))));
   }
   for (const Tiling &t : kTilings) {
     if (pin != MI355_GEMM_TILING_AUTO && pin != t.pin) continue;
