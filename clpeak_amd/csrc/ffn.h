@@ -35,7 +35,7 @@ struct FfnProduct {
   FfnOut out;
 };
 
-// ffn_rows.hip: any shape; the kernel for few rows.  op: kQuadBf16 / kQuadF16 / kQuadI8.
+// ffn_rows.hip: at most 64 rows of A.  op: kQuadBf16 / kQuadF16 / kQuadI8.
 int mi355_launch_ffn_rows(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p);
 
 // ffn_quad.hip / ffn_small.hip: on 256x256 and on 128x128 tiles of sums (gated: of 256x128 / 128x64 outputs).

@@ -6,7 +6,7 @@
 
 namespace {
 
-constexpr uint32_t kMaxCount = 1u << 30;          // rows / columns of a matrix: indices and launches stay within 32 bits
+constexpr uint32_t kMaxRows = 1u << 30, kMaxCols = 1u << 26;   // of a matrix: indices and a launch's threads stay within 32 bits
 constexpr uint64_t kMaxRow = 64ull << 20;         // bytes between two rows of an operand (32-bit offsets within 64 rows)
 constexpr uint64_t kMaxStride = 1ull << 40;       // elements between two rows of any other matrix
 
@@ -37,7 +37,7 @@ int check_16bit(mi355_dev *dev, const char *what, int type, int act) {
 // rows x cols outputs, sums over k.
 int check_sizes(mi355_dev *dev, const char *what, uint32_t rows, uint32_t cols, uint32_t k, uint32_t elem) {
   MI355_REQUIRE(dev, cols > 0 && k > 0, "%s: empty problem", what);
-  MI355_REQUIRE(dev, rows <= kMaxCount && cols <= kMaxCount, "%s: %u rows and %u columns: at most 2^30 of each are taken", what, rows, cols);
+  MI355_REQUIRE(dev, rows <= kMaxRows && cols <= kMaxCols, "%s: %u rows and %u columns: at most 2^30 and 2^26 are taken", what, rows, cols);
   MI355_REQUIRE(dev, (uint64_t)k * elem % 128u == 0 && (uint64_t)k * elem <= kMaxRow, "%s: sums over %u elements: a multiple of %u and at most 64 MiB are wanted", what, k, 128u / elem);
   return MI355_OK;
 }

@@ -233,7 +233,7 @@ int mi355_launch_glu_backward(mi355_dev *dev, int type, int act, const void *dH,
   const Plan p = plan_of(dev, T, F, D);
   const int op = type == MI355_TYPE_BF16 ? kQuadBf16 : kQuadF16;
   const uint64_t tiles = p.fk / 64u * (p.tp / 64u) + (uint64_t)(D / 64u) * (2u * (p.fk / 64u) + p.tp / 64u);
-  MI355_REQUIRE(dev, tiles <= 0x7fffffffull, "glu_backward: T = %u, F = %u, D = %u are more than one launch takes", T, F, D);
+  MI355_REQUIRE(dev, tiles <= 0xffffffull, "glu_backward: T = %u, F = %u, D = %u are more than one launch takes", T, F, D);
   uint8_t *const wu_copy = ws + p.w + (p.dx_across ? 64 * (uint64_t)D * 2 : p.fk * 2);
   Gate gate;
   gate.dH = (const uint16_t *)dH; gate.G = (const uint16_t *)G; gate.U = (const uint16_t *)U;

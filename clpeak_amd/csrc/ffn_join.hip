@@ -28,7 +28,7 @@ __global__ void __launch_bounds__(256) ffn_join_kernel(FfnOut o, const int32_t *
 template <int OP, int EPI>
 int launch(mi355_dev *dev, const char *what, const FfnProduct &p, uint32_t slices, const void *workspace) {
   const uint64_t blocks = ((p.n + 3ull) / 4u * p.m + 255u) / 256u;
-  MI355_REQUIRE(dev, blocks <= 0x7fffffffull, "%s: %u x %u outputs are more than one launch takes", what, p.m, p.n);
+  MI355_REQUIRE(dev, blocks <= 0xffffffull, "%s: %u x %u outputs are more than one launch takes", what, p.m, p.n);
   ffn_join_kernel<OP, EPI><<<(uint32_t)blocks, 256, 0, dev->stream>>>(p.out, (const int32_t *)workspace, slices, mi355_ffn_slice_row(p.n), p.m, p.n);
   MI355_LAUNCH_CHECK(dev, what);
   return MI355_OK;

@@ -108,7 +108,7 @@ int launch_tiles(mi355_dev *dev, const char *what, const FfnProduct &p, uint32_t
   if (int rc = allow_full_lds(dev, &ffn_mid_kernel<OP, EPI>, kLdsFfnMid0 + ffn_kind(OP, EPI))) return rc;
   const uint32_t cols = epi_is_gated(EPI) ? 32 : 64;
   const uint64_t tiles_m = (p.m + 63ull) / 64u, tiles_n = (p.n + cols - 1ull) / cols;
-  MI355_REQUIRE(dev, tiles_m * tiles_n <= 0x3fffffffull, "%s: %u x %u outputs are more than one launch takes", what, p.m, p.n);
+  MI355_REQUIRE(dev, tiles_m * tiles_n <= 0xffffffull, "%s: %u x %u outputs are more than one launch takes", what, p.m, p.n);
   ffn_mid_kernel<OP, EPI><<<dim3((uint32_t)(tiles_m * tiles_n), slices), kMidThreads, kRingBytes, dev->stream>>>(p, (uint32_t)tiles_n);
   MI355_LAUNCH_CHECK(dev, what);
   return MI355_OK;

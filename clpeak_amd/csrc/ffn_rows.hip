@@ -2,7 +2,7 @@
 // of rows, so the time is that of reading the weights.
 //
 // A workgroup of eight waves owns 16 rows of B (gated: 16 of the gate's and the same 16 of the other projection's) and
-// 16 MT rows of A, over the whole of K.  K is cut into windows of 128 bytes, which the waves take in turn: a wave reads
+// all rows of A (16 MT of them, at most 64), over the whole of K.  K is cut into windows of 128 bytes, which the waves take in turn: a wave reads
 // its window's fragments straight from memory into registers (nothing is shared between the waves, so LDS would only
 // add a trip), the workgroup's eight windows are 1 KiB of every row, and the waves' sums meet in LDS at the end, added
 // in the order of the waves: results do not depend on timing.  No sum is split over workgroups: N = 4096 rows are 256
@@ -53,19 +53,18 @@ struct RowStage {
 constexpr int rows_unroll(int mt, int nb) { return mt == 1 ? (nb == 1 ? 2 : 1) : mt == 4 || mt * nb > 4 ? (nb == 1 ? 2 : 1) : 2; }
 
 template <int OP, int EPI, int MT>
-__global__ void __launch_bounds__(kRowThreads, MT == 1 ? 4 : 2) ffn_rows_kernel(FfnProduct p, uint32_t tiles_n) {
+__global__ void __launch_bounds__(kRowThreads, MT == 1 ? 4 : 2) ffn_rows_kernel(FfnProduct p) {
   constexpr int NB = epi_is_gated(EPI) ? 2 : 1;
   constexpr int U = rows_unroll(MT, NB);
   __shared__ int32_t sums[kRowWaves][MT][NB][16][16];   // [row][column]
   const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t r = lane % 16, g = lane / 16;
-  const uint32_t tn = blockIdx.x % tiles_n, tm = blockIdx.x / tiles_n;
-  const uint32_t m0 = tm * 16u * MT, n0 = tn * 16u;
+  const uint32_t tn = blockIdx.x, n0 = tn * 16u;
 
   // Rows past the last one are read as the last one; what they give is never stored.
   const uint8_t *pa[MT], *pb[NB];
 #pragma unroll
-  for (int i = 0; i < MT; i++) pa[i] = p.a + (uint64_t)min(m0 + 16u * i + r, p.m - 1u) * p.lda + 16u * g;
+  for (int i = 0; i < MT; i++) pa[i] = p.a + (uint64_t)min(16u * i + r, p.m - 1u) * p.lda + 16u * g;
   const uint64_t b_row = (uint64_t)min(n0 + r, p.n - 1u) * p.ldb + 16u * g;
   pb[0] = p.b + b_row;
   if constexpr (NB == 2) pb[1] = p.b2 + b_row;
@@ -125,15 +124,13 @@ __global__ void __launch_bounds__(kRowThreads, MT == 1 ? 4 : 2) ffn_rows_kernel(
         s[j] = __builtin_bit_cast(int32_t, f);
       }
     }
-    if (m0 + 16u * i + row < p.m && n0 + col < p.n) ffn_finish1<EPI>(p.out, m0 + 16u * i + row, n0 + col, s[0], s[1]);
+    if (16u * i + row < p.m && n0 + col < p.n) ffn_finish1<EPI>(p.out, 16u * i + row, n0 + col, s[0], s[1]);
   }
 }
 
 template <int OP, int EPI, int MT>
 int launch(mi355_dev *dev, const char *what, const FfnProduct &p) {
-  const uint64_t tiles_n = (p.n + 15ull) / 16u, tiles_m = (p.m + 16ull * MT - 1u) / (16u * MT);
-  MI355_REQUIRE(dev, tiles_n * tiles_m <= 0x7fffffffull, "%s: %u x %u outputs are more than one launch takes", what, p.m, p.n);
-  ffn_rows_kernel<OP, EPI, MT><<<(uint32_t)(tiles_n * tiles_m), kRowThreads, 0, dev->stream>>>(p, (uint32_t)tiles_n);
+  ffn_rows_kernel<OP, EPI, MT><<<(p.n + 15u) / 16u, kRowThreads, 0, dev->stream>>>(p);
   MI355_LAUNCH_CHECK(dev, what);
   return MI355_OK;
 }

@@ -17,6 +17,7 @@
 // A row of up to 2048 elements belongs to one wave (no barrier, four rows per workgroup), a longer one to a workgroup of 4, 8
 // or 16 waves; past 65536 elements the row is read again, from the caches.  Bound by the 2 (4) bytes read and the byte written.
 #include "ffn.h"
+#include <algorithm>
 
 namespace {
 
@@ -194,8 +195,7 @@ __global__ void __launch_bounds__(LANES > 64 ? LANES : 256) quantize_i8_kernel(c
 
 template <int TYPE>
 void launch(mi355_dev *dev, const void *X, uint64_t ldx, int8_t *Q, uint64_t ldq, float *scale, uint32_t M, uint32_t K, uint32_t kv) {
-  const uint32_t by_wave = M / 4u + (M % 4u != 0u);
-#define GO(lanes, ch) quantize_i8_kernel<TYPE, lanes, ch><<<lanes > 64 ? M : by_wave, lanes > 64 ? lanes : 256, 0, dev->stream>>>(X, ldx, Q, ldq, scale, M, K, kv)
+#define GO(lanes, ch) quantize_i8_kernel<TYPE, lanes, ch><<<lanes > 64 ? M : (M + 3u) / 4u, lanes > 64 ? lanes : 256, 0, dev->stream>>>(X, ldx, Q, ldq, scale, M, K, kv)
   if (K <= 512u) GO(64, 1);
   else if (K <= 1024u) GO(64, 2);
   else if (K <= 2048u) GO(64, 4);
@@ -207,6 +207,8 @@ void launch(mi355_dev *dev, const void *X, uint64_t ldx, int8_t *Q, uint64_t ldq
   else GO(1024, 0);
 #undef GO
 }
+
+constexpr uint32_t kMaxLaunchRows = 1u << 21;   // (a launch has less than 2^32 threads, a row at most 1024)
 
 }  // namespace
 
@@ -225,9 +227,13 @@ extern "C" int mi355_quantize_i8(mi355_dev *dev, int type, const void *X, uint64
   const uintptr_t e = type == MI355_TYPE_F32 ? 4 : 2;
   MI355_REQUIRE(dev, (uintptr_t)X % e == 0 && (uintptr_t)scale % 4 == 0, "quantize_i8: X and the scales must be aligned to their elements");
   MI355_SET_DEVICE(dev);
-  if (type == MI355_TYPE_BF16) launch<MI355_TYPE_BF16>(dev, X, ldx, Q, ldq, scale, M, K, k_pad);
-  else if (type == MI355_TYPE_F16) launch<MI355_TYPE_F16>(dev, X, ldx, Q, ldq, scale, M, K, k_pad);
-  else launch<MI355_TYPE_F32>(dev, X, ldx, Q, ldq, scale, M, K, k_pad);
-  MI355_LAUNCH_CHECK(dev, "quantize_i8");
+  for (uint32_t m = 0; m < M; m += kMaxLaunchRows) {
+    const uint32_t rows = std::min(M - m, kMaxLaunchRows);
+    const uint8_t *x = static_cast<const uint8_t *>(X) + m * ldx * e;
+    if (type == MI355_TYPE_BF16) launch<MI355_TYPE_BF16>(dev, x, ldx, Q + m * ldq, ldq, scale + m, rows, K, k_pad);
+    else if (type == MI355_TYPE_F16) launch<MI355_TYPE_F16>(dev, x, ldx, Q + m * ldq, ldq, scale + m, rows, K, k_pad);
+    else launch<MI355_TYPE_F32>(dev, x, ldx, Q + m * ldq, ldq, scale + m, rows, K, k_pad);
+    MI355_LAUNCH_CHECK(dev, "quantize_i8");
+  }
   return MI355_OK;
 }

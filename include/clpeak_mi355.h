@@ -357,8 +357,8 @@ int mi355_fill_bytes(mi355_dev *dev, uint8_t *dst, uint64_t n, uint64_t seed, ui
  * Common rules.  Matrices are row-major, ld* is the distance of two rows in elements of that matrix.  All buffers are
  * device memory of the handle's GPU; outputs overlap neither each other nor an input.  Operands of the products (X, W*, A,
  * B) start on 16 bytes, their rows are a multiple of 16 bytes apart, and a row of K is a multiple of 128 bytes (64 16-bit values, 128
- * int8) and at most 64 MiB; every other matrix needs the alignment of its elements only.  Numbers of rows and columns are
- * otherwise free.  No rows (T or M zero) is a call that writes nothing (mi355_glu_backward: zero weight gradients);
+ * int8) and at most 64 MiB; every other matrix needs the alignment of its elements only.  Numbers of rows (to 2^30)
+ * and of columns (to 2^26) are otherwise free.  No rows (T or M zero) is a call that writes nothing (mi355_glu_backward: zero weight gradients);
  * anything else empty is refused.  Of an output only its rows and columns are written, not what lies between them.
  * Calls enqueue and return; they allocate nothing, keep nothing from one call to the next and launch kernels only,
  * so that they can be captured into a graph.  A workspace belongs to a call until that call's work is done: calls

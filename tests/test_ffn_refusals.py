@@ -91,7 +91,7 @@ BAD = [
     product(type=3), product(A=None), product(A=P + 8), product(lda=128), product(lda=264), product(B=None), product(B=P + 4), product(ldb=255),
     product(sa=None), product(sb=None), product(sa=P + 1), product(sb=P + 2), product(bias=P + 1), product(C=None), product(type=2, C=P + 2),
     product(ldc=32), product(N=0), product(K=0), product(K=192), product(K=131072, lda=131072, ldb=131072), product(ws=P + 8, bytes=64),
-    product(M=(1 << 30) + 1), product(N=(1 << 30) + 1),
+    product(M=(1 << 30) + 1), product(N=(1 << 30) + 1), product(N=(1 << 26) + 1, ldc=1 << 27), forward(F=(1 << 26) + 1, ldh=1 << 27, ldg=1 << 27),
     glu_i8(act=4), glu_i8(type=5), glu_i8(A=None), glu_i8(Bg=None), glu_i8(Bu=P + 8), glu_i8(sg=None), glu_i8(su=None), glu_i8(sa=None),
     glu_i8(H=None), glu_i8(ldh=10), glu_i8(F=0), glu_i8(K=64), glu_i8(K=131072, lda=131072, ldb=131072), glu_i8(ldb=128), glu_i8(H=P + 1),
 ]

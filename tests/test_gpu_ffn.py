@@ -804,3 +804,14 @@ def test_the_handles_own_stream():
     for b in (q, s, c):
         b.free()
     d.close()
+
+
+@pytest.mark.parametrize("M", [(1 << 21) - 1, 1 << 21, (1 << 22) + 5])
+def test_quantize_more_rows_than_a_launch_takes(dv, M):
+    K, ldx, ldq = 13, 14, 16
+    x = torch.randn(M, ldx, generator=gen(M), device="cuda").to(torch.bfloat16)
+    q, s = torch.full((M, ldq), 77, dtype=torch.int8, device="cuda"), torch.empty(M + 1, device="cuda").fill_(-1.0)
+    dv.quantize_i8(capi.TYPE_BF16, x, ldx, q, ldq, s, M, K, K)
+    rq, rs = quantized(x[:, :K])
+    assert torch.equal(q[:, :K].double(), rq) and torch.equal(s[:-1], rs) and s[-1] == -1
+    assert bool((q[:, K:] == 77).all())
