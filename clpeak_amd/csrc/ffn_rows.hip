@@ -2,11 +2,15 @@
 // of rows, so the time is that of reading the weights.
 //
 // A workgroup of eight waves owns 16 rows of B (gated: 16 of the gate's and the same 16 of the other projection's) and
-// all rows of A (16 MT of them, at most 64), over the whole of K.  K is cut into windows of 128 bytes, which the waves take in turn: a wave reads
-// its window's fragments straight from memory into registers (nothing is shared between the waves, so LDS would only
-// add a trip), the workgroup's eight windows are 1 KiB of every row, and the waves' sums meet in LDS at the end, added
-// in the order of the waves: results do not depend on timing.  No sum is split over workgroups: N = 4096 rows are 256
-// workgroups, one for each CU.
+// all rows of A (16 MT of them, at most 64), over the whole of K.  K is cut into windows of 128 bytes, which the waves
+// take in turn: a wave reads its window's fragments straight from memory into registers (nothing is shared between the
+// waves, so LDS would only add a trip), the workgroup's eight windows are 1 KiB of every row, and the waves' sums meet in
+// LDS at the end, added in the order of the waves: results do not depend on timing.  No sum is split over workgroups:
+// N = 4096 rows are 256 workgroups, one for each CU.
+//
+// Measured: the gated projection of one token, 2 x 8192 rows of 4096 bf16, 134 MB in 23.0 us (5.8 TB/s); gated 7 x 8192 x
+// 4096 int8, 67 MB in 12.4 us (5.4 TB/s); 1x4096x4096 int8 5.4 us, on 64x64 tiles (ffn_mid.hip) 9.9 us.  With more rows the
+// vector caches bound it: every workgroup reads all of A.
 #include "ffn.h"
 
 namespace {

