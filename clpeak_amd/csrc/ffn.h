@@ -41,12 +41,39 @@ int mi355_launch_ffn_rows(mi355_dev *dev, int op, int epi, const char *what, con
 // ffn_quad.hip / ffn_small.hip: on 256x256 and on 128x128 tiles of sums (gated: of 256x128 / 128x64 outputs).
 int mi355_launch_ffn_quad(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p);
 // ffn_mid.hip: on 64x64 tiles of sums (gated: of 64x32 outputs), for some dozens of rows.
-// slices > 1 (one product, not gated): K is cut into so many, `workspace` holds `slices` matrices of m rows of
+// slices > 1 (kEpiScaled): K is cut into so many, `workspace` holds `slices` matrices of m rows of
 // mi355_ffn_slice_row(n) 32-bit sums, on 16 bytes.
 int mi355_launch_ffn_small(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p, uint32_t slices, void *workspace);
 int mi355_launch_ffn_mid(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p, uint32_t slices, void *workspace);
-// ffn_join.hip: the second launch of a product in slices.
-int mi355_launch_ffn_join(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p, uint32_t slices, const void *workspace);
+// kEpiPlain, on either: up to three products of 16-bit operands in one launch, each in slices of its own number.
+struct FfnGroup {
+  struct One {
+    const uint8_t *a, *b;
+    uint64_t lda, ldb, ldc;
+    void *c;
+    uint32_t m, n, k_bytes, slices;
+    uint32_t tiles_m, tiles_n, first;   // (the launch's: the number of the product's first workgroup)
+  } of[3];
+  uint32_t count;
+  int type;
+};
+struct FfnGroupChoice {
+  bool small;             // 128x128 tiles rather than 64x64
+  uint32_t slices[3];
+  double us;
+};
+// (ffn.hip: the longest walks first; tiles of edge x edge sums)
+int mi355_ffn_lay_out_group(mi355_dev *dev, const char *what, FfnGroup &g, uint32_t edge, uint32_t &blocks);
+int mi355_launch_ffn_small_group(mi355_dev *dev, int op, const char *what, FfnGroup g);
+int mi355_launch_ffn_mid_group(mi355_dev *dev, int op, const char *what, FfnGroup g);
+// ffn_join.hip: the second launch of products in slices, up to three of them.
+struct FfnJoin {
+  FfnOut out;
+  const int32_t *partial;
+  uint64_t ldp;
+  uint32_t m, n, slices, first;   // (first: the launch's)
+};
+int mi355_launch_ffn_join(mi355_dev *dev, int op, int epi, const char *what, FfnJoin *parts, uint32_t count);
 inline uint64_t mi355_ffn_slice_row(uint32_t n) { return (n + 3ull) / 4u * 4u; }
 // The product whose outputs are the sums of the slices, in the workspace.
 inline FfnProduct mi355_ffn_slices_of(const FfnProduct &p, void *workspace) {
@@ -56,6 +83,53 @@ inline FfnProduct mi355_ffn_slices_of(const FfnProduct &p, void *workspace) {
   q.out.type = MI355_TYPE_F32;
   return q;
 }
+inline FfnJoin mi355_ffn_join_of(const FfnProduct &p, uint32_t slices, const void *workspace) {
+  return {p.out, static_cast<const int32_t *>(workspace), mi355_ffn_slice_row(p.n), p.m, p.n, slices, 0};
+}
+
+// What the kernels on 64x64 and 128x128 tiles are given, and what a workgroup makes of it: a tile of a product, and a slice
+// of its K.
+struct FfnWork {
+  FfnProduct p;
+  uint32_t tiles_m, tiles_n, tile, slice, slices;
+};
+template <int EPI>
+struct FfnLaunch {
+  FfnProduct p;
+  uint32_t tiles_m, tiles_n;
+  __device__ __forceinline__ FfnWork work() const {
+    FfnWork w{p, tiles_m, tiles_n, blockIdx.x, 0, 1};
+    if constexpr (EPI == kEpiPartial) {   // (the sums go to p.out.c as matrix number blockIdx.y there)
+      w.slice = blockIdx.y; w.slices = gridDim.y;
+      w.p.out.c = static_cast<float *>(p.out.c) + (uint64_t)blockIdx.y * p.m * p.out.ldc;
+    }
+    return w;
+  }
+};
+template <>
+struct FfnLaunch<kEpiPlain> {
+  FfnGroup g;
+  __device__ __forceinline__ FfnWork work() const {
+    // member by member, with no index that varies: the addresses have to stay in scalar registers
+    const bool second = blockIdx.x >= g.of[1].first, third = blockIdx.x >= g.of[2].first;
+    FfnGroup::One o;
+#define MI355_PICK(x) o.x = third ? g.of[2].x : second ? g.of[1].x : g.of[0].x
+    MI355_PICK(a); MI355_PICK(b); MI355_PICK(lda); MI355_PICK(ldb); MI355_PICK(ldc); MI355_PICK(c);
+    MI355_PICK(m); MI355_PICK(n); MI355_PICK(k_bytes); MI355_PICK(slices); MI355_PICK(tiles_m); MI355_PICK(tiles_n); MI355_PICK(first);
+#undef MI355_PICK
+    const uint32_t at = blockIdx.x - o.first, tiles = o.tiles_m * o.tiles_n;
+    FfnWork w{};
+    w.p.a = o.a; w.p.b = o.b; w.p.lda = o.lda; w.p.ldb = o.ldb;
+    w.p.m = o.m; w.p.n = o.n; w.p.k_bytes = o.k_bytes;
+    w.tiles_m = o.tiles_m; w.tiles_n = o.tiles_n;
+    w.slice = at / tiles; w.tile = at - w.slice * tiles; w.slices = o.slices;
+    w.p.out.ldc = o.ldc;
+    w.p.out.type = o.slices > 1u ? MI355_TYPE_F32 : g.type;
+    w.p.out.c = static_cast<uint8_t *>(o.c) + (o.slices > 1u ? (uint64_t)w.slice * o.m * o.ldc * 4u : 0u);
+    return w;
+  }
+};
+
 // Bits of mi355_dev::full_lds_allowed: the kernels of each tiling (the 256x256 one has one for each output type).
 constexpr int ffn_kind(int op, int epi, int type = 0) {
   return op != kQuadI8 ? (op - kQuadBf16) * 3 + (epi == kEpiPartial ? 2 : epi_is_gated(epi) ? 1 : 0) : epi == kEpiPartial ? 12 : 6 + 3 * epi_is_gated(epi) + type;
@@ -65,7 +139,12 @@ enum { kLdsFfnQuad0 = 24, kLdsFfnSmall0 = 37, kLdsFfnMid0 = 50 };   // 13 each
 // ffn.hip: the product on the kernel that suits it, and the workspace that it can use.
 int mi355_ffn_product(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p, void *workspace, size_t workspace_bytes);
 size_t mi355_ffn_workspace(const mi355_dev *dev, int epi, uint32_t m, uint32_t n, uint32_t k_bytes);
-double mi355_ffn_expected_us(const mi355_dev *dev, int epi, uint32_t m, uint32_t n, uint32_t k_bytes);
+// A group's tiling and slices (of its products m, n and k_bytes are looked at) and its launches, slices joined; the
+// workspace that the slices need; the time expected of a product on ffn_rows.hip (more than 64 rows: forever).
+FfnGroupChoice mi355_choose_ffn_group(const mi355_dev *dev, const FfnGroup &g);
+size_t mi355_ffn_group_workspace(const FfnGroup &g, const FfnGroupChoice &c);
+int mi355_ffn_group(mi355_dev *dev, int op, const char *what, const FfnGroup &g, const FfnGroupChoice &c, uint8_t *workspace);
+double mi355_ffn_rows_us(const mi355_dev *dev, int epi, uint32_t m, uint32_t n, uint32_t k_bytes);
 
 // ffn_backward.hip (arguments checked by the caller).
 int mi355_glu_backward_limits(mi355_dev *dev, const char *what, uint32_t T, uint32_t F);
@@ -236,6 +315,13 @@ __device__ __forceinline__ i32x4v ffn_mfma(const i32x4v &b, const i32x4v &a, con
   }
 }
 
+// The type of an output: that of 16-bit operands but for a slice's sums.
+template <int OP, int EPI>
+__device__ __forceinline__ int ffn_type_out(const FfnOut &o) {
+  if (EPI == kEpiPartial || (EPI == kEpiPlain && o.type == MI355_TYPE_F32)) return MI355_TYPE_F32;
+  return OP == kQuadBf16 ? MI355_TYPE_BF16 : OP == kQuadF16 ? MI355_TYPE_F16 : o.type;
+}
+
 // What a lane needs for its columns of a pair of tiles, and for a row.
 template <int EPI>
 struct FfnColumns {
@@ -259,7 +345,7 @@ struct FfnColumns {
 template <int OP, int EPI>
 __device__ __forceinline__ void ffn_finish_pair(const FfnOut &o, uint32_t row, uint32_t col0, uint32_t lane, uint32_t m, uint32_t n, float sa,
                                                 const FfnColumns<EPI> &c, const i32x4v (&s)[2], const i32x4v (&s2)[2]) {
-  const int type = EPI == kEpiPartial ? MI355_TYPE_F32 : OP == kQuadBf16 ? MI355_TYPE_BF16 : OP == kQuadF16 ? MI355_TYPE_F16 : o.type;
+  const int type = ffn_type_out<OP, EPI>(o);
   FfnPair a, b;
 #pragma unroll
   for (int t = 0; t < 2; t++)
@@ -304,7 +390,7 @@ __device__ __forceinline__ void ffn_finish_pair(const FfnOut &o, uint32_t row, u
 template <int OP, int EPI>
 __device__ __forceinline__ void ffn_finish4(const FfnOut &o, uint32_t row, uint32_t col, uint32_t n, const i32x4v &s, const i32x4v &s2) {
   if (col >= n) return;
-  const int type = EPI == kEpiPartial ? MI355_TYPE_F32 : OP == kQuadBf16 ? MI355_TYPE_BF16 : OP == kQuadF16 ? MI355_TYPE_F16 : o.type;
+  const int type = ffn_type_out<OP, EPI>(o);
   float x[4], y[4];
   const float sa = EPI == kEpiScaled || EPI == kEpiGatedScaled ? o.sa[row] : 0.0f;
 #pragma unroll

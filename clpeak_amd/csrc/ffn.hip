@@ -72,6 +72,8 @@ constexpr Tiling kTilings[] = {{kOn64, MI355_GEMM_TILING_64, 64, 0.20, 0.32, 4.0
                                {kOn128, MI355_GEMM_TILING_128, 128, 0.30, 0.47, 5.0, 0.0, 4.5e6},
                                {kOn256, MI355_GEMM_TILING_256, 256, 0.85, 1.30, 4.0, 10.0, 4.5e6}};
 
+constexpr uint32_t kMostSlices = 16;
+
 double count_of_cus(const mi355_dev *dev) { return dev->props.num_cus > 0 ? dev->props.num_cus : 1; }
 double columns_of_sums(int epi, uint32_t n) { return epi_is_gated(epi) ? 2.0 * n : (double)n; }
 
@@ -92,15 +94,10 @@ Choice choose(const mi355_dev *dev, int epi, uint32_t m, uint32_t n, uint32_t k_
     if (us < best.us) { best.kernel = k; best.slices = slices; best.us = us; }
   };
   const int pin = dev->gemm_tiling;
-  if (pin == MI355_GEMM_TILING_AUTO && m <= 64u) {
-    const double a_rows = m <= 16u ? m : (m + 15u) / 16u * 16u;
-    const double groups = (n + 15u) / 16u, all_read = (sums_n + groups * a_rows) * k_bytes;
-    take(kOnRows, 1, 2.5 + std::max(sums_n * k_bytes / 5.5e6, all_read / (8.4e6 * std::min(1.0, groups / cus))));
-  }
+  if (pin == MI355_GEMM_TILING_AUTO) take(kOnRows, 1, mi355_ffn_rows_us(dev, epi, m, n, k_bytes));
   for (const Tiling &t : kTilings) {
     if (pin != MI355_GEMM_TILING_AUTO && pin != t.pin) continue;
-    if (epi == kEpiPlain && t.kernel == kOn256) continue;   // (those are ffn_across.hip's)
-    const uint32_t most = can_slice && !epi_is_gated(epi) && t.kernel != kOn256 ? 16 : 1;
+    const uint32_t most = can_slice && epi == kEpiScaled && t.kernel != kOn256 ? kMostSlices : 1;
     for (uint32_t s = 1; s <= most && (s == 1 || s * 4u <= k_bytes / 128u); s++) take(t.kernel, s, tiling_us(t, cus, m, n, sums_n, k_bytes, s));
   }
   return best;
@@ -144,8 +141,131 @@ int launch(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &
 
 }  // namespace
 
-double mi355_ffn_expected_us(const mi355_dev *dev, int epi, uint32_t m, uint32_t n, uint32_t k_bytes) {
-  return divide(dev, epi, m, n, k_bytes, true).us;
+double mi355_ffn_rows_us(const mi355_dev *dev, int epi, uint32_t m, uint32_t n, uint32_t k_bytes) {
+  if (m > 64u) return 1e30;
+  const double a_rows = m <= 16u ? m : (m + 15u) / 16u * 16u, sums_n = columns_of_sums(epi, n);
+  const double groups = (n + 15u) / 16u, all_read = (sums_n + groups * a_rows) * k_bytes;
+  return 2.5 + std::max(sums_n * k_bytes / 5.5e6, all_read / (8.4e6 * std::min(1.0, groups / count_of_cus(dev))));
+}
+
+namespace {
+
+// When the last of so many workgroups ends, each CU taking the next when it is done with one; the longest come first.
+struct Workgroups {
+  double count, us;
+};
+double last_end(double cus, Workgroups (&w)[3], uint32_t kinds) {
+  std::sort(w, w + kinds, [](const Workgroups &a, const Workgroups &b) { return a.us > b.us; });
+  struct { double at, cus; } busy[16] = {{0.0, cus}};   // (a kind splits one of them at most, and leaves the rest whole)
+  uint32_t n = 1;
+  double end = 0.0;
+  for (uint32_t k = 0; k < kinds; k++) {
+    double left = w[k].count;
+    if (left > 8.0 * cus) {   // (many rounds: as many on every CU)
+      const double whole = std::floor(left / cus) - 4.0;
+      for (uint32_t i = 0; i < n; i++) busy[i].at += whole * w[k].us;
+      left -= whole * cus;
+    }
+    while (left > 0.0) {
+      uint32_t first = 0;
+      for (uint32_t i = 1; i < n; i++)
+        if (busy[i].at < busy[first].at) first = i;
+      if (left < busy[first].cus && n < 16u) {
+        busy[n++] = {busy[first].at, busy[first].cus - left};
+        busy[first].cus = left;
+      }
+      busy[first].at += w[k].us;
+      left -= busy[first].cus;
+    }
+  }
+  for (uint32_t i = 0; i < n; i++) end = std::max(end, busy[i].at);
+  return end;
+}
+
+}  // namespace
+
+// Slices of about as many steps for all of them, so that no walk outlasts the others.
+FfnGroupChoice mi355_choose_ffn_group(const mi355_dev *dev, const FfnGroup &g) {
+  const double cus = count_of_cus(dev);
+  FfnGroupChoice best{false, {1, 1, 1}, 1e30};
+  uint32_t longest = 1;
+  for (uint32_t i = 0; i < g.count; i++) longest = std::max(longest, g.of[i].k_bytes / 128u);
+  for (const Tiling &t : kTilings) {
+    if (t.kernel == kOn256 || (dev->gemm_tiling != MI355_GEMM_TILING_AUTO && dev->gemm_tiling != t.pin)) continue;
+    double weights_us = 0.0, tiles[3] = {};
+    for (uint32_t i = 0; i < g.count; i++) {
+      weights_us += (double)g.of[i].n * g.of[i].k_bytes / t.weights;
+      tiles[i] = std::ceil(g.of[i].m / t.edge) * std::ceil(g.of[i].n / t.edge);
+    }
+    for (uint32_t s = 1; s <= kMostSlices && (s == 1 || s * 4u <= longest); s++) {
+      FfnGroupChoice c{t.kernel == kOn128, {1, 1, 1}, 0.0};
+      Workgroups w[3] = {};
+      double steps_of[3] = {}, join = 0.0;
+      for (uint32_t i = 0; i < g.count; i++) {
+        const uint32_t steps = g.of[i].k_bytes / 128u;
+        c.slices[i] = std::max(1u, (steps * s + longest / 2u) / longest);
+        while (c.slices[i] > 1u && c.slices[i] * 4u > steps) c.slices[i]--;
+        if (c.slices[i] > 1u) join += (double)g.of[i].m * g.of[i].n * (c.slices[i] * 6.0 + 2.0) / 4e6;
+        steps_of[i] = std::ceil(steps / (double)c.slices[i]);
+      }
+      double step = t.full_step_us, end = 0.0;
+      for (int again = 0; again < 2; again++) {   // (a step is as long as the part is busy, over all of the launch)
+        double work = 0.0;
+        for (uint32_t i = 0; i < g.count; i++) {
+          w[i] = {tiles[i] * c.slices[i], steps_of[i] * step + t.round_us};
+          work += w[i].count * w[i].us;
+        }
+        end = last_end(cus, w, g.count);
+        step = t.step_us + (t.full_step_us - t.step_us) * work / (cus * end);
+      }
+      c.us = t.once_us + std::max(weights_us, end) + (join > 0.0 ? 3.0 + join : 0.0);
+      if (c.us < best.us) best = c;
+    }
+  }
+  return best;
+}
+
+size_t mi355_ffn_group_workspace(const FfnGroup &g, const FfnGroupChoice &c) {
+  uint64_t bytes = 0;
+  for (uint32_t i = 0; i < g.count; i++)
+    if (c.slices[i] > 1u) bytes += c.slices[i] * (uint64_t)g.of[i].m * mi355_ffn_slice_row(g.of[i].n) * 4u;
+  return (size_t)bytes;
+}
+
+int mi355_ffn_lay_out_group(mi355_dev *dev, const char *what, FfnGroup &g, uint32_t edge, uint32_t &blocks) {
+  std::stable_sort(g.of, g.of + g.count, [](const FfnGroup::One &a, const FfnGroup::One &b) { return a.k_bytes / a.slices > b.k_bytes / b.slices; });
+  uint64_t first = 0;
+  for (uint32_t i = 0; i < 3; i++) {
+    FfnGroup::One &o = g.of[i];
+    o.first = i < g.count ? (uint32_t)first : 0xffffffffu;
+    if (i >= g.count) continue;
+    const uint64_t tiles_m = (o.m + (uint64_t)edge - 1u) / edge, tiles_n = (o.n + (uint64_t)edge - 1u) / edge;
+    MI355_REQUIRE(dev, tiles_m * tiles_n <= 0xffffffull && first + tiles_m * tiles_n * o.slices <= 0xffffffull, "%s: %u x %u outputs are more than one launch takes", what, o.m, o.n);
+    o.tiles_m = (uint32_t)tiles_m; o.tiles_n = (uint32_t)tiles_n;
+    first += tiles_m * tiles_n * o.slices;
+  }
+  blocks = (uint32_t)first;
+  return MI355_OK;
+}
+
+int mi355_ffn_group(mi355_dev *dev, int op, const char *what, const FfnGroup &group, const FfnGroupChoice &c, uint8_t *workspace) {
+  FfnGroup g = group;
+  FfnJoin join[3];
+  uint32_t joins = 0;
+  for (uint32_t i = 0; i < g.count; i++) {
+    FfnGroup::One &o = g.of[i];
+    o.slices = c.slices[i];
+    if (o.slices <= 1u) continue;
+    FfnProduct p{};
+    p.m = o.m; p.n = o.n;
+    p.out.c = o.c; p.out.ldc = o.ldc; p.out.type = g.type;
+    join[joins++] = mi355_ffn_join_of(p, o.slices, workspace);
+    o.c = workspace;
+    o.ldc = mi355_ffn_slice_row(o.n);
+    workspace += o.slices * (uint64_t)o.m * o.ldc * 4u;
+  }
+  if (int rc = c.small ? mi355_launch_ffn_small_group(dev, op, what, g) : mi355_launch_ffn_mid_group(dev, op, what, g)) return rc;
+  return joins ? mi355_launch_ffn_join(dev, op, kEpiPlain, what, join, joins) : MI355_OK;
 }
 
 AcrossChoice mi355_choose_ffn_across(const mi355_dev *dev, uint32_t m, uint32_t parts, uint32_t n, uint32_t steps) {

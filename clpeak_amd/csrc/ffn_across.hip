@@ -299,14 +299,15 @@ int launch_slices(mi355_dev *dev, const char *what, const FfnAcross &p, uint32_t
   q.c2 = workspace + part;
   q.out.ldc = p.n;
   if (int rc = launch<OP, ACROSS_A, kEpiPartial, MI355_TYPE_F32>(dev, what, q, slices)) return rc;
+  FfnJoin join[2];
   for (uint32_t i = 0; i < p.parts; i++) {
     FfnProduct o{};
     o.m = p.m; o.n = p.n;
     o.out = p.out;
     if (i) o.out.c = p.c2;
-    if (int rc = mi355_launch_ffn_join(dev, OP, kEpiPlain, what, o, slices, workspace + i * part)) return rc;
+    join[i] = mi355_ffn_join_of(o, slices, workspace + i * part);
   }
-  return MI355_OK;
+  return mi355_launch_ffn_join(dev, OP, kEpiPlain, what, join, p.parts);
 }
 
 }  // namespace

@@ -2,9 +2,11 @@
 // rows of their operands: dX over F, the rows of the weights, dW over T, the rows of X and of dG, dU.
 //
 // Products of many tiles read such operands as they are (ffn_across.hip).  The others run on the kernels that want the
-// sum's index innermost, for which the pass that makes dG and dU writes them both ways and X and the weights are turned
-// once into the workspace.  Which of the two goes by the expected times, for each product by itself: turning costs the
-// products of a training batch (8192x8192x4096) 106 of 1585 us.  Either way the workspace's copies are padded with zeros
+// sum's index innermost, together in one launch (or dX of few rows in one of its own), for which the pass that makes dG
+// and dU writes them both ways and X and the weights are turned once into the workspace.  Which of these goes by the
+// expected times: turning costs the products of a training batch (8192x8192x4096) 106 of 1585 us; one launch for all
+// three products instead of one each takes a call of 1024x1024x1024 from 41.9 to 28.2 us, of 200x700x512 from 24.4 to 16.8,
+// of 1009x2752x1024 from 55.0 to 51.4 (in graphs).  Either way the workspace's copies are padded with zeros
 // to the kernels' 64 values of the sum, which is what lets T and F be anything.
 //
 // The pass that makes dG and dU rounds them to the operands' 16 bits, half a step each: what the matrix instructions take.
@@ -25,8 +27,11 @@ __host__ __device__ constexpr uint64_t round_up(uint64_t x, uint64_t to) { retur
 // cut along their sums.
 struct Plan {
   uint64_t fk, fp, tp;                         // F padded to a row of a product, F padded to whole tiles, T padded to a row
+  enum { kNone, kAcross, kOnRows, kGrouped } dx_on, dw_on;
   bool dx_across, dw_across;
   AcrossChoice dx, dw;
+  FfnGroup group;                              // what goes together (dX first): sizes
+  FfnGroupChoice grouped;
   uint64_t rows, cols, w, x, sums, bytes;      // offsets
 };
 Plan plan_of(const mi355_dev *dev, uint32_t T, uint32_t F, uint32_t D) {
@@ -39,12 +44,34 @@ Plan plan_of(const mi355_dev *dev, uint32_t T, uint32_t F, uint32_t D) {
   p.dx = mi355_choose_ffn_across(dev, T ? T : 1, 1, D, dx_k / 128u);
   p.dw = mi355_choose_ffn_across(dev, F, 2, D, dw_k / 128u);
   const double turn_dx = 8.0 * F * D / 4.5e6, turn_dw = (4.0 * T * F + 4.0 * T * D) / 4.5e6;
-  p.dx_across = T && p.dx.us < mi355_ffn_expected_us(dev, kEpiPlain, T, D, dx_k) + turn_dx;
-  p.dw_across = p.dw.us < 2.0 * mi355_ffn_expected_us(dev, kEpiPlain, F, D, dw_k) + turn_dw;
-  if (dev->gemm_tiling != MI355_GEMM_TILING_AUTO) {
-    p.dw_across = dev->gemm_tiling == MI355_GEMM_TILING_256;
-    p.dx_across = T && p.dw_across;
+  const bool pinned = dev->gemm_tiling != MI355_GEMM_TILING_AUTO, pinned_256 = dev->gemm_tiling == MI355_GEMM_TILING_256;
+  double least = 1e30;
+  for (int on = 0; on < 6; on++) {
+    const auto dx_on = !T ? Plan::kNone : on % 3 == 0 ? Plan::kAcross : on % 3 == 1 ? Plan::kOnRows : Plan::kGrouped;
+    const auto dw_on = on / 3 ? Plan::kGrouped : Plan::kAcross;
+    if (pinned && ((dx_on != Plan::kNone && (dx_on == Plan::kAcross) != pinned_256) || dx_on == Plan::kOnRows || (dw_on == Plan::kAcross) != pinned_256)) continue;
+    FfnGroup g{};
+    auto add = [&](uint32_t m, uint32_t k_bytes) {
+      FfnGroup::One &o = g.of[g.count++];
+      o.m = m; o.n = D; o.k_bytes = k_bytes;
+    };
+    double us = 1.5 * ((dx_on == Plan::kAcross || dx_on == Plan::kOnRows) + (dw_on == Plan::kAcross));   // (from a launch to the next)
+    if (dx_on == Plan::kAcross) us += p.dx.us;
+    else if (dx_on != Plan::kNone) us += turn_dx;
+    if (dx_on == Plan::kOnRows) us += mi355_ffn_rows_us(dev, kEpiPlain, T, D, dx_k);
+    if (dx_on == Plan::kGrouped) add(T, dx_k);
+    if (dw_on == Plan::kAcross) us += p.dw.us;
+    else us += turn_dw, add(F, dw_k), add(F, dw_k);
+    FfnGroupChoice c{};
+    if (g.count) c = mi355_choose_ffn_group(dev, g);
+    us += c.us;
+    if (us >= least) continue;
+    least = us;
+    p.dx_on = dx_on; p.dw_on = dw_on;
+    p.group = g; p.grouped = c;
   }
+  p.dx_across = p.dx_on == Plan::kAcross;
+  p.dw_across = p.dw_on == Plan::kAcross;
   p.rows = 0;
   p.cols = round_up(p.rows + p.tp * 2 * p.fk * 2, 256);
   p.w = round_up(p.cols + (p.dw_across ? 0 : 2 * p.fp * p.tp * 2), 256);
@@ -53,10 +80,9 @@ Plan plan_of(const mi355_dev *dev, uint32_t T, uint32_t F, uint32_t D) {
   auto sums = [&](uint32_t slices, uint64_t rows) { return slices > 1 ? slices * rows * D * 4 : 0; };
   uint64_t dx = 0, dw = 0;
   if (p.dx_across) dx = std::max(sums(p.dx.slices, p.dx.main_rows ? p.dx.main_rows : T), sums(p.dx.rest_slices, T - p.dx.main_rows));
-  else if (T) dx = mi355_ffn_workspace(dev, kEpiPlain, T, D, dx_k);
   if (p.dw_across) dw = sums(p.dw.slices, 2 * (uint64_t)F);
-  else dw = mi355_ffn_workspace(dev, kEpiPlain, F, D, dw_k);
-  p.bytes = round_up(p.sums + (dx > dw ? dx : dw), 256);
+  const uint64_t group = p.group.count ? mi355_ffn_group_workspace(p.group, p.grouped) : 0;
+  p.bytes = round_up(p.sums + std::max(std::max(dx, dw), group), 256);
   return p;
 }
 
@@ -259,8 +285,25 @@ int mi355_launch_glu_backward(mi355_dev *dev, int type, int act, const void *dH,
   c.a = ws + p.rows; c.lda = 4 * p.fk;
   c.n = D;
   c.out.type = type;
-  FfnProduct q{};
-  q.out.type = type;
+  FfnGroup g{};           // the members of the planned group that are wanted
+  FfnGroupChoice choice = p.grouped;
+  g.type = type;
+  uint32_t planned = 0;
+  auto add = [&](bool wanted, const uint8_t *a, uint64_t lda, const uint8_t *b, uint64_t ldb, void *out, uint64_t ldc) {
+    const FfnGroup::One &size = p.group.of[planned];
+    if (wanted) {
+      choice.slices[g.count] = p.grouped.slices[planned];
+      FfnGroup::One &o = g.of[g.count++];
+      o = size;
+      o.a = a; o.lda = lda; o.b = b; o.ldb = ldb; o.c = out; o.ldc = ldc;
+    }
+    planned++;
+  };
+  if (p.dx_on == Plan::kGrouped) add(dX, ws + p.rows, 4 * p.fk, ws + p.w, 4 * p.fk, dX, lddx);
+  if (p.dw_on == Plan::kGrouped) {
+    add(dWg, ws + p.cols, 2 * p.tp, ws + p.x, 2 * p.tp, dWg, lddw);
+    add(dWu, ws + p.cols + p.fp * p.tp * 2, 2 * p.tp, ws + p.x, 2 * p.tp, dWu, lddw);
+  }
   if (dX && p.dx_across) {
     c.m = p.dx.main_rows ? p.dx.main_rows : T; c.steps = (uint32_t)(2 * p.fk / 64u); c.parts = 1; c.stretches = 0;
     add_stretches(c, Wg, ldw, ws + p.w, F, D);
@@ -273,12 +316,13 @@ int mi355_launch_glu_backward(mi355_dev *dev, int type, int act, const void *dH,
       c.out.c = (uint16_t *)dX + p.dx.main_rows * lddx;
       if (int rc = mi355_launch_ffn_across(dev, op, false, "glu_backward (dX)", c, p.dx.rest_slices, ws + p.sums)) return rc;
     }
-  } else if (dX) {
+  } else if (dX && p.dx_on == Plan::kOnRows) {
+    FfnProduct q{};
     q.a = ws + p.rows; q.lda = 4 * p.fk;
     q.b = ws + p.w; q.ldb = 4 * p.fk;
     q.m = T; q.n = D; q.k_bytes = (uint32_t)(4 * p.fk);
-    q.out.c = dX; q.out.ldc = lddx;
-    if (int rc = mi355_ffn_product(dev, op, kEpiPlain, "glu_backward (dX)", q, ws + p.sums, p.bytes - p.sums)) return rc;
+    q.out.c = dX; q.out.ldc = lddx; q.out.type = type;
+    if (int rc = mi355_launch_ffn_rows(dev, op, kEpiPlain, "glu_backward (dX)", q)) return rc;
   }
   if (dWg && p.dw_across) {
     c.a = ws + p.rows;
@@ -286,16 +330,6 @@ int mi355_launch_glu_backward(mi355_dev *dev, int type, int act, const void *dH,
     add_stretches(c, X, ldx, ws + p.x, T, D);
     c.out.c = dWg; c.c2 = dWu; c.out.ldc = lddw;
     if (int rc = mi355_launch_ffn_across(dev, op, true, "glu_backward (dW)", c, p.dw.slices, ws + p.sums)) return rc;
-  } else if (dWg) {
-    q.lda = q.ldb = 2 * p.tp;
-    q.b = ws + p.x;
-    q.m = F; q.n = D; q.k_bytes = (uint32_t)(2 * p.tp);
-    q.out.ldc = lddw;
-    for (int half = 0; half < 2; half++) {
-      q.a = ws + p.cols + half * p.fp * p.tp * 2;
-      q.out.c = half ? dWu : dWg;
-      if (int rc = mi355_ffn_product(dev, op, kEpiPlain, "glu_backward (dW)", q, ws + p.sums, p.bytes - p.sums)) return rc;
-    }
   }
-  return MI355_OK;
+  return g.count ? mi355_ffn_group(dev, op, "glu_backward", g, choice, ws + p.sums) : MI355_OK;
 }

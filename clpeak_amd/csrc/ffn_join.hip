@@ -6,15 +6,18 @@
 namespace {
 
 template <int OP, int EPI>
-__global__ void __launch_bounds__(256) ffn_join_kernel(FfnOut o, const int32_t *partial, uint32_t slices, uint64_t ldp, uint32_t m, uint32_t n) {
-  const uint64_t quads = (n + 3u) / 4u, at = (uint64_t)blockIdx.x * 256u + threadIdx.x;
-  if (at >= quads * m) return;
+__global__ void __launch_bounds__(256) ffn_join_kernel(FfnJoin j0, FfnJoin j1, FfnJoin j2) {
+  FfnJoin j = j0;
+  if (blockIdx.x >= j1.first) j = j1;
+  if (blockIdx.x >= j2.first) j = j2;
+  const uint64_t quads = (j.n + 3u) / 4u, at = (uint64_t)(blockIdx.x - j.first) * 256u + threadIdx.x;
+  if (at >= quads * j.m) return;
   const uint32_t row = (uint32_t)(at / quads), col = (uint32_t)(at % quads) * 4u;
-  const int32_t *from = partial + (uint64_t)row * ldp + col;
+  const int32_t *from = j.partial + (uint64_t)row * j.ldp + col;
   i32x4v s = *reinterpret_cast<const i32x4v *>(from);
 #pragma unroll 4
-  for (uint32_t k = 1; k < slices; k++) {
-    const i32x4v t = *reinterpret_cast<const i32x4v *>(from + (uint64_t)k * m * ldp);
+  for (uint32_t k = 1; k < j.slices; k++) {
+    const i32x4v t = *reinterpret_cast<const i32x4v *>(from + (uint64_t)k * j.m * j.ldp);
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       const int32_t x = s[e], y = t[e];
@@ -22,21 +25,28 @@ __global__ void __launch_bounds__(256) ffn_join_kernel(FfnOut o, const int32_t *
       else s[e] = __builtin_bit_cast(int32_t, __builtin_bit_cast(float, x) + __builtin_bit_cast(float, y));
     }
   }
-  ffn_finish4<OP, EPI>(o, row, col, n, s, s);
+  ffn_finish4<OP, EPI>(j.out, row, col, j.n, s, s);
 }
 
 template <int OP, int EPI>
-int launch(mi355_dev *dev, const char *what, const FfnProduct &p, uint32_t slices, const void *workspace) {
-  const uint64_t blocks = ((p.n + 3ull) / 4u * p.m + 255u) / 256u;
-  MI355_REQUIRE(dev, blocks <= 0xffffffull, "%s: %u x %u outputs are more than one launch takes", what, p.m, p.n);
-  ffn_join_kernel<OP, EPI><<<(uint32_t)blocks, 256, 0, dev->stream>>>(p.out, (const int32_t *)workspace, slices, mi355_ffn_slice_row(p.n), p.m, p.n);
-  MI355_LAUNCH_CHECK(dev, what);
-  return MI355_OK;
+void launch(mi355_dev *dev, const FfnJoin (&j)[3], uint32_t blocks) {
+  ffn_join_kernel<OP, EPI><<<blocks, 256, 0, dev->stream>>>(j[0], j[1], j[2]);
 }
 
 }  // namespace
 
-int mi355_launch_ffn_join(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p, uint32_t slices, const void *workspace) {
-  if (op == kQuadI8 && epi == kEpiScaled) return launch<kQuadI8, kEpiScaled>(dev, what, p, slices, workspace);
-  return op == kQuadBf16 ? launch<kQuadBf16, kEpiPlain>(dev, what, p, slices, workspace) : launch<kQuadF16, kEpiPlain>(dev, what, p, slices, workspace);
+int mi355_launch_ffn_join(mi355_dev *dev, int op, int epi, const char *what, FfnJoin *parts, uint32_t count) {
+  FfnJoin j[3] = {};
+  uint64_t blocks = 0;
+  for (uint32_t i = 0; i < 3; i++) {
+    if (i < count) j[i] = parts[i];
+    j[i].first = i < count ? (uint32_t)blocks : 0xffffffffu;
+    if (i < count) blocks += ((j[i].n + 3ull) / 4u * j[i].m + 255u) / 256u;
+    MI355_REQUIRE(dev, blocks <= 0xffffffull, "%s: %u x %u outputs are more than one launch takes", what, j[i].m, j[i].n);
+  }
+  if (op == kQuadI8 && epi == kEpiScaled) launch<kQuadI8, kEpiScaled>(dev, j, (uint32_t)blocks);
+  else if (op == kQuadBf16) launch<kQuadBf16, kEpiPlain>(dev, j, (uint32_t)blocks);
+  else launch<kQuadF16, kEpiPlain>(dev, j, (uint32_t)blocks);
+  MI355_LAUNCH_CHECK(dev, what);
+  return MI355_OK;
 }

@@ -20,17 +20,21 @@ constexpr uint32_t kMidTile = 64, kMidThreads = 256;
 constexpr uint32_t kMidSlab = kMidTile * kRowBytes, kMidSlot = 2 * kMidSlab, kMidSlots = 10, kMidAhead = 9;
 static_assert(kMidSlots * kMidSlot == kRingBytes && kMidAhead + 1 == kMidSlots, "the ring is the whole LDS of a CU");
 
-// Slice blockIdx.y of gridDim.y of K (kEpiPartial: its sums go to p.out.c as matrix number blockIdx.y there).
 template <int OP, int EPI>
-__global__ void __launch_bounds__(kMidThreads) ffn_mid_kernel(FfnProduct p, uint32_t tiles_n) {
+__global__ void __launch_bounds__(kMidThreads) ffn_mid_kernel(FfnLaunch<EPI> args) {
+  const FfnWork work = args.work();
+  const FfnProduct &p = work.p;
   constexpr bool kGated = epi_is_gated(EPI);
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t wm = wave / 2, wn = wave % 2;
-  const uint32_t tn = blockIdx.x % tiles_n, tm = blockIdx.x / tiles_n;
-  const uint32_t all = p.k_bytes / kRowBytes;
-  const uint32_t k0 = EPI == kEpiPartial ? (uint32_t)((uint64_t)all * blockIdx.y / gridDim.y) : 0u;
-  const uint32_t steps = EPI == kEpiPartial ? (uint32_t)((uint64_t)all * (blockIdx.y + 1u) / gridDim.y) - k0 : all;
+  const uint32_t tm = work.tile / work.tiles_n, tn = work.tile - tm * work.tiles_n;
+  uint32_t steps = p.k_bytes / kRowBytes, k0 = 0;
+  if constexpr (EPI == kEpiPlain || EPI == kEpiPartial) {   // (at most 2^19 steps and 16 slices)
+    const uint32_t all = steps;
+    k0 = all * work.slice / work.slices;
+    steps = all * (work.slice + 1u) / work.slices - k0;
+  }
   const uint32_t lda = (uint32_t)p.lda, ldb = (uint32_t)p.ldb;
 
   // global -> LDS: wave w fills rows [16w, 16w+16) of the A slab and of the B slab, 8 rows per instruction (rows past the
@@ -90,8 +94,7 @@ __global__ void __launch_bounds__(kMidThreads) ffn_mid_kernel(FfnProduct p, uint
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the fetches that ran ahead still write LDS
 
-  FfnOut o = p.out;
-  if constexpr (EPI == kEpiPartial) o.c = static_cast<float *>(o.c) + (uint64_t)blockIdx.y * p.m * o.ldc;
+  const FfnOut &o = p.out;
   const uint32_t g4 = 4u * (lane / 16u);
 #pragma unroll
   for (uint32_t i = 0; i < 2; i++) {
@@ -112,24 +115,39 @@ int launch_tiles(mi355_dev *dev, const char *what, const FfnProduct &p, uint32_t
   const uint32_t cols = epi_is_gated(EPI) ? 32 : 64;
   const uint64_t tiles_m = (p.m + 63ull) / 64u, tiles_n = (p.n + cols - 1ull) / cols;
   MI355_REQUIRE(dev, tiles_m * tiles_n <= 0xffffffull, "%s: %u x %u outputs are more than one launch takes", what, p.m, p.n);
-  ffn_mid_kernel<OP, EPI><<<dim3((uint32_t)(tiles_m * tiles_n), slices), kMidThreads, kRingBytes, dev->stream>>>(p, (uint32_t)tiles_n);
+  const FfnLaunch<EPI> args{p, (uint32_t)tiles_m, (uint32_t)tiles_n};
+  ffn_mid_kernel<OP, EPI><<<dim3((uint32_t)(tiles_m * tiles_n), slices), kMidThreads, kRingBytes, dev->stream>>>(args);
   MI355_LAUNCH_CHECK(dev, what);
   return MI355_OK;
 }
 template <int OP, int EPI>
 int launch(mi355_dev *dev, const char *what, const FfnProduct &p, uint32_t slices, void *workspace) {
-  if constexpr (EPI == kEpiPlain || EPI == kEpiScaled)
+  if constexpr (EPI == kEpiScaled)
     if (slices > 1) {
       if (int rc = launch_tiles<OP, kEpiPartial>(dev, what, mi355_ffn_slices_of(p, workspace), slices)) return rc;
-      return mi355_launch_ffn_join(dev, OP, EPI, what, p, slices, workspace);
+      FfnJoin join = mi355_ffn_join_of(p, slices, workspace);
+      return mi355_launch_ffn_join(dev, OP, EPI, what, &join, 1);
     }
   return launch_tiles<OP, EPI>(dev, what, p, 1);
+}
+template <int OP>
+int launch_group(mi355_dev *dev, const char *what, const FfnGroup &g) {
+  if (int rc = allow_full_lds(dev, &ffn_mid_kernel<OP, kEpiPlain>, kLdsFfnMid0 + ffn_kind(OP, kEpiPlain))) return rc;
+  FfnLaunch<kEpiPlain> args{g};
+  uint32_t blocks = 0;
+  if (int rc = mi355_ffn_lay_out_group(dev, what, args.g, kMidTile, blocks)) return rc;
+  ffn_mid_kernel<OP, kEpiPlain><<<blocks, kMidThreads, kRingBytes, dev->stream>>>(args);
+  MI355_LAUNCH_CHECK(dev, what);
+  return MI355_OK;
 }
 
 }  // namespace
 
 int mi355_launch_ffn_mid(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p, uint32_t slices, void *workspace) {
   if (op == kQuadI8) return epi == kEpiScaled ? launch<kQuadI8, kEpiScaled>(dev, what, p, slices, workspace) : launch<kQuadI8, kEpiGatedScaled>(dev, what, p, 1, nullptr);
-  if (op == kQuadBf16) return epi == kEpiPlain ? launch<kQuadBf16, kEpiPlain>(dev, what, p, slices, workspace) : launch<kQuadBf16, kEpiGated>(dev, what, p, 1, nullptr);
-  return epi == kEpiPlain ? launch<kQuadF16, kEpiPlain>(dev, what, p, slices, workspace) : launch<kQuadF16, kEpiGated>(dev, what, p, 1, nullptr);
+  if (epi != kEpiGated) return mi355_fail(dev, MI355_ERR_ARG, "%s: such products go in groups", what);
+  return op == kQuadBf16 ? launch<kQuadBf16, kEpiGated>(dev, what, p, 1, nullptr) : launch<kQuadF16, kEpiGated>(dev, what, p, 1, nullptr);
+}
+int mi355_launch_ffn_mid_group(mi355_dev *dev, int op, const char *what, FfnGroup g) {
+  return op == kQuadBf16 ? launch_group<kQuadBf16>(dev, what, g) : launch_group<kQuadF16>(dev, what, g);
 }

@@ -36,24 +36,25 @@ __device__ __forceinline__ void finish_columns(const FfnProduct &p, uint32_t row
   finish_tiles<OP, EPI, 3, JP>(p, row0, col0, lane, c);
 }
 
-// Slice blockIdx.y of gridDim.y of K (kEpiPartial: its sums go to p.out.c as matrix number blockIdx.y there).
 template <int OP, int EPI>
-__global__ void __launch_bounds__(kSmallThreads) ffn_small_kernel(FfnProduct p, uint32_t tiles_m, uint32_t tiles_n) {
+__global__ void __launch_bounds__(kSmallThreads) ffn_small_kernel(FfnLaunch<EPI> args) {
+  const FfnWork work = args.work();
+  const FfnProduct &p = work.p;
   constexpr bool kGated = epi_is_gated(EPI);
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const uint32_t tid = threadIdx.x, lane = tid % 64;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const uint32_t wm = wave / 2, wn = wave % 2;
   TileGrid grid;
-  grid.tiles_m = tiles_m; grid.tiles_n = tiles_n; grid.total = tiles_m * tiles_n;
-  grid.first = blockIdx.x; grid.stride = gridDim.x; grid.mine = 1;
+  grid.tiles_m = work.tiles_m; grid.tiles_n = work.tiles_n; grid.total = grid.stride = work.tiles_m * work.tiles_n;
+  grid.first = work.tile; grid.mine = 1;
   uint32_t tm, tn;
   tile_at(grid, 0, tm, tn);
   uint32_t steps = p.k_bytes / kRowBytes, k0 = 0;
-  if constexpr (EPI == kEpiPartial) {
+  if constexpr (EPI == kEpiPlain || EPI == kEpiPartial) {   // (at most 2^19 steps and 16 slices)
     const uint32_t all = steps;
-    k0 = (uint32_t)((uint64_t)all * blockIdx.y / gridDim.y);
-    steps = (uint32_t)((uint64_t)all * (blockIdx.y + 1u) / gridDim.y) - k0;
+    k0 = all * work.slice / work.slices;
+    steps = all * (work.slice + 1u) / work.slices - k0;
   }
   const uint32_t lda = (uint32_t)p.lda, ldb = (uint32_t)p.ldb;
   constexpr uint32_t kRing = kSmallSlots * kSmallSlot;
@@ -131,7 +132,6 @@ __global__ void __launch_bounds__(kSmallThreads) ffn_small_kernel(FfnProduct p, 
   // ahead of the last step still write LDS
   asm volatile("s_nop 15\n s_nop 15\n s_waitcnt vmcnt(0)" ::: "memory");
   const uint32_t row0 = tm * 128u + wm * 64u + lane % 16u, col0 = tn * (kGated ? 64u : 128u) + wn * (kGated ? 32u : 64u);
-  if constexpr (EPI == kEpiPartial) p.out.c = static_cast<float *>(p.out.c) + (uint64_t)blockIdx.y * p.m * p.out.ldc;
   finish_columns<OP, EPI, 0>(p, row0, col0, lane);
   if constexpr (!kGated) finish_columns<OP, EPI, 2>(p, row0, col0, lane);
 }
@@ -142,24 +142,39 @@ int launch_tiles(mi355_dev *dev, const char *what, const FfnProduct &p, uint32_t
   const uint32_t cols = epi_is_gated(EPI) ? 64 : 128;
   const uint64_t tiles_m = (p.m + 127ull) / 128u, tiles_n = (p.n + cols - 1ull) / cols;
   MI355_REQUIRE(dev, tiles_m * tiles_n <= 0xffffffull, "%s: %u x %u outputs are more than one launch takes", what, p.m, p.n);
-  ffn_small_kernel<OP, EPI><<<dim3((uint32_t)(tiles_m * tiles_n), slices), kSmallThreads, kRingBytes, dev->stream>>>(p, (uint32_t)tiles_m, (uint32_t)tiles_n);
+  const FfnLaunch<EPI> args{p, (uint32_t)tiles_m, (uint32_t)tiles_n};
+  ffn_small_kernel<OP, EPI><<<dim3((uint32_t)(tiles_m * tiles_n), slices), kSmallThreads, kRingBytes, dev->stream>>>(args);
   MI355_LAUNCH_CHECK(dev, what);
   return MI355_OK;
 }
 template <int OP, int EPI>
 int launch(mi355_dev *dev, const char *what, const FfnProduct &p, uint32_t slices, void *workspace) {
-  if constexpr (EPI == kEpiPlain || EPI == kEpiScaled)
+  if constexpr (EPI == kEpiScaled)
     if (slices > 1) {
       if (int rc = launch_tiles<OP, kEpiPartial>(dev, what, mi355_ffn_slices_of(p, workspace), slices)) return rc;
-      return mi355_launch_ffn_join(dev, OP, EPI, what, p, slices, workspace);
+      FfnJoin join = mi355_ffn_join_of(p, slices, workspace);
+      return mi355_launch_ffn_join(dev, OP, EPI, what, &join, 1);
     }
   return launch_tiles<OP, EPI>(dev, what, p, 1);
+}
+template <int OP>
+int launch_group(mi355_dev *dev, const char *what, const FfnGroup &g) {
+  if (int rc = allow_full_lds(dev, &ffn_small_kernel<OP, kEpiPlain>, kLdsFfnSmall0 + ffn_kind(OP, kEpiPlain))) return rc;
+  FfnLaunch<kEpiPlain> args{g};
+  uint32_t blocks = 0;
+  if (int rc = mi355_ffn_lay_out_group(dev, what, args.g, kSmallTile, blocks)) return rc;
+  ffn_small_kernel<OP, kEpiPlain><<<blocks, kSmallThreads, kRingBytes, dev->stream>>>(args);
+  MI355_LAUNCH_CHECK(dev, what);
+  return MI355_OK;
 }
 
 }  // namespace
 
 int mi355_launch_ffn_small(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p, uint32_t slices, void *workspace) {
   if (op == kQuadI8) return epi == kEpiScaled ? launch<kQuadI8, kEpiScaled>(dev, what, p, slices, workspace) : launch<kQuadI8, kEpiGatedScaled>(dev, what, p, 1, nullptr);
-  if (op == kQuadBf16) return epi == kEpiPlain ? launch<kQuadBf16, kEpiPlain>(dev, what, p, slices, workspace) : launch<kQuadBf16, kEpiGated>(dev, what, p, 1, nullptr);
-  return epi == kEpiPlain ? launch<kQuadF16, kEpiPlain>(dev, what, p, slices, workspace) : launch<kQuadF16, kEpiGated>(dev, what, p, 1, nullptr);
+  if (epi != kEpiGated) return mi355_fail(dev, MI355_ERR_ARG, "%s: such products go in groups", what);
+  return op == kQuadBf16 ? launch<kQuadBf16, kEpiGated>(dev, what, p, 1, nullptr) : launch<kQuadF16, kEpiGated>(dev, what, p, 1, nullptr);
+}
+int mi355_launch_ffn_small_group(mi355_dev *dev, int op, const char *what, FfnGroup g) {
+  return op == kQuadBf16 ? launch_group<kQuadBf16>(dev, what, g) : launch_group<kQuadF16>(dev, what, g);
 }

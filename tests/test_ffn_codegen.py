@@ -35,7 +35,7 @@ def kernels(text, name):
     return found
 
 
-@pytest.mark.parametrize("source, name, count", [("ffn_rows.hip", "ffn_rows_kernel", 24), ("ffn_mid.hip", "ffn_mid_kernel", 9), ("ffn_small.hip", "ffn_small_kernel", 9),
+@pytest.mark.parametrize("source, name, count", [("ffn_rows.hip", "ffn_rows_kernel", 24), ("ffn_mid.hip", "ffn_mid_kernel", 7), ("ffn_small.hip", "ffn_small_kernel", 7),
                                                  ("ffn_quad.hip", "ffn_quad_kernel", 8), ("ffn_across.hip", "ffn_across_kernel", 8), ("ffn_join.hip", "ffn_join_kernel", 3),
                                                  ("quantize.hip", "quantize_i8_kernel", 27), ("ffn_backward.hip", "glu_backward_prepare_kernel", 2)])
 def test_no_kernel_uses_memory_for_registers(asm, source, name, count):

@@ -243,7 +243,8 @@ def test_glu_backward(tiled, type, T, F, D):
     assert bool((room[ws.data_ptr() - room.data_ptr() + n:] == 0xFF).all())
 
 
-@pytest.mark.parametrize("T, F, D", [(4200, 320, 4096), (600, 4096, 512), (2048, 2752, 1024), (130, 8192, 256), (3000, 70, 2048)])
+@pytest.mark.parametrize("T, F, D", [(4200, 320, 4096), (600, 4096, 512), (2048, 2752, 1024), (130, 8192, 256), (3000, 70, 2048), (33, 2752, 1024), (100, 5000, 2048),
+                                     (8192, 500, 512), (1, 8192, 512), (16, 4099, 1024)])
 def test_glu_backward_larger(tiled, T, F, D):
     """Sizes at which the products are cut along their sums, go round the CUs more than once, and have rows left over for a
     launch of their own."""
