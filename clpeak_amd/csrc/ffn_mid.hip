@@ -5,8 +5,8 @@
 // slots of 16 KiB (64 rows of A and 64 of B, 128 bytes of K), nine of them being filled while the tenth is read.  That is
 // 72 KiB of weights on their way to each CU, 18 MiB to the part.
 //
-// Measured: 48x4096x16384 int8, 64 tiles in 4 slices, 67 MB of weights in 15.8 us (4.2 TB/s), with the join
-// 18.5 us; not cut 29.0 us.  128x4096x4096 int8 11.7 us, on 128x128 tiles 17.4 us.  Bound by the weights' way from memory.
+// Measured: 48x4096x16384 int8, 64 tiles in 4 slices, 67 MB of weights in 15.5 us (4.3 TB/s), with the join
+// 18.1 us; not cut 28.0 us.  128x4096x4096 int8 10.5 us, on 128x128 tiles 17.4 us.  Bound by the weights' way from memory.
 //
 // A step: wait for this wave's four loads of the slab (they complete in order, eight younger slabs may be in flight) and
 // for its own reads of the slab before; barrier; four loads into the slot that everybody has read; eight fragment reads,
@@ -95,16 +95,20 @@ __global__ void __launch_bounds__(kMidThreads) ffn_mid_kernel(FfnLaunch<EPI> arg
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the fetches that ran ahead still write LDS
 
   const FfnOut &o = p.out;
-  const uint32_t g4 = 4u * (lane / 16u);
+  const uint32_t row0 = tm * kMidTile + wm * 32u + lane % 16u;
+  if constexpr (kGated) {   // (no two neighbouring tiles: 16 channels of both matrices)
 #pragma unroll
-  for (uint32_t i = 0; i < 2; i++) {
-    const uint32_t row = tm * kMidTile + wm * 32u + 16u * i + lane % 16u;
-    if (row >= p.m) continue;
-    if constexpr (kGated) {
-      ffn_finish4<OP, EPI>(o, row, tn * 32u + wn * 16u + g4, p.n, acc[i][0], acc[i][1]);
-    } else {
-      ffn_finish4<OP, EPI>(o, row, tn * kMidTile + wn * 32u + g4, p.n, acc[i][0], acc[i][0]);
-      ffn_finish4<OP, EPI>(o, row, tn * kMidTile + wn * 32u + 16u + g4, p.n, acc[i][1], acc[i][1]);
+    for (uint32_t i = 0; i < 2; i++)
+      if (row0 + 16u * i < p.m) ffn_finish4<OP, EPI>(o, row0 + 16u * i, tn * 32u + wn * 16u + 4u * (lane / 16u), p.n, acc[i][0], acc[i][1]);
+  } else {
+    const uint32_t col0 = tn * kMidTile + wn * 32u;
+    FfnColumns<EPI> c;
+    c.load(o, col0, lane, p.n);
+#pragma unroll
+    for (uint32_t i = 0; i < 2; i++) {
+      float sa = 0.0f;
+      if constexpr (EPI == kEpiScaled) sa = o.sa[min(row0 + 16u * i, p.m - 1u)];
+      ffn_finish_pair<OP, EPI>(o, row0 + 16u * i, col0, lane, p.m, p.n, sa, c, acc[i], acc[i]);
     }
   }
 }
