@@ -36,7 +36,7 @@ MAD_F32, MAD_F16, MAD_F64, MAD_MP, MAD_BF16, MAD_I32, MAD_I8DP = range(7)
 (MFMA_F16_16x16x32, MFMA_BF16_16x16x32, MFMA_F16_32x32x16, MFMA_BF16_32x32x16, MFMA_I8_16x16x64,
  MFMA_FP8_16x16x128, MFMA_BF8_16x16x128, MFMA_MXFP6_E2M3, MFMA_MXFP6_E3M2, MFMA_MXFP4_E2M1) = range(10)
 SMFMAC_F16_16x16x64, SMFMAC_BF16_16x16x64, SMFMAC_FP8_16x16x128, SMFMAC_BF8_16x16x128, SMFMAC_I8_16x16x128 = range(5)
-GEMM_TILING_AUTO, GEMM_TILING_256, GEMM_TILING_128, GEMM_TILING_64 = range(4)
+GEMM_TILING_AUTO, GEMM_TILING_256, GEMM_TILING_128, GEMM_TILING_64, GEMM_TILING_256X128 = range(5)
 TYPE_BF16, TYPE_F16, TYPE_F32 = 0, 1, 2
 GLU_SILU, GLU_GELU, GLU_GELU_TANH, GLU_RELU = range(4)
 MATRIX_ON_HALF_THE_CUS = 0x200   # diagnosis: only the workgroups of the first 16 CUs of every XCD take part
@@ -296,7 +296,7 @@ class Device:
                                             sel0, sel1, d.ptr))
 
     def gemm_tiling(self, tiling):
-        """GEMM_TILING_AUTO / _256 / _128 for the 8- and 16-bit GEMM calls of this handle (and _64 for its feed-forward operators)."""
+        """GEMM_TILING_AUTO / _256 / _128 for the 8- and 16-bit GEMM calls of this handle (and _64 / _256X128 for its feed-forward operators)."""
         self._check(self.lib.mi355_gemm_tiling(self.h, tiling))
 
     def gemm_bf16(self, A, B, Cbuf, M, N, K):

@@ -38,12 +38,12 @@ struct FfnProduct {
 // ffn_rows.hip: at most 64 rows of A.  op: kQuadBf16 / kQuadF16 / kQuadI8.
 int mi355_launch_ffn_rows(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p);
 
-// ffn_quad.hip / ffn_small.hip: on 256x256 and on 128x128 tiles of sums (gated: of 256x128 / 128x64 outputs).
+// ffn_quad.hip / ffn_small.hip: on 256x256 and on 128x128 (tall: 256x128) tiles of sums (gated: half as many columns of outputs).
 int mi355_launch_ffn_quad(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p);
 // ffn_mid.hip: on 64x64 tiles of sums (gated: of 64x32 outputs), for some dozens of rows.
 // slices > 1 (kEpiScaled): K is cut into so many, `workspace` holds `slices` matrices of m rows of
 // mi355_ffn_slice_row(n) 32-bit sums, on 16 bytes.
-int mi355_launch_ffn_small(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p, uint32_t slices, void *workspace);
+int mi355_launch_ffn_small(mi355_dev *dev, int op, int epi, const char *what, bool tall, const FfnProduct &p, uint32_t slices, void *workspace);
 int mi355_launch_ffn_mid(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p, uint32_t slices, void *workspace);
 // kEpiPlain, on either: up to three products of 16-bit operands in one launch, each in slices of its own number.
 struct FfnGroup {
@@ -58,14 +58,14 @@ struct FfnGroup {
   int type;
 };
 struct FfnGroupChoice {
-  bool small;             // 128x128 tiles rather than 64x64
+  int kernel;             // (ffn.hip's number of it)
   uint32_t slices[3];
   double us;
 };
-// (ffn.hip: the longest walks first; tiles of edge x edge sums)
-int mi355_ffn_lay_out_group(mi355_dev *dev, const char *what, FfnGroup &g, uint32_t edge, uint32_t &blocks);
-int mi355_launch_ffn_small_group(mi355_dev *dev, int op, const char *what, FfnGroup g);
-int mi355_launch_ffn_mid_group(mi355_dev *dev, int op, const char *what, FfnGroup g);
+// (ffn.hip: the longest walks first; tiles of rows x cols sums)
+int mi355_ffn_lay_out_group(mi355_dev *dev, const char *what, FfnGroup &g, uint32_t rows, uint32_t cols, uint32_t &blocks);
+int mi355_launch_ffn_small_group(mi355_dev *dev, int op, const char *what, bool tall, const FfnGroup &g);
+int mi355_launch_ffn_mid_group(mi355_dev *dev, int op, const char *what, const FfnGroup &g);
 // ffn_join.hip: the second launch of products in slices, up to three of them.
 struct FfnJoin {
   FfnOut out;
@@ -130,11 +130,11 @@ struct FfnLaunch<kEpiPlain> {
   }
 };
 
-// Bits of mi355_dev::full_lds_allowed: the kernels of each tiling (the 256x256 one has one for each output type).
-constexpr int ffn_kind(int op, int epi, int type = 0) {
-  return op != kQuadI8 ? (op - kQuadBf16) * 3 + (epi == kEpiPartial ? 2 : epi_is_gated(epi) ? 1 : 0) : epi == kEpiPartial ? 12 : 6 + 3 * epi_is_gated(epi) + type;
+// Bits of mi355_dev::full_lds_allowed: 8 kernels on 256x256 tiles, on the others 7 for each shape of tile.
+constexpr int ffn_kind(int op, int epi) {
+  return op != kQuadI8 ? (op - kQuadBf16) * 2 + epi_is_gated(epi) : 4 + (epi == kEpiPartial ? 2 : epi_is_gated(epi));
 }
-enum { kLdsFfnQuad0 = 24, kLdsFfnSmall0 = 37, kLdsFfnMid0 = 50 };   // 13 each
+enum { kLdsFfnQuad0 = 24, kLdsFfnSmall0 = 32, kLdsFfnMid0 = 39, kLdsFfnTall0 = 46 };
 
 // ffn.hip: the product on the kernel that suits it, and the workspace that it can use.
 int mi355_ffn_product(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p, void *workspace, size_t workspace_bytes);

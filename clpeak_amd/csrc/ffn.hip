@@ -47,7 +47,7 @@ int check_sizes(mi355_dev *dev, const char *what, uint32_t rows, uint32_t cols, 
 // Which kernel: the one whose time, by what was measured of it, is least.  Each has its own limit.
 //   rows   everything the workgroups read, the weights once and the rows of A once for each workgroup, at 8.4 TB/s through
 //          the vector caches of all CUs, the weights at 5.5 TB/s from memory;
-//   tiles  of 64x64, 128x128 or 256x256 sums: rounds of tiles over the CUs, each the steps of K (128 bytes) times a step's
+//   tiles  of 64x64, 128x128, 256x128 or 256x256 sums: rounds of tiles over the CUs, each the steps of K (128 bytes) times a step's
 //          time and what surrounds the walk (the 256x256 tiles' workgroups go on to their next tile without a break).  A
 //          step takes longer as the part fills up and its clock falls.  At least the time of the weights, more where CUs
 //          are idle and fewer bytes are in flight.
@@ -57,7 +57,7 @@ int check_sizes(mi355_dev *dev, const char *what, uint32_t rows, uint32_t cols, 
 // mi355_gemm_tiling pins a tiling, whatever the number of rows.
 namespace {
 
-enum Kernel { kOnRows, kOn64, kOn128, kOn256 };
+enum Kernel { kOnRows, kOn64, kOn128, kOn256x128, kOn256 };
 struct Choice {
   Kernel kernel = kOn256;
   uint32_t slices = 1;
@@ -66,11 +66,13 @@ struct Choice {
 struct Tiling {
   Kernel kernel;
   int pin;
-  double edge, step_us, full_step_us, round_us, once_us, weights;   // (the weights' bytes per us)
+  double rows, cols, step_us, full_step_us, round_us, once_us, weights;   // (the weights' bytes per us)
 };
-constexpr Tiling kTilings[] = {{kOn64, MI355_GEMM_TILING_64, 64, 0.20, 0.32, 4.0, 1.0, 5.5e6},
-                               {kOn128, MI355_GEMM_TILING_128, 128, 0.30, 0.47, 5.0, 0.0, 4.5e6},
-                               {kOn256, MI355_GEMM_TILING_256, 256, 0.85, 1.30, 4.0, 10.0, 4.5e6}};
+constexpr Tiling kTilings[] = {{kOn64, MI355_GEMM_TILING_64, 64, 64, 0.20, 0.32, 4.0, 1.0, 5.5e6},
+                               {kOn128, MI355_GEMM_TILING_128, 128, 128, 0.30, 0.47, 5.0, 0.0, 4.5e6},
+                               {kOn256x128, MI355_GEMM_TILING_256X128, 256, 128, 0.55, 0.85, 7.0, 0.0, 4.5e6},
+                               {kOn256, MI355_GEMM_TILING_256, 256, 256, 0.85, 1.30, 4.0, 10.0, 4.5e6}};
+constexpr const Tiling &tiling_of(Kernel k) { return kTilings[k - kOn64]; }
 
 constexpr uint32_t kMostSlices = 16;
 
@@ -79,7 +81,7 @@ double columns_of_sums(int epi, uint32_t n) { return epi_is_gated(epi) ? 2.0 * n
 
 double tiling_us(const Tiling &t, double cus, uint32_t m, uint32_t n, double sums_n, uint32_t k_bytes, uint32_t slices) {
   const double steps = std::ceil(k_bytes / 128u / (double)slices), weights_us = sums_n * k_bytes / t.weights;
-  const double tiles = std::ceil(m / t.edge) * std::ceil(sums_n / t.edge) * slices;
+  const double tiles = std::ceil(m / t.rows) * std::ceil(sums_n / t.cols) * slices;
   const double busy = std::min(1.0, tiles / cus), rounds = std::ceil(tiles / cus);
   const double step = t.step_us + (t.full_step_us - t.step_us) * busy;
   double us = t.once_us + std::max(weights_us * (1.6 - 0.6 * busy) + t.round_us, rounds * (steps * step + t.round_us));
@@ -120,7 +122,7 @@ Division divide(const mi355_dev *dev, int epi, uint32_t m, uint32_t n, uint32_t 
   if (rows < 256.0 || rows >= m) return d;
   const uint32_t main_rows = (uint32_t)rows;
   const Choice rest = choose(dev, epi, m - main_rows, n, k_bytes, can_slice);
-  const double us = tiling_us(kTilings[2], cus, main_rows, n, sums_n, k_bytes, 1) + rest.us;
+  const double us = tiling_us(tiling_of(kOn256), cus, main_rows, n, sums_n, k_bytes, 1) + rest.us;
   if (us < d.us) { d.main_rows = main_rows; d.rest = rest; d.us = us; }
   return d;
 }
@@ -135,8 +137,8 @@ size_t division_bytes(const Division &d, uint32_t m, uint32_t n) {
 int launch(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p, const Choice &c, void *workspace) {
   if (c.kernel == kOnRows) return mi355_launch_ffn_rows(dev, op, epi, what, p);
   if (c.kernel == kOn64) return mi355_launch_ffn_mid(dev, op, epi, what, p, c.slices, workspace);
-  if (c.kernel == kOn128) return mi355_launch_ffn_small(dev, op, epi, what, p, c.slices, workspace);
-  return mi355_launch_ffn_quad(dev, op, epi, what, p);
+  if (c.kernel == kOn256) return mi355_launch_ffn_quad(dev, op, epi, what, p);
+  return mi355_launch_ffn_small(dev, op, epi, what, c.kernel == kOn256x128, p, c.slices, workspace);
 }
 
 }  // namespace
@@ -187,7 +189,7 @@ double last_end(double cus, Workgroups (&w)[3], uint32_t kinds) {
 // Slices of about as many steps for all of them, so that no walk outlasts the others.
 FfnGroupChoice mi355_choose_ffn_group(const mi355_dev *dev, const FfnGroup &g) {
   const double cus = count_of_cus(dev);
-  FfnGroupChoice best{false, {1, 1, 1}, 1e30};
+  FfnGroupChoice best{kOn128, {1, 1, 1}, 1e30};
   uint32_t longest = 1;
   for (uint32_t i = 0; i < g.count; i++) longest = std::max(longest, g.of[i].k_bytes / 128u);
   for (const Tiling &t : kTilings) {
@@ -195,10 +197,10 @@ FfnGroupChoice mi355_choose_ffn_group(const mi355_dev *dev, const FfnGroup &g) {
     double weights_us = 0.0, tiles[3] = {};
     for (uint32_t i = 0; i < g.count; i++) {
       weights_us += (double)g.of[i].n * g.of[i].k_bytes / t.weights;
-      tiles[i] = std::ceil(g.of[i].m / t.edge) * std::ceil(g.of[i].n / t.edge);
+      tiles[i] = std::ceil(g.of[i].m / t.rows) * std::ceil(g.of[i].n / t.cols);
     }
     for (uint32_t s = 1; s <= kMostSlices && (s == 1 || s * 4u <= longest); s++) {
-      FfnGroupChoice c{t.kernel == kOn128, {1, 1, 1}, 0.0};
+      FfnGroupChoice c{t.kernel, {1, 1, 1}, 0.0};
       Workgroups w[3] = {};
       double steps_of[3] = {}, join = 0.0;
       for (uint32_t i = 0; i < g.count; i++) {
@@ -232,14 +234,14 @@ size_t mi355_ffn_group_workspace(const FfnGroup &g, const FfnGroupChoice &c) {
   return (size_t)bytes;
 }
 
-int mi355_ffn_lay_out_group(mi355_dev *dev, const char *what, FfnGroup &g, uint32_t edge, uint32_t &blocks) {
+int mi355_ffn_lay_out_group(mi355_dev *dev, const char *what, FfnGroup &g, uint32_t rows, uint32_t cols, uint32_t &blocks) {
   std::stable_sort(g.of, g.of + g.count, [](const FfnGroup::One &a, const FfnGroup::One &b) { return a.k_bytes / a.slices > b.k_bytes / b.slices; });
   uint64_t first = 0;
   for (uint32_t i = 0; i < 3; i++) {
     FfnGroup::One &o = g.of[i];
     o.first = i < g.count ? (uint32_t)first : 0xffffffffu;
     if (i >= g.count) continue;
-    const uint64_t tiles_m = (o.m + (uint64_t)edge - 1u) / edge, tiles_n = (o.n + (uint64_t)edge - 1u) / edge;
+    const uint64_t tiles_m = (o.m + (uint64_t)rows - 1u) / rows, tiles_n = (o.n + (uint64_t)cols - 1u) / cols;
     MI355_REQUIRE(dev, tiles_m * tiles_n <= 0xffffffull && first + tiles_m * tiles_n * o.slices <= 0xffffffull, "%s: %u x %u outputs are more than one launch takes", what, o.m, o.n);
     o.tiles_m = (uint32_t)tiles_m; o.tiles_n = (uint32_t)tiles_n;
     first += tiles_m * tiles_n * o.slices;
@@ -264,13 +266,13 @@ int mi355_ffn_group(mi355_dev *dev, int op, const char *what, const FfnGroup &gr
     o.ldc = mi355_ffn_slice_row(o.n);
     workspace += o.slices * (uint64_t)o.m * o.ldc * 4u;
   }
-  if (int rc = c.small ? mi355_launch_ffn_small_group(dev, op, what, g) : mi355_launch_ffn_mid_group(dev, op, what, g)) return rc;
+  if (int rc = c.kernel == kOn64 ? mi355_launch_ffn_mid_group(dev, op, what, g) : mi355_launch_ffn_small_group(dev, op, what, c.kernel == kOn256x128, g)) return rc;
   return joins ? mi355_launch_ffn_join(dev, op, kEpiPlain, what, join, joins) : MI355_OK;
 }
 
 AcrossChoice mi355_choose_ffn_across(const mi355_dev *dev, uint32_t m, uint32_t parts, uint32_t n, uint32_t steps) {
   const double cus = count_of_cus(dev);
-  const Tiling &t = kTilings[2];
+  const Tiling &t = tiling_of(kOn256);
   auto best = [&](uint32_t rows, uint32_t &slices) {
     double least = 1e30;
     for (uint32_t s = 1; s <= 16u && (s == 1 || s * 4u <= steps); s++) {

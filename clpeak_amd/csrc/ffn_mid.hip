@@ -139,7 +139,7 @@ int launch_group(mi355_dev *dev, const char *what, const FfnGroup &g) {
   if (int rc = allow_full_lds(dev, &ffn_mid_kernel<OP, kEpiPlain>, kLdsFfnMid0 + ffn_kind(OP, kEpiPlain))) return rc;
   FfnLaunch<kEpiPlain> args{g};
   uint32_t blocks = 0;
-  if (int rc = mi355_ffn_lay_out_group(dev, what, args.g, kMidTile, blocks)) return rc;
+  if (int rc = mi355_ffn_lay_out_group(dev, what, args.g, kMidTile, kMidTile, blocks)) return rc;
   ffn_mid_kernel<OP, kEpiPlain><<<blocks, kMidThreads, kRingBytes, dev->stream>>>(args);
   MI355_LAUNCH_CHECK(dev, what);
   return MI355_OK;
@@ -152,6 +152,6 @@ int mi355_launch_ffn_mid(mi355_dev *dev, int op, int epi, const char *what, cons
   if (epi != kEpiGated) return mi355_fail(dev, MI355_ERR_ARG, "%s: such products go in groups", what);
   return op == kQuadBf16 ? launch<kQuadBf16, kEpiGated>(dev, what, p, 1, nullptr) : launch<kQuadF16, kEpiGated>(dev, what, p, 1, nullptr);
 }
-int mi355_launch_ffn_mid_group(mi355_dev *dev, int op, const char *what, FfnGroup g) {
+int mi355_launch_ffn_mid_group(mi355_dev *dev, int op, const char *what, const FfnGroup &g) {
   return op == kQuadBf16 ? launch_group<kQuadBf16>(dev, what, g) : launch_group<kQuadF16>(dev, what, g);
 }

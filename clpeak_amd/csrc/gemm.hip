@@ -212,7 +212,8 @@ int launch_quad(mi355_dev *dev, int op, const char *what, const void *A, const v
 
 extern "C" int mi355_gemm_tiling(mi355_dev *dev, int tiling) {
   if (!dev) return mi355_fail(nullptr, MI355_ERR_ARG, "null device handle");
-  MI355_REQUIRE(dev, tiling == MI355_GEMM_TILING_AUTO || tiling == MI355_GEMM_TILING_256 || tiling == MI355_GEMM_TILING_128 || tiling == MI355_GEMM_TILING_64,
+  MI355_REQUIRE(dev, tiling == MI355_GEMM_TILING_AUTO || tiling == MI355_GEMM_TILING_256 || tiling == MI355_GEMM_TILING_128 || tiling == MI355_GEMM_TILING_64 ||
+                tiling == MI355_GEMM_TILING_256X128,
                 "gemm_tiling: unknown tiling %d", tiling);
   dev->gemm_tiling = tiling;
   return MI355_OK;

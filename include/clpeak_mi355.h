@@ -290,12 +290,13 @@ int mi355_gemm_fp8_e5m2(mi355_dev *dev, const uint8_t *A, const uint8_t *B, uint
  * 256 CUs), 256 otherwise.  The 256 tiling needs M and N to be multiples of 256: a product with a multiple of 128 only
  * runs on the 128 tiling under AUTO and is refused under 256.  Results of the two agree within rounding (int8 exactly).
  * The feed-forward operators further down, whose sizes need not be multiples of anything, take it too: under AUTO they
- * choose by the time each tiling is measured to need, among them one of 64x64 tiles (64: pinned; the five calls above,
- * which have no such tiling, take it as AUTO) and a kernel for few rows that has none. */
+ * choose by the time each tiling is measured to need, among them tilings of 64x64 and 256x128 (pinned likewise; the five
+ * calls above, which have neither, take them as AUTO) and a kernel for few rows that has no tiles. */
 #define MI355_GEMM_TILING_AUTO 0
 #define MI355_GEMM_TILING_256  1
 #define MI355_GEMM_TILING_128  2
 #define MI355_GEMM_TILING_64   3
+#define MI355_GEMM_TILING_256X128 4
 int mi355_gemm_tiling(mi355_dev *dev, int tiling);
 /*   "fp32" of runRocblas (src/rocm/rocblas.cpp:246-254, rocblas_sgemm): fp32 operands, accumulation
  *          and output, on the fp32 matrix instruction; M, N multiples of 256, K a multiple of 32;

@@ -32,10 +32,11 @@ def dv():
     d.close()
 
 
-@pytest.fixture(params=["auto", "256", "128", "64"])
+@pytest.fixture(params=["auto", "256", "128", "64", "256x128"])
 def tiled(dv, request):
-    """The library's own choice of kernel (one for few rows, three tilings) and each tiling pinned."""
-    dv.gemm_tiling({"auto": capi.GEMM_TILING_AUTO, "256": capi.GEMM_TILING_256, "128": capi.GEMM_TILING_128, "64": capi.GEMM_TILING_64}[request.param])
+    """The library's own choice of kernel (one for few rows, four tilings) and each tiling pinned."""
+    dv.gemm_tiling({"auto": capi.GEMM_TILING_AUTO, "256": capi.GEMM_TILING_256, "128": capi.GEMM_TILING_128, "64": capi.GEMM_TILING_64,
+                     "256x128": capi.GEMM_TILING_256X128}[request.param])
     yield dv
     dv.gemm_tiling(capi.GEMM_TILING_AUTO)
 
