@@ -52,6 +52,7 @@ struct FfnGroup {
     uint64_t lda, ldb, ldc;
     void *c;
     uint32_t m, n, k_bytes, slices;
+    uint32_t pairs;                     // 1: the result is the sum of the upper and the lower half of the rows
     uint32_t tiles_m, tiles_n, first;   // (the launch's: the number of the product's first workgroup)
   } of[3];
   uint32_t count;
@@ -83,8 +84,9 @@ inline FfnProduct mi355_ffn_slices_of(const FfnProduct &p, void *workspace) {
   q.out.type = MI355_TYPE_F32;
   return q;
 }
-inline FfnJoin mi355_ffn_join_of(const FfnProduct &p, uint32_t slices, const void *workspace) {
-  return {p.out, static_cast<const int32_t *>(workspace), mi355_ffn_slice_row(p.n), p.m, p.n, slices, 0};
+// (pairs: each slice's matrix is two of half as many rows)
+inline FfnJoin mi355_ffn_join_of(const FfnProduct &p, uint32_t slices, bool pairs, const void *workspace) {
+  return {p.out, static_cast<const int32_t *>(workspace), mi355_ffn_slice_row(p.n), pairs ? p.m / 2u : p.m, p.n, pairs ? 2u * slices : slices, 0};
 }
 
 // What the kernels on 64x64 and 128x128 tiles are given, and what a workgroup makes of it: a tile of a product, and a slice
@@ -115,7 +117,7 @@ struct FfnLaunch<kEpiPlain> {
     FfnGroup::One o;
 #define MI355_PICK(x) o.x = third ? g.of[2].x : second ? g.of[1].x : g.of[0].x
     MI355_PICK(a); MI355_PICK(b); MI355_PICK(lda); MI355_PICK(ldb); MI355_PICK(ldc); MI355_PICK(c);
-    MI355_PICK(m); MI355_PICK(n); MI355_PICK(k_bytes); MI355_PICK(slices); MI355_PICK(tiles_m); MI355_PICK(tiles_n); MI355_PICK(first);
+    MI355_PICK(m); MI355_PICK(n); MI355_PICK(k_bytes); MI355_PICK(slices); MI355_PICK(pairs); MI355_PICK(tiles_m); MI355_PICK(tiles_n); MI355_PICK(first);
 #undef MI355_PICK
     const uint32_t at = blockIdx.x - o.first, tiles = o.tiles_m * o.tiles_n;
     FfnWork w{};
@@ -124,7 +126,7 @@ struct FfnLaunch<kEpiPlain> {
     w.tiles_m = o.tiles_m; w.tiles_n = o.tiles_n;
     w.slice = at / tiles; w.tile = at - w.slice * tiles; w.slices = o.slices;
     w.p.out.ldc = o.ldc;
-    w.p.out.type = o.slices > 1u ? MI355_TYPE_F32 : g.type;
+    w.p.out.type = o.slices > 1u || o.pairs ? MI355_TYPE_F32 : g.type;
     w.p.out.c = static_cast<uint8_t *>(o.c) + (o.slices > 1u ? (uint64_t)w.slice * o.m * o.ldc * 4u : 0u);
     return w;
   }

@@ -207,7 +207,7 @@ FfnGroupChoice mi355_choose_ffn_group(const mi355_dev *dev, const FfnGroup &g) {
         const uint32_t steps = g.of[i].k_bytes / 128u;
         c.slices[i] = std::max(1u, (steps * s + longest / 2u) / longest);
         while (c.slices[i] > 1u && c.slices[i] * 4u > steps) c.slices[i]--;
-        if (c.slices[i] > 1u) join += (double)g.of[i].m * g.of[i].n * (c.slices[i] * 6.0 + 2.0) / 4e6;
+        if (c.slices[i] > 1u || g.of[i].pairs) join += (double)g.of[i].m * g.of[i].n * (c.slices[i] * 6.0 + 2.0) / 4e6;
         steps_of[i] = std::ceil(steps / (double)c.slices[i]);
       }
       double step = t.full_step_us, end = 0.0;
@@ -230,7 +230,7 @@ FfnGroupChoice mi355_choose_ffn_group(const mi355_dev *dev, const FfnGroup &g) {
 size_t mi355_ffn_group_workspace(const FfnGroup &g, const FfnGroupChoice &c) {
   uint64_t bytes = 0;
   for (uint32_t i = 0; i < g.count; i++)
-    if (c.slices[i] > 1u) bytes += c.slices[i] * (uint64_t)g.of[i].m * mi355_ffn_slice_row(g.of[i].n) * 4u;
+    if (c.slices[i] > 1u || g.of[i].pairs) bytes += c.slices[i] * (uint64_t)g.of[i].m * mi355_ffn_slice_row(g.of[i].n) * 4u;
   return (size_t)bytes;
 }
 
@@ -257,11 +257,11 @@ int mi355_ffn_group(mi355_dev *dev, int op, const char *what, const FfnGroup &gr
   for (uint32_t i = 0; i < g.count; i++) {
     FfnGroup::One &o = g.of[i];
     o.slices = c.slices[i];
-    if (o.slices <= 1u) continue;
+    if (o.slices <= 1u && !o.pairs) continue;
     FfnProduct p{};
     p.m = o.m; p.n = o.n;
     p.out.c = o.c; p.out.ldc = o.ldc; p.out.type = g.type;
-    join[joins++] = mi355_ffn_join_of(p, o.slices, workspace);
+    join[joins++] = mi355_ffn_join_of(p, o.slices, o.pairs, workspace);
     o.c = workspace;
     o.ldc = mi355_ffn_slice_row(o.n);
     workspace += o.slices * (uint64_t)o.m * o.ldc * 4u;

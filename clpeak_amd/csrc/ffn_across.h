@@ -17,8 +17,9 @@ struct FfnAcross {
   } b[4];
   FfnOut out;             // c, ldc, type
   void *c2;
+  bool pairs;             // C is the sum of the upper and the lower half of the m rows
 };
-// slices > 1: the sum is cut into so many, `workspace` holds slices x parts matrices of m rows of n 32-bit sums, on 16 bytes.
+// slices > 1: the sum is cut into so many; then, and where C is one of pairs, `workspace` holds slices x parts matrices of m rows of n 32-bit sums, on 16 bytes.
 int mi355_launch_ffn_across(mi355_dev *dev, int op, bool across_a, const char *what, const FfnAcross &p, uint32_t slices, uint8_t *workspace);
 
 // How such a product is best launched (ffn.hip), and the time expected of it: the rows behind main_rows (if that is not 0)

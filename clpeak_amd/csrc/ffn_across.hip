@@ -292,7 +292,7 @@ int launch(mi355_dev *dev, const char *what, const FfnAcross &p, uint32_t slices
 }
 template <int OP, bool ACROSS_A, int TYPE>
 int launch_slices(mi355_dev *dev, const char *what, const FfnAcross &p, uint32_t slices, uint8_t *workspace) {
-  if (slices <= 1) return launch<OP, ACROSS_A, kEpiPlain, TYPE>(dev, what, p, 1);
+  if (slices <= 1 && !p.pairs) return launch<OP, ACROSS_A, kEpiPlain, TYPE>(dev, what, p, 1);
   const uint64_t part = slices * (uint64_t)p.m * p.n * 4u;
   FfnAcross q = p;
   q.out.c = workspace;
@@ -305,7 +305,7 @@ int launch_slices(mi355_dev *dev, const char *what, const FfnAcross &p, uint32_t
     o.m = p.m; o.n = p.n;
     o.out = p.out;
     if (i) o.out.c = p.c2;
-    join[i] = mi355_ffn_join_of(o, slices, workspace + i * part);
+    join[i] = mi355_ffn_join_of(o, slices, p.pairs, workspace + i * part);
   }
   return mi355_launch_ffn_join(dev, OP, kEpiPlain, what, join, p.parts);
 }

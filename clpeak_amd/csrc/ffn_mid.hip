@@ -129,7 +129,7 @@ int launch(mi355_dev *dev, const char *what, const FfnProduct &p, uint32_t slice
   if constexpr (EPI == kEpiScaled)
     if (slices > 1) {
       if (int rc = launch_tiles<OP, kEpiPartial>(dev, what, mi355_ffn_slices_of(p, workspace), slices)) return rc;
-      FfnJoin join = mi355_ffn_join_of(p, slices, workspace);
+      FfnJoin join = mi355_ffn_join_of(p, slices, false, workspace);
       return mi355_launch_ffn_join(dev, OP, EPI, what, &join, 1);
     }
   return launch_tiles<OP, EPI>(dev, what, p, 1);

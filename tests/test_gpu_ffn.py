@@ -208,9 +208,11 @@ def test_glu_backward(tiled, type, T, F, D):
     dh, G, U = operand(g, T, F, ldd, dt), operand(g, T, F, ldg, dt, 1.5), operand(g, T, F, ldg, dt)
     G64, U64, d64 = G.double(), U.double(), dh.double()
     dG, dU = d64 * U64 * grad64(act, G64), d64 * act64(act, G64)
-    # rounded to the type before the products, on top of what the activations are off
-    oG = UNIT[dt] * dG.abs() + TINY[dt] + (d64 * U64).abs() * (grad_off(act, G64) + 4 * E)
-    oU = UNIT[dt] * dU.abs() + TINY[dt] + d64.abs() * (act_off(act, G64) + 4 * E)
+    # rounded to the type before the products, on top of what the activations are off; few values as two of the type,
+    # the second of which is what the first is off, at most a unit of the value, and off by a unit of that
+    unit = UNIT[dt] ** 2 if T * F <= 32768 else UNIT[dt]
+    oG = unit * dG.abs() + TINY[dt] + (d64 * U64).abs() * (grad_off(act, G64) + 4 * E)
+    oU = unit * dU.abs() + TINY[dt] + d64.abs() * (act_off(act, G64) + 4 * E)
     w64g, w64u, x64 = wg.double(), wu.double(), x.double()
     n = dv.glu_backward_workspace(T, F, D)
     room = torch.full((n + 512,), 0xFF, dtype=torch.uint8, device="cuda")     # (0xffff is a NaN of both types)
@@ -245,7 +247,8 @@ def test_glu_backward(tiled, type, T, F, D):
 
 
 @pytest.mark.parametrize("T, F, D", [(4200, 320, 4096), (600, 4096, 512), (2048, 2752, 1024), (130, 8192, 256), (3000, 70, 2048), (33, 2752, 1024), (100, 5000, 2048),
-                                     (8192, 500, 512), (1, 8192, 512), (16, 4099, 1024)])
+                                     (8192, 500, 512), (1, 8192, 512), (16, 4099, 1024), (32, 1000, 4096), (33, 992, 64), (33, 993, 64), (450, 70, 1024), (2000, 16, 8192),
+                                     (256, 128, 256)])
 def test_glu_backward_larger(tiled, T, F, D):
     """Sizes at which the products are cut along their sums, go round the CUs more than once, and have rows left over for a
     launch of their own."""
