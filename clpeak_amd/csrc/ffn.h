@@ -5,6 +5,7 @@
 #include "internal.h"
 #include "mfma_common.h"
 #include "gemm_quad.h"
+#include "gemm_ring.h"
 
 // What becomes of the sums.
 enum FfnEpi {
@@ -202,6 +203,20 @@ __device__ __forceinline__ void ffn_act_grad(int act, float x, float &a, float &
     a = x < 0.0f ? 0.0f : x;
     da = x > 0.0f ? 1.0f : x <= 0.0f ? 0.0f : x;
   }
+}
+
+// ---- the order of the tiles --------------------------------------------------------------------------------------------
+// tile_at's, and where the number of tiles is no multiple of the XCDs' (8) still consecutive tiles for each XCD: neighbours
+// share rows of both operands, and where rows of C do not start on lines also the lines between them, which an L2 can
+// only complete if both are its own.
+__device__ __forceinline__ void ffn_tile_at(const TileGrid &g, uint32_t round, uint32_t &tm, uint32_t &tn) {
+  if (g.total % 8u == 0u) return tile_at(g, round, tm, tn);
+  const uint32_t id = g.first + round * g.stride, xcd = id % 8u, rest = g.total % 8u;
+  const uint32_t lin = xcd * (g.total / 8u) + min(xcd, rest) + id / 8u;
+  const uint32_t per_group = 4u * g.tiles_n, group = lin / per_group, in_group = lin - group * per_group;
+  const uint32_t rows_here = min(4u, g.tiles_m - group * 4u);
+  tn = in_group / rows_here;
+  tm = group * 4u + in_group - tn * rows_here;
 }
 
 // ---- stores of narrow values -----------------------------------------------------------------------------------------

@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(kQuadThreads) ffn_across_kernel(FfnAcross p, u
   w.step_a = ACROSS_A ? 64ull * lda : (uint64_t)kRowBytes;
   auto place = [&](uint32_t rnd, uint32_t pos) __attribute__((always_inline)) {   // the stream stands on slab `pos` of the tile of round `rnd`
     uint32_t tm, tn;
-    tile_at(grid, rnd, tm, tn);
+    ffn_tile_at(grid, rnd, tm, tn);
     const uint32_t slab = k0 + pos;
     if constexpr (ACROSS_A) {
       const uint32_t part = tm / tiles_part, col0 = (tm - part * tiles_part) * 256u;
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(kQuadThreads) ffn_across_kernel(FfnAcross p, u
     bool done = false;
     if (left == 0u) {
       uint32_t tm, tn;
-      tile_at(grid, round, tm, tn);
+      ffn_tile_at(grid, round, tm, tn);
       FfnProduct o{};
       o.m = p.m; o.n = p.n;
       o.out = p.out;

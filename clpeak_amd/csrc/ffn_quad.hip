@@ -31,7 +31,7 @@ __global__ void __launch_bounds__(kQuadThreads) ffn_quad_kernel(FfnProduct p, ui
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const uint32_t wm = wave / 2, wn = wave % 2;
   const TileGrid grid = tiles_of_workgroup(tiles_m, tiles_n);
-  const bool many_rounds = grid.total >= Finish<OP, EPI, TYPE>::kManyRounds * grid.stride;
+  const bool many_rounds = grid.total >= Finish<OP, EPI, TYPE>::kManyRounds * grid.stride && Finish<OP, EPI, TYPE>::on_64_bytes(p.out);
   const uint32_t k_bytes = p.k_bytes, steps = k_bytes / kRowBytes;
   const uint32_t lda = (uint32_t)p.lda, ldb = (uint32_t)p.ldb;
   const uint32_t lds_base = (uint32_t)(uintptr_t)lds;
@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(kQuadThreads) ffn_quad_kernel(FfnProduct p, ui
   const uint32_t k_rot = (grid.first % 8u) * (steps / 8u);
   auto rows_of = [&](uint32_t rnd) {
     uint32_t tm, tn;
-    tile_at(grid, rnd, tm, tn);
+    ffn_tile_at(grid, rnd, tm, tn);
     const uint8_t *b = kGated && (wave & 1u) ? p.b2 : p.b;
     const uint32_t a_row = min(tm * 256u + wave * 64u, p.m - 1u);
     const uint32_t b_row = min(kGated ? tn * 128u + wave / 2u * 64u : tn * 256u + wave * 64u, p.n - 1u);
@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(kQuadThreads) ffn_quad_kernel(FfnProduct p, ui
     bool done = false;
     if (left == 0u) {
       uint32_t tm, tn;
-      tile_at(grid, round, tm, tn);
+      ffn_tile_at(grid, round, tm, tn);
       Finish<OP, EPI, TYPE>{p, tm * 256u + wm * 128u + lane % 16u, tn * kCols + wn * (kCols / 2u), lane, many_rounds}.run();
       left = steps;
       w.first = 1;

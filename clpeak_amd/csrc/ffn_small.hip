@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(kSmallThreads) ffn_small_kernel(FfnLaunch<EPI>
   grid.tiles_m = work.tiles_m; grid.tiles_n = work.tiles_n; grid.total = grid.stride = work.tiles_m * work.tiles_n;
   grid.first = work.tile; grid.mine = 1;
   uint32_t tm, tn;
-  tile_at(grid, 0, tm, tn);
+  ffn_tile_at(grid, 0, tm, tn);
   uint32_t steps = p.k_bytes / kRowBytes, k0 = 0;
   if constexpr (EPI == kEpiPlain || EPI == kEpiPartial) {   // (at most 2^19 steps and 16 slices)
     const uint32_t all = steps;
