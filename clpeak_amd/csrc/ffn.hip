@@ -45,8 +45,8 @@ int check_sizes(mi355_dev *dev, const char *what, uint32_t rows, uint32_t cols, 
 }  // namespace
 
 // Which kernel: the one whose time, by what was measured of it, is least.  Each has its own limit.
-//   rows   everything the workgroups read, the weights once and the rows of A once for each workgroup, at 8.4 TB/s through
-//          the vector caches of all CUs, the weights at 5.5 TB/s from memory;
+//   rows   what the workgroups of one CU read, their weights and all rows of A each, at 33 KB a microsecond through
+//          its vector cache, and what surrounds a walk; at least the weights at 5.5 TB/s from memory;
 //   tiles  of 64x64, 128x128, 256x128 or 256x256 sums: rounds of tiles over the CUs, each the steps of K (128 bytes) times a step's
 //          time and what surrounds the walk (the 256x256 tiles' workgroups go on to their next tile without a break).  A
 //          step takes longer as the part fills up and its clock falls.  At least the time of the weights, more where CUs
@@ -69,7 +69,7 @@ struct Tiling {
   double rows, cols, step_us, full_step_us, round_us, once_us, weights;   // (the weights' bytes per us)
 };
 constexpr Tiling kTilings[] = {{kOn64, MI355_GEMM_TILING_64, 64, 64, 0.20, 0.32, 4.0, 1.0, 5.5e6},
-                               {kOn128, MI355_GEMM_TILING_128, 128, 128, 0.30, 0.47, 5.0, 0.0, 4.5e6},
+                               {kOn128, MI355_GEMM_TILING_128, 128, 128, 0.30, 0.47, 5.0, 0.0, 5.5e6},
                                {kOn256x128, MI355_GEMM_TILING_256X128, 256, 128, 0.55, 0.85, 7.0, 0.0, 4.5e6},
                                {kOn256, MI355_GEMM_TILING_256, 256, 256, 0.85, 1.30, 4.0, 10.0, 4.5e6}};
 constexpr const Tiling &tiling_of(Kernel k) { return kTilings[k - kOn64]; }
@@ -105,7 +105,7 @@ Choice choose(const mi355_dev *dev, int epi, uint32_t m, uint32_t n, uint32_t k_
   return best;
 }
 
-// A product as one launch, or (main_rows > 0) as two by rows.
+// A product as one launch, or (main_rows > 0) as two by rows, the first on 256x256 tiles.
 struct Division {
   Choice whole, rest;
   uint32_t main_rows = 0;
@@ -115,7 +115,7 @@ Division divide(const mi355_dev *dev, int epi, uint32_t m, uint32_t n, uint32_t 
   Division d;
   d.whole = choose(dev, epi, m, n, k_bytes, can_slice);
   d.us = d.whole.us;
-  if (d.whole.kernel != kOn256 || dev->gemm_tiling != MI355_GEMM_TILING_AUTO) return d;
+  if (dev->gemm_tiling != MI355_GEMM_TILING_AUTO) return d;
   const double cus = count_of_cus(dev), sums_n = columns_of_sums(epi, n), tiles_n = std::ceil(sums_n / 256.0);
   const double rounds = std::ceil(std::ceil(m / 256.0) * tiles_n / cus);
   const double rows = std::floor((rounds - 1.0) * cus / tiles_n) * 256.0;   // in one round less
@@ -146,8 +146,8 @@ int launch(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &
 double mi355_ffn_rows_us(const mi355_dev *dev, int epi, uint32_t m, uint32_t n, uint32_t k_bytes) {
   if (m > 64u) return 1e30;
   const double a_rows = m <= 16u ? m : (m + 15u) / 16u * 16u, sums_n = columns_of_sums(epi, n);
-  const double groups = (n + 15u) / 16u, all_read = (sums_n + groups * a_rows) * k_bytes;
-  return 2.5 + std::max(sums_n * k_bytes / 5.5e6, all_read / (8.4e6 * std::min(1.0, groups / count_of_cus(dev))));
+  const double on_one_cu = std::ceil(std::ceil(n / 16.0) / count_of_cus(dev)), read = (16.0 * sums_n / n + a_rows) * k_bytes;
+  return 2.5 + std::max(sums_n * k_bytes / 5.5e6, on_one_cu * (read / 3.3e4 + (m <= 16u ? 0.4 : 0.9)));
 }
 
 namespace {
@@ -316,7 +316,7 @@ int mi355_ffn_product(mi355_dev *dev, int op, int epi, const char *what, const F
     rest.out.g = static_cast<uint8_t *>(p.out.g) + d.main_rows * p.out.ldg * elem;
     rest.out.u = static_cast<uint8_t *>(p.out.u) + d.main_rows * p.out.ldg * elem;
   }
-  if (int rc = launch(dev, op, epi, what, first, d.whole, nullptr)) return rc;
+  if (int rc = launch(dev, op, epi, what, first, Choice{}, nullptr)) return rc;
   return launch(dev, op, epi, what, rest, d.rest, workspace);
 }
 
