@@ -80,9 +80,11 @@ __global__ void __launch_bounds__(kSmallThreads) ffn_small_kernel(FfnLaunch<EPI>
     w.voff[q] = min(lane / 8u + 8u * q, p.m - 1u - a_row) * lda + chunk;
     if (q < 4u) w.voff_b[q] = min(lane / 8u + 8u * q, p.n - 1u - b_row) * ldb + chunk;
   }
-  w.ga = (uint64_t)(uintptr_t)(p.a + (uint64_t)a_row * lda + (uint64_t)k0 * kRowBytes);
-  w.gb = (uint64_t)(uintptr_t)(b + (uint64_t)b_row * ldb + (uint64_t)k0 * kRowBytes);
-  uint32_t fetch_left = steps, fill = 0, look = 0;   // slot offsets: the one to fill, the one to read
+  // the walk over K starts at a place of the XCD's own (ffn_rows.hip says why) and wraps around
+  const uint32_t k_rot = work.tile % 8u * (steps / 8u);
+  w.ga = (uint64_t)(uintptr_t)(p.a + (uint64_t)a_row * lda + (uint64_t)(k0 + k_rot) * kRowBytes);
+  w.gb = (uint64_t)(uintptr_t)(b + (uint64_t)b_row * ldb + (uint64_t)(k0 + k_rot) * kRowBytes);
+  uint32_t fetch_left = steps - k_rot, fill = 0, look = 0;   // slot offsets: the one to fill, the one to read
   auto fetched = [&]() {                             // on to the next slab; past the last one: the first again
     w.ga += kRowBytes;
     w.gb += kRowBytes;
