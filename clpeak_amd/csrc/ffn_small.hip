@@ -8,9 +8,9 @@
 // slice go to the workspace as they are and a second launch (ffn_join.hip) adds the slices and finishes.  The plain
 // products of 16-bit operands come in groups of up to three, whose workgroups are one launch.
 //
-// Measured: 512x8192x4096 int8 22.2 us (on 64x64 tiles 41.1, on 256x256 41.4); the gated projection 333x2731x1024 fp16 11.0 us
-// (20.0, 26.2), 512x8192x4096 bf16 on tall tiles 62.7 us (on 128x128 80.1, on 256x256 81.1), 1000x8192x8192 int8 59.4 us (68.0,
-// 73.1).  Few tiles: bound by the walk along K, 0.3 us a step (tall 0.55 to 0.85), and 5 us for its start and the sums'
+// Measured: 512x8192x4096 int8 22.1 us (on 64x64 tiles 42.6, on 256x256 40.8); the gated projection 333x2731x1024 bf16 10.4 us
+// (20.2, 25.8), 512x8192x4096 bf16 on tall tiles 56.3 us (on 128x128 75.5, on 256x256 81.4), 1000x8192x8192 int8 60.4 us (66.0,
+// 73.3).  Few tiles: bound by the walk along K, 0.3 us a step (tall 0.55 to 0.85), and 5 us for its start and the sums'
 // way out.
 #include "ffn.h"
 #include "gemm_small_step.h"
