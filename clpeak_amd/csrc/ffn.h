@@ -22,7 +22,7 @@ struct FfnOut {
   uint64_t ldc;
   void *g, *u;           // kEpiGated: where the two sums are kept (both or neither)
   uint64_t ldg;
-  const float *sa, *sb, *sb2, *bias;
+  const float *sa, *sb, *sb2, *bias;   // (kEpiPlain of fp16: one value at sa, which C's sums are multiplied by)
   int type;              // of C / H: MI355_TYPE_*
   int act;               // MI355_GLU_*
 };
@@ -58,6 +58,7 @@ struct FfnGroup {
   } of[3];
   uint32_t count;
   int type;
+  const float *sa;                      // (FfnOut's)
 };
 struct FfnGroupChoice {
   int kernel;             // (ffn.hip's number of it)
@@ -127,6 +128,7 @@ struct FfnLaunch<kEpiPlain> {
     w.tiles_m = o.tiles_m; w.tiles_n = o.tiles_n;
     w.slice = at / tiles; w.tile = at - w.slice * tiles; w.slices = o.slices;
     w.p.out.ldc = o.ldc;
+    w.p.out.sa = g.sa;
     w.p.out.type = o.slices > 1u || o.pairs ? MI355_TYPE_F32 : g.type;
     w.p.out.c = static_cast<uint8_t *>(o.c) + (o.slices > 1u ? (uint64_t)w.slice * o.m * o.ldc * 4u : 0u);
     return w;
@@ -339,10 +341,14 @@ __device__ __forceinline__ int ffn_type_out(const FfnOut &o) {
   return OP == kQuadBf16 ? MI355_TYPE_BF16 : OP == kQuadF16 ? MI355_TYPE_F16 : o.type;
 }
 
+// kEpiPlain: 32-bit sums (a slice's, and rows that are added later) are kept as they are.
+__device__ __forceinline__ float ffn_plain_factor(const FfnOut &o) { return o.sa && o.type != MI355_TYPE_F32 ? *o.sa : 1.0f; }
+
 // What a lane needs for its columns of a pair of tiles, and for a row.
 template <int EPI>
 struct FfnColumns {
   float sb[2][4], sb2[2][4], bias[2][4];
+  float plain;   // (kEpiPlain of fp16)
   __device__ __forceinline__ void load(const FfnOut &o, uint32_t col0, uint32_t lane, uint32_t n) {
     if constexpr (EPI == kEpiScaled || EPI == kEpiGatedScaled) {
 #pragma unroll
@@ -355,6 +361,7 @@ struct FfnColumns {
           else bias[t][e] = o.bias ? o.bias[col] : 0.0f;
         }
     }
+    if constexpr (EPI == kEpiPlain) plain = ffn_plain_factor(o);
   }
 };
 
@@ -376,6 +383,7 @@ __device__ __forceinline__ void ffn_finish_pair(const FfnOut &o, uint32_t row, u
         if constexpr (EPI == kEpiGatedScaled) b.x[t][e] = ffn_scaled(v2, sa, c.sb2[t][e]);
       } else {
         a.x[t][e] = __builtin_bit_cast(float, v);
+        if constexpr (OP == kQuadF16 && EPI == kEpiPlain) a.x[t][e] *= c.plain;
         if constexpr (EPI == kEpiGated) b.x[t][e] = __builtin_bit_cast(float, v2);
       }
     }
@@ -409,7 +417,8 @@ __device__ __forceinline__ void ffn_finish4(const FfnOut &o, uint32_t row, uint3
   if (col >= n) return;
   const int type = ffn_type_out<OP, EPI>(o);
   float x[4], y[4];
-  const float sa = EPI == kEpiScaled || EPI == kEpiGatedScaled ? o.sa[row] : 0.0f;
+  float sa = EPI == kEpiScaled || EPI == kEpiGatedScaled ? o.sa[row] : 0.0f;
+  if constexpr (OP == kQuadF16 && EPI == kEpiPlain) sa = ffn_plain_factor(o);
 #pragma unroll
   for (int e = 0; e < 4; e++) {
     const int32_t v = s[e], v2 = s2[e];   // (through a scalar: __builtin_bit_cast of a vector's element reads element 0)
@@ -422,6 +431,7 @@ __device__ __forceinline__ void ffn_finish4(const FfnOut &o, uint32_t row, uint3
     } else {
       x[e] = __builtin_bit_cast(float, v);
       y[e] = __builtin_bit_cast(float, v2);
+      if constexpr (OP == kQuadF16 && EPI == kEpiPlain) x[e] *= sa;
     }
   }
   if constexpr (EPI == kEpiGated)
@@ -441,7 +451,7 @@ template <int EPI>
 __device__ __forceinline__ void ffn_finish1(const FfnOut &o, uint32_t row, uint32_t col, int32_t s0, int32_t s1) {
   const uint64_t at = (uint64_t)row * o.ldc + col;
   if constexpr (EPI == kEpiPlain) {
-    ffn_store1(o.c, at, o.type, __builtin_bit_cast(float, s0));
+    ffn_store1(o.c, at, o.type, __builtin_bit_cast(float, s0) * ffn_plain_factor(o));
   } else if constexpr (EPI == kEpiScaled) {
     const float sa = o.sa[row], sb = o.sb[col];
     ffn_store1(o.c, at, o.type, o.bias ? ffn_scaled_plus(s0, sa, sb, o.bias[col]) : ffn_scaled(s0, sa, sb));

@@ -260,7 +260,7 @@ int mi355_ffn_group(mi355_dev *dev, int op, const char *what, const FfnGroup &gr
     if (o.slices <= 1u && !o.pairs) continue;
     FfnProduct p{};
     p.m = o.m; p.n = o.n;
-    p.out.c = o.c; p.out.ldc = o.ldc; p.out.type = g.type;
+    p.out.c = o.c; p.out.ldc = o.ldc; p.out.type = g.type; p.out.sa = g.sa;
     join[joins++] = mi355_ffn_join_of(p, o.slices, o.pairs, workspace);
     o.c = workspace;
     o.ldc = mi355_ffn_slice_row(o.n);

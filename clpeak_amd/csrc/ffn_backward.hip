@@ -17,21 +17,30 @@
 // products of three normal values as many as some hundred alike), where it is the launch that adds the rows that takes
 // time: 1x100x512 bf16 8.3 -> 10.2 us, 300x100x512 10.9 -> 14.5, 1x8192x4096 77.8 -> 79.5.
 // The pass is bound by memory, 3 T F values read and 2 T F written (131 us at 8192x8192).
+//
+// fp16 has five bits of exponent: dG and dU of a loss that is a mean over many tokens lie below its normal values, those of
+// one that is scaled up may lie above its largest, where the results, sums with other factors, are in range.  They are
+// therefore rounded after a power of two that brings the largest of them, finite ones, to 2^14 .. 2^15, and the products' sums
+// are multiplied by its inverse: values down to 2^-28 of the largest keep all their bits, smaller ones are off by at
+// most 2^-39 of it.  (One factor for both: dX sums over F and dW over T, so none for each row or column would do.)  Finding
+// the largest is a pass of its own in front, 3 T F values read (90 us at 8192x8192, 4.5 TB/s and nearly as much arithmetic; 8
+// at 1009x2752).  bf16 has the range of fp32 and needs none of this.
 #include "ffn.h"
 #include "ffn_across.h"
 #include <algorithm>
 
 namespace {
 
-constexpr int kTileEdge = 64, kThreads = 256, kVec = 8;
+constexpr int kTileEdge = 64, kThreads = 256, kVec = 8, kLargestThreads = 512;   // (the latter: a row of a tile for every 8)
 
 __host__ __device__ constexpr uint64_t round_up(uint64_t x, uint64_t to) { return (x + to - 1) / to * to; }
 
 constexpr uint64_t kFewValues = 1u << 15;
+constexpr uint32_t kLargest = 1024;   // workgroups that look for the largest value, at most
 
 // The workspace: dG | dU by rows [Tp][2 Fk]; by columns 2 x [Fp][Tp] where dW wants that; the weights turned [D][2 Fk], or
 // their last rows 2 x [64][D]; X turned [D][Tp], or its last rows [64][D] (where it stands twice, all of it [Tp][D]); and
-// what the products use of it where they are cut along their sums.
+// what the products use of it where they are cut along their sums; of fp16 the workgroups' largest values and the factor that undoes the scaling.
 struct Plan {
   bool twice;                                  // a value is two rows
   uint32_t rows_of;                            // T or 2 T
@@ -41,7 +50,7 @@ struct Plan {
   AcrossChoice dx, dw;
   FfnGroup group;                              // what goes together (dX first): sizes
   FfnGroupChoice grouped;
-  uint64_t rows, cols, w, x, sums, bytes;      // offsets
+  uint64_t rows, cols, w, x, sums, largest, bytes;   // offsets
 };
 Plan plan_of(const mi355_dev *dev, uint32_t T, uint32_t F, uint32_t D) {
   Plan p;
@@ -95,7 +104,8 @@ Plan plan_of(const mi355_dev *dev, uint32_t T, uint32_t F, uint32_t D) {
   else if (p.dx_on == Plan::kOnRows) dx = sums(1, R, p.twice);
   if (p.dw_across) dw = sums(p.dw.slices, 2 * (uint64_t)F, false);
   const uint64_t group = p.group.count ? mi355_ffn_group_workspace(p.group, p.grouped) : 0;
-  p.bytes = round_up(p.sums + std::max(std::max(dx, dw), group), 256);
+  p.largest = round_up(p.sums + std::max(std::max(dx, dw), group), 256);
+  p.bytes = p.largest + round_up((kLargest + 1) * 4, 256);
   return p;
 }
 
@@ -161,12 +171,90 @@ struct Gate {
   int act;
   uint32_t tiles_f, tiles;
   bool by_rows, by_columns;
+  uint32_t *largest;          // fp16: the bits of the largest finite values that workgroups have found, `found` of them,
+  uint32_t found;             // and behind kLargest the factor that undoes the scaling
 };
+
+// 8 neighbours of a row, and dG and dU of them (past F: 0).
+template <int TYPE>
+struct GateIn {
+  Vec8 h, g, u;
+  __device__ __forceinline__ void load(const Gate &p, uint32_t t, uint32_t f) {
+    h = load8(p.dH + (uint64_t)t * p.lddh, f, p.F);
+    g = load8(p.G + (uint64_t)t * p.ldg, f, p.F);
+    u = load8(p.U + (uint64_t)t * p.ldg, f, p.F);
+  }
+  __device__ __forceinline__ void values(int act, float (&x)[kVec], float (&y)[kVec]) const {
+    // one branch on the activation for the 8 values
+    auto with = [&](int act) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < kVec; e++) {
+        float a, da;
+        ffn_act_grad(act, widen<TYPE>(g.v[e]), a, da);
+        const float d = widen<TYPE>(h.v[e]);
+        x[e] = d * da * widen<TYPE>(u.v[e]);
+        y[e] = d * a;
+      }
+    };
+    if (act == MI355_GLU_SILU) with(MI355_GLU_SILU);
+    else if (act == MI355_GLU_GELU_TANH) with(MI355_GLU_GELU_TANH);
+    else if (act == MI355_GLU_GELU) with(MI355_GLU_GELU);
+    else with(MI355_GLU_RELU);
+  }
+};
+
+// The largest of a workgroup's values; every thread's once all have arrived.
+template <int WAVES>
+__device__ __forceinline__ uint32_t workgroup_max(uint32_t v, uint32_t (&of_wave)[WAVES]) {
+#pragma unroll
+  for (int d = 32; d > 0; d /= 2) v = max(v, (uint32_t)__shfl_xor((int)v, d));
+  if (threadIdx.x % 64u == 0u) of_wave[threadIdx.x / 64u] = v;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < WAVES; i++) v = max(v, of_wave[i]);
+  return v;
+}
+
+// The largest finite magnitude of dG and dU, as bits (whole numbers order them), one for each workgroup.
+__global__ void __launch_bounds__(kLargestThreads) glu_backward_largest_kernel(Gate p, uint32_t tiles) {
+  __shared__ uint32_t of_wave[kLargestThreads / 64];
+  float top = 0.0f;
+  for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const uint32_t f = tile % p.tiles_f * kTileEdge + threadIdx.x % 8u * kVec, t0 = tile / p.tiles_f * kTileEdge + threadIdx.x / 8u;
+    GateIn<MI355_TYPE_F16> in;
+    in.load(p, min(t0, p.T - 1u), f);   // (the last row again changes nothing)
+    float x[kVec], y[kVec];
+    in.values(p.act, x, y);
+    float here = 0.0f;   // (the larger of a number and a NaN is the number)
+#pragma unroll
+    for (int e = 0; e < kVec; e++) here = fmaxf(here, fmaxf(fabsf(x[e]), fabsf(y[e])));
+    if (__builtin_expect(__builtin_isinf(here), 0)) {
+      here = 0.0f;
+#pragma unroll
+      for (int e = 0; e < kVec; e++) {
+        here = fmaxf(here, __builtin_isinf(x[e]) ? 0.0f : fabsf(x[e]));
+        here = fmaxf(here, __builtin_isinf(y[e]) ? 0.0f : fabsf(y[e]));
+      }
+    }
+    top = fmaxf(top, here);
+  }
+  const uint32_t all = workgroup_max(__builtin_bit_cast(uint32_t, top), of_wave);
+  if (threadIdx.x == 0) p.largest[blockIdx.x] = all;
+}
+// The power of two that brings that value to 2^14 .. 2^15 (one below 2^-112: times 2^126), from its exponent; the inverse goes
+// to memory for the launches that follow.
+__device__ __forceinline__ float scale_for_f16(const Gate &p, uint32_t (&of_wave)[kThreads / 64]) {
+  uint32_t top = 0;
+  for (uint32_t i = threadIdx.x; i < p.found; i += kThreads) top = max(top, p.largest[i]);
+  const uint32_t exponent = max(workgroup_max(top, of_wave) >> 23, 15u);
+  if (blockIdx.x == 0 && threadIdx.x == 0) p.largest[kLargest] = (exponent - 14u) << 23;
+  return __builtin_bit_cast(float, (268u - exponent) << 23);
+}
 
 // dG and dU of a tile: by rows (dG at column f, dU at column fk + f of a row of 2 fk; zeros from F to fk and in the rows
 // from R to tp) and by columns (row f of [fp][tp], dU fp rows on; zeros from R to tp).
 template <int TYPE>
-__device__ __forceinline__ void gate_tile(const Gate &p, uint32_t tile, Tile &tg, Tile &tu) {
+__device__ __forceinline__ void gate_tile(const Gate &p, uint32_t tile, float scale, Tile &tg, Tile &tu) {
   const uint32_t f0 = tile % p.tiles_f * kTileEdge, t0 = tile / p.tiles_f * kTileEdge;
   const uint32_t c = threadIdx.x % 8u * kVec, r0 = threadIdx.x / 8u;
 #pragma unroll
@@ -176,15 +264,15 @@ __device__ __forceinline__ void gate_tile(const Gate &p, uint32_t tile, Tile &tg
     if (row < p.R) {
       const bool left = row >= p.T;
       const uint32_t t = left ? row - p.T : row;
-      const Vec8 h = load8(p.dH + (uint64_t)t * p.lddh, f, p.F), g = load8(p.G + (uint64_t)t * p.ldg, f, p.F), u = load8(p.U + (uint64_t)t * p.ldg, f, p.F);
+      float x[kVec], y[kVec];
+      GateIn<TYPE> in;
+      in.load(p, t, f);
+      in.values(p.act, x, y);
 #pragma unroll
       for (int e = 0; e < kVec; e++) {
-        float a, da;
-        ffn_act_grad(p.act, widen<TYPE>(g.v[e]), a, da);
-        const float d = widen<TYPE>(h.v[e]);
-        const float x = d * da * widen<TYPE>(u.v[e]), y = d * a;   // (past F: 0; da is at most 1.13: nothing overflows before the result does)
-        dg.v[e] = narrow<TYPE>(left ? left_of<TYPE>(x) : x);
-        du.v[e] = narrow<TYPE>(left ? left_of<TYPE>(y) : y);
+        if constexpr (TYPE == MI355_TYPE_F16) { x[e] *= scale; y[e] *= scale; }
+        dg.v[e] = narrow<TYPE>(left ? left_of<TYPE>(x[e]) : x[e]);
+        du.v[e] = narrow<TYPE>(left ? left_of<TYPE>(y[e]) : y[e]);
       }
     }
     if (p.by_rows) {
@@ -236,7 +324,14 @@ template <int TYPE>
 __global__ void __launch_bounds__(kThreads) glu_backward_prepare_kernel(Gate gate, Layout l0, Layout l1, Layout l2) {
   __shared__ Tile a, b;
   uint32_t i = blockIdx.x;
-  if (i < gate.tiles) return gate_tile<TYPE>(gate, i, a, b);
+  if (i < gate.tiles) {
+    float scale = 1.0f;
+    if constexpr (TYPE == MI355_TYPE_F16) {
+      __shared__ uint32_t of_wave[kThreads / 64];
+      scale = scale_for_f16(gate, of_wave);
+    }
+    return gate_tile<TYPE>(gate, i, scale, a, b);
+  }
   i -= gate.tiles;
   if (i < l0.tiles) return layout_tile(l0, i, a);
   i -= l0.tiles;
@@ -309,6 +404,14 @@ int mi355_launch_glu_backward(mi355_dev *dev, int type, int act, const void *dH,
   }
   if (dWg && p.dw_across) x = p.twice && T ? all_twice(X, ldx, ws + p.x, T, p.tp, D) : last_rows(X, ldx, ws + p.x, T, D);
   else if (dWg) x = turned(X, ldx, ws + p.x, p.tp, p.rows_of, T, p.tp, D);
+  gate.largest = (uint32_t *)(ws + p.largest); gate.found = 0;
+  const float *const undo = type == MI355_TYPE_F16 ? (const float *)gate.largest + kLargest : nullptr;
+  if (type == MI355_TYPE_F16 && T) {
+    const uint32_t tiles_t = (T + 63u) / 64u, all = gate.tiles_f * tiles_t;
+    gate.found = std::min(all, kLargest);
+    glu_backward_largest_kernel<<<gate.found, kLargestThreads, 0, dev->stream>>>(gate, all);
+    MI355_LAUNCH_CHECK(dev, "glu_backward (largest)");
+  }
   const uint32_t grid = gate.tiles + wg.tiles + wu.tiles + x.tiles;
   if (type == MI355_TYPE_BF16) glu_backward_prepare_kernel<MI355_TYPE_BF16><<<grid, kThreads, 0, dev->stream>>>(gate, wg, wu, x);
   else glu_backward_prepare_kernel<MI355_TYPE_F16><<<grid, kThreads, 0, dev->stream>>>(gate, wg, wu, x);
@@ -316,10 +419,10 @@ int mi355_launch_glu_backward(mi355_dev *dev, int type, int act, const void *dH,
   FfnAcross c{};
   c.a = ws + p.rows; c.lda = 4 * p.fk;
   c.n = D;
-  c.out.type = type;
+  c.out.type = type; c.out.sa = undo;
   FfnGroup g{};           // the members of the planned group that are wanted
   FfnGroupChoice choice = p.grouped;
-  g.type = type;
+  g.type = type; g.sa = undo;
   uint32_t planned = 0;
   auto add = [&](bool wanted, const uint8_t *a, uint64_t lda, const uint8_t *b, uint64_t ldb, void *out, uint64_t ldc) {
     const FfnGroup::One &size = p.group.of[planned];
@@ -353,7 +456,7 @@ int mi355_launch_glu_backward(mi355_dev *dev, int type, int act, const void *dH,
     q.a = ws + p.rows; q.lda = 4 * p.fk;
     q.b = ws + p.w; q.ldb = 4 * p.fk;
     q.m = p.rows_of; q.n = D; q.k_bytes = (uint32_t)(4 * p.fk);
-    q.out.c = dX; q.out.ldc = lddx; q.out.type = type;
+    q.out.c = dX; q.out.ldc = lddx; q.out.type = type; q.out.sa = undo;
     if (int rc = mi355_launch_ffn_rows(dev, op, kEpiPlain, "glu_backward (dX)", p.twice ? mi355_ffn_slices_of(q, ws + p.sums) : q)) return rc;
     FfnJoin join = mi355_ffn_join_of(q, 1, true, ws + p.sums);
     if (p.twice)

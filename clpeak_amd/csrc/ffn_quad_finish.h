@@ -113,7 +113,7 @@ struct Finish {
   // 177 -> 186 us, the last round's stores being all that is left to wait for; int8, whose operands are half as large:
   // 2 % slower)
   bool many_rounds;
-  float sa[8];
+  float sa[8], plain;
   PairOut<TYPE> c, g, u;
 
   template <int I, int JP>
@@ -128,6 +128,7 @@ struct Finish {
         if constexpr (EPI == kEpiScaled) x[t][e] = p.out.bias ? ffn_scaled_plus(v, sa[I], k.sb[t][e], k.more[t][e]) : ffn_scaled(v, sa[I], k.sb[t][e]);
         else if constexpr (EPI == kEpiGatedScaled) x[t][e] = ffn_scaled(v, sa[I], k.sb[t][e]);
         else x[t][e] = __builtin_bit_cast(float, v);
+        if constexpr (OP == kQuadF16 && EPI == kEpiPlain) x[t][e] *= plain;
       }
     const bool row = 16u * I < p.m - row0 && row0 < p.m;
     const bool whole = row && rem >= (TYPE == MI355_TYPE_F32 ? 20 : 8);
@@ -181,6 +182,7 @@ struct Finish {
 #pragma unroll
       for (uint32_t i = 0; i < 8; i++) sa[i] = p.out.sa[min(row0 + 16u * i, p.m - 1u)];
     }
+    if constexpr (OP == kQuadF16 && EPI == kEpiPlain) plain = ffn_plain_factor(p.out);
     // the wait states the compiler cannot know about, then every load of this wave (the next barrier X then needs no
     // wait of its own, and the stores issued here do not enter its count)
     asm volatile("s_nop 15\n s_nop 15\n s_waitcnt vmcnt(0)" ::: "memory");

@@ -380,7 +380,8 @@ int mi355_glu_forward(mi355_dev *dev, int type, int act, const void *X, uint64_t
                       void *H, uint64_t ldh, void *G, void *U, uint64_t ldg, uint32_t T, uint32_t F, uint32_t D);
 /* Its gradients, from dH[T][F] and the kept G and U:
  *     dG = dH * U * act'(G),  dU = dH * act(G)      (fp32, rounded to `type` for the products that follow;
- *         of up to 2^15 values (T F) each as two of `type`, its rounding and the rounding of what that leaves)
+ *         of up to 2^15 values (T F) each as two of `type`, its rounding and the rounding of what that leaves;
+ *         fp16: after a power of two that brings the largest finite one of both to 2^14 .. 2^15 and that the sums lose again)
  *     dX[T][D] = dG Wg + dU Wu,   dWg[F][D] = dG^T X,   dWu[F][D] = dU^T X      (fp32 sums, rounded once to `type`)
  * dX NULL, or dWg and dWu NULL: that part is left out (a frozen weight, a first layer); its operand (Wg and Wu, or X)
  * may then be NULL too.  `workspace` holds what mi355_glu_backward_workspace says (for this handle, as its

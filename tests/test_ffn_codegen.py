@@ -130,3 +130,11 @@ def test_across_reads_lds_the_other_way_round(asm):
         assert body.count("ds_read_b64_tr_b16") == (2 * 64 + 32 + 8 if across_a else 2 * 32 + 32), (k, body.count("ds_read_b64_tr_b16"))
         assert body.count("ds_read_b128") == (0 if across_a else 2 * 16 + 4), (k, body.count("ds_read_b128"))
         assert len(re.findall(r"^\s*s_barrier", body, re.M)) == 2 + 2 * 2, k
+
+
+def test_the_pass_that_looks_for_the_largest_value_uses_no_memory_for_registers(asm):
+    text = asm("ffn_backward.hip")
+    meta = gen.kernel_metadata(text)
+    (k,) = [k for k in meta if "glu_backward_largest_kernel" in k]
+    assert meta[k]["vgpr_spill_count"] == 0 and meta[k]["private_segment_fixed_size"] == 0, meta[k]
+    assert "scratch_" not in gen.kernel_body(text, k) and not re.search(r"v_pk_(add|mul|fma)_f32", gen.kernel_body(text, k))

@@ -1,0 +1,100 @@
+"""fp16 gradients of the gated projection on the GPU from dH far from 1, against 64 bits; bounds fixed from the arithmetic
+before the first run."""
+import math
+
+import pytest
+import torch
+
+from clpeak_amd import capi
+from test_gpu_ffn import ACTS, E, UNIT, act64, act_off, dv, gen, grad64, grad_off, tiled, within  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def gradients_f16(dv, act, dh, x, wg, wu, G, U):
+    """The call on contiguous operands, and the definition with how far dG and dU may be off: their rounding to fp16 (few
+    values: twice) after a power of two that brings the largest of them, `top`, to 2^14 at least: below 2^-14 / 2^14 top the
+    step is 2^-24 / 2^14 top, half of it 2^-39 top."""
+    T, D = x.shape
+    F = wg.shape[0]
+    n = dv.glu_backward_workspace(T, F, D)
+    ws = torch.full((n,), 0xFF, dtype=torch.uint8, device="cuda")
+    dx, dwg, dwu = (torch.empty(r, D, dtype=torch.float16, device="cuda") for r in (T, F, F))
+    dv.glu_backward(capi.TYPE_F16, act, dh, F, x, D, wg, wu, D, G, U, F, dx, D, dwg, dwu, D, T, F, D, ws, n)
+    G64, U64, d64 = G.double(), U.double(), dh.double()
+    dG, dU = d64 * U64 * grad64(act, G64), d64 * act64(act, G64)
+    top = max(float(v[torch.isfinite(v)].abs().max()) for v in (dG, dU))
+    unit = UNIT[torch.float16] ** 2 if T * F <= 32768 else UNIT[torch.float16]
+    oG = unit * dG.abs() + top * 2.0 ** -39 + (d64 * U64).abs() * (grad_off(act, G64) + 4 * E)
+    oU = unit * dU.abs() + top * 2.0 ** -39 + d64.abs() * (act_off(act, G64) + 4 * E)
+    w64g, w64u, x64 = wg.double(), wu.double(), x.double()
+    got = (dx, dwg, dwu)
+    ref = (dG @ w64g + dU @ w64u, dG.T @ x64, dU.T @ x64)
+    off = ((oG + 4 * F * E * dG.abs()) @ w64g.abs() + (oU + 4 * F * E * dU.abs()) @ w64u.abs(),
+           (oG + 2 * T * E * dG.abs()).T @ x64.abs(), (oU + 2 * T * E * dU.abs()).T @ x64.abs())
+    return got, ref, off
+
+
+F16_SIZES = [(1, 300, 128), (48, 992, 64), (300, 1000, 256), (2048, 200, 128), (4200, 300, 128), (513, 2100, 64)]
+
+
+@pytest.mark.parametrize("size", [1e-7, 1e-6, 1e-5, 1e-3])
+@pytest.mark.parametrize("T, F, D", F16_SIZES)
+def test_fp16_gradients_of_a_small_loss(tiled, size, T, F, D):
+    """dH as an unscaled mean over many tokens gives it.  X and the weights are large enough that the results are not lost
+    in fp16 as well."""
+    act = ACTS[(T + F) % 4]
+    g = gen(T + F)
+    h = lambda r, c, s: (torch.randn(r, c, generator=g, device="cuda") * s).half()  # noqa: E731
+    dh, x, wg, wu, G, U = h(T, F, size), h(T, D, 64), h(F, D, 64), h(F, D, 64), h(T, F, 1.5), h(T, F, 1)
+    got, ref, off = gradients_f16(tiled, act, dh, x, wg, wu, G, U)
+    for a, b, o in zip(got, ref, off):
+        within(a, b, o, torch.float16)
+
+
+@pytest.mark.parametrize("T, F, D", F16_SIZES)
+def test_fp16_gradients_of_a_large_loss(tiled, T, F, D):
+    """dG and dU past 65504, results well within: small weights and activations."""
+    act = ACTS[(T + F) % 4]
+    g = gen(T + F + 1)
+    h = lambda r, c, s: (torch.randn(r, c, generator=g, device="cuda") * s).half()  # noqa: E731
+    dh, x, wg, wu, G, U = h(T, F, 8000), h(T, D, 2e-4), h(F, D, 2e-4), h(F, D, 2e-4), h(T, F, 1.5).abs() + 30, h(T, F, 40)
+    got, ref, off = gradients_f16(tiled, act, dh, x, wg, wu, G, U)
+    for a, b, o in zip(got, ref, off):
+        within(a, b, o, torch.float16)
+    assert float((dh.double() * U.double()).abs().max()) > 2 * 65504
+
+
+@pytest.mark.parametrize("T, F, D", F16_SIZES[1:])
+def test_fp16_gradients_of_rows_of_very_different_sizes(tiled, T, F, D):
+    """Rows of dH from 1e-7 to 1e3 in one call: every value as near as the largest one allows."""
+    act = ACTS[(T + F) % 4]
+    g = gen(T + F + 2)
+    h = lambda r, c, s: (torch.randn(r, c, generator=g, device="cuda") * s).half()  # noqa: E731
+    rows = 10 ** (10 * torch.rand(T, 1, generator=g, device="cuda") - 7)
+    dh, x, wg, wu, G, U = h(T, F, rows), h(T, D, 1 / 16), h(F, D, 1 / 16), h(F, D, 1 / 16), h(T, F, 1.5), h(T, F, 1)
+    got, ref, off = gradients_f16(tiled, act, dh, x, wg, wu, G, U)
+    for a, b, o in zip(got, ref, off):
+        within(a, b, o, torch.float16)
+
+
+@pytest.mark.parametrize("T, F, D", [(40, 70, 64), (300, 1000, 128)])
+def test_fp16_gradients_where_dh_is_not_finite(tiled, T, F, D):
+    """An infinity and a NaN in dH stay in their rows of dX and of the weights' gradients, and say nothing about the size of
+    the others."""
+    g = gen(T)
+    h = lambda r, c, s: (torch.randn(r, c, generator=g, device="cuda") * s).half()  # noqa: E731
+    dh, x, wg, wu, G, U = h(T, F, 1e-6), h(T, D, 64), h(F, D, 64), h(F, D, 64), h(T, F, 1.5), h(T, F, 1)
+    dh[5, 3], dh[20, 60] = math.inf, math.nan
+    got, ref, off = gradients_f16(tiled, capi.GLU_SILU, dh, x, wg, wu, G, U)
+    for a, b, o, rows in zip(got, ref, off, ((5, 20), (3, 60), (3, 60))):
+        rest = [r for r in range(a.shape[0]) if r not in rows]
+        assert not bool(torch.isfinite(a[list(rows)]).any())
+        within(a[rest], b[rest], o[rest], torch.float16)
+
+
+def test_fp16_gradients_that_are_all_zero(tiled):
+    T, F, D = 130, 300, 128
+    z = lambda r, c, v: torch.full((r, c), v, dtype=torch.float16, device="cuda")  # noqa: E731
+    got, _, _ = gradients_f16(tiled, capi.GLU_SILU, z(T, F, 0.0), z(T, D, 1.0), z(F, D, 1.0), z(F, D, 1.0), z(T, F, 1.0), z(T, F, 1.0))
+    assert all(bool((a == 0).all()) for a in got)
