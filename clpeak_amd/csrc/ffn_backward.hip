@@ -191,8 +191,11 @@ struct GateIn {
       for (int e = 0; e < kVec; e++) {
         float a, da;
         ffn_act_grad(act, widen<TYPE>(g.v[e]), a, da);
-        const float d = widen<TYPE>(h.v[e]);
-        x[e] = d * da * widen<TYPE>(u.v[e]);
+        const float d = widen<TYPE>(h.v[e]), v = widen<TYPE>(u.v[e]);
+        // half of act' (which is at most 1.13) first times the larger of the other two, then the smaller: neither product
+        // overflows, or falls below the normal values, unless the result does
+        const bool d_first = fabsf(d) > fabsf(v);
+        x[e] = 2.0f * (0.5f * da * (d_first ? d : v) * (d_first ? v : d));
         y[e] = d * a;
       }
     };

@@ -98,3 +98,23 @@ def test_fp16_gradients_that_are_all_zero(tiled):
     z = lambda r, c, v: torch.full((r, c), v, dtype=torch.float16, device="cuda")  # noqa: E731
     got, _, _ = gradients_f16(tiled, capi.GLU_SILU, z(T, F, 0.0), z(T, D, 1.0), z(F, D, 1.0), z(F, D, 1.0), z(T, F, 1.0), z(T, F, 1.0))
     assert all(bool((a == 0).all()) for a in got)
+
+
+@pytest.mark.parametrize("rows", [1, 700])
+def test_bf16_gradients_of_factors_that_are_far_apart(tiled, rows):
+    """dG = dH U act'(G) in range with dH or U at the end of theirs: no product of two of the three leaves it, or loses
+    bits below it, on the way.  X is the identity, so dWg is dG turned (dU = dH act(G) is out of range in some of the rows, which
+    shows in dWu).  silu' at -14 is two terms of 14 : 1 that are each (8 + 2 |x|) u off: 50 u with the products."""
+    T, F, dt = 8 * rows, 64, torch.bfloat16
+    D = -(-T // 64) * 64
+    big, small, u = 1.9921875 * 2.0 ** 127, 1.5 * 2.0 ** -126, 2.0 ** -20
+    case = torch.tensor([(big, 2.4, u), (u, 2.4, big), (-big, 2.4, -u), (small, -14.0, 2.0 ** 100), (2.0 ** 100, -14.0, small), (small, 2.4, 1.0),
+                         (1.0, 2.4, -big / 2), (big, -14.0, 1.0)], dtype=torch.float64).repeat(rows, 1)
+    dh, G, U = (case[:, k, None].expand(T, F).to(dt).contiguous().cuda() for k in range(3))
+    x, dwg, dwu = torch.eye(T, D, dtype=dt, device="cuda"), *(torch.empty(F, D, dtype=dt, device="cuda") for _ in range(2))
+    n = tiled.glu_backward_workspace(T, F, D)
+    tiled.glu_backward(capi.TYPE_BF16, capi.GLU_SILU, dh, F, x, D, None, None, D, G, U, F, None, D, dwg, dwu, D, T, F, D, torch.empty(n, dtype=torch.uint8, device="cuda"), n)
+    ref = dh.double() * U.double() * grad64(capi.GLU_SILU, G.double())
+    assert float(ref.abs().max()) < 3.38e38
+    # (of many values dG is rounded to bf16 first)
+    within(dwg[:, :T].T, ref, (50 * E + (0 if T * F <= 32768 else UNIT[dt])) * ref.abs(), dt)
