@@ -135,11 +135,10 @@ struct FfnLaunch<kEpiPlain> {
   }
 };
 
-// Bits of mi355_dev::full_lds_allowed: 8 kernels on 256x256 tiles, on the others 7 for each shape of tile.
+// The number of a kernel among those on one shape of tile (256x256 ones apart).
 constexpr int ffn_kind(int op, int epi) {
   return op != kQuadI8 ? (op - kQuadBf16) * 2 + epi_is_gated(epi) : 4 + (epi == kEpiPartial ? 2 : epi_is_gated(epi));
 }
-enum { kLdsFfnQuad0 = 24, kLdsFfnSmall0 = 32, kLdsFfnMid0 = 39, kLdsFfnTall0 = 46 };
 
 // ffn.hip: the product on the kernel that suits it, and the workspace that it can use.
 int mi355_ffn_product(mi355_dev *dev, int op, int epi, const char *what, const FfnProduct &p, void *workspace, size_t workspace_bytes);

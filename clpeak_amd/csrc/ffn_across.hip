@@ -281,8 +281,7 @@ __global__ void __launch_bounds__(kQuadThreads) ffn_across_kernel(FfnAcross p, u
 
 template <int OP, bool ACROSS_A, int EPI, int TYPE>
 int launch(mi355_dev *dev, const char *what, const FfnAcross &p, uint32_t slices) {
-  // bits 1 to 8 of mi355_dev::full_lds_allowed
-  if (int rc = allow_full_lds(dev, &ffn_across_kernel<OP, ACROSS_A, EPI, TYPE>, 1 + (OP == kQuadF16) * 4 + ACROSS_A * 2 + (EPI == kEpiPartial))) return rc;
+  if (int rc = allow_full_lds<kLdsFfnAcross, (OP == kQuadF16) * 4 + ACROSS_A * 2 + (EPI == kEpiPartial)>(dev, &ffn_across_kernel<OP, ACROSS_A, EPI, TYPE>)) return rc;
   const uint64_t tiles_m = (uint64_t)p.parts * ((p.m + 255u) / 256u), tiles_n = (p.n + 255u) / 256u;
   MI355_REQUIRE(dev, tiles_m * tiles_n <= 0x3fffffffull, "%s: %u x %u outputs are more than one launch takes", what, p.m, p.n);
   const dim3 grid(slices > 1 ? (uint32_t)(tiles_m * tiles_n) : gemm_workgroups(dev, (uint32_t)(tiles_m * tiles_n)), slices);

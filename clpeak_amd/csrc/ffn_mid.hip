@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(kMidThreads) ffn_mid_kernel(FfnLaunch<EPI> arg
 
 template <int OP, int EPI>
 int launch_tiles(mi355_dev *dev, const char *what, const FfnProduct &p, uint32_t slices) {
-  if (int rc = allow_full_lds(dev, &ffn_mid_kernel<OP, EPI>, kLdsFfnMid0 + ffn_kind(OP, EPI))) return rc;
+  if (int rc = allow_full_lds<kLdsFfnMid, ffn_kind(OP, EPI)>(dev, &ffn_mid_kernel<OP, EPI>)) return rc;
   const uint32_t cols = epi_is_gated(EPI) ? 32 : 64;
   const uint64_t tiles_m = (p.m + 63ull) / 64u, tiles_n = (p.n + cols - 1ull) / cols;
   MI355_REQUIRE(dev, tiles_m * tiles_n <= 0xffffffull, "%s: %u x %u outputs are more than one launch takes", what, p.m, p.n);
@@ -136,7 +136,7 @@ int launch(mi355_dev *dev, const char *what, const FfnProduct &p, uint32_t slice
 }
 template <int OP>
 int launch_group(mi355_dev *dev, const char *what, const FfnGroup &g) {
-  if (int rc = allow_full_lds(dev, &ffn_mid_kernel<OP, kEpiPlain>, kLdsFfnMid0 + ffn_kind(OP, kEpiPlain))) return rc;
+  if (int rc = allow_full_lds<kLdsFfnMid, ffn_kind(OP, kEpiPlain)>(dev, &ffn_mid_kernel<OP, kEpiPlain>)) return rc;
   FfnLaunch<kEpiPlain> args{g};
   uint32_t blocks = 0;
   if (int rc = mi355_ffn_lay_out_group(dev, what, args.g, kMidTile, kMidTile, blocks)) return rc;

@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(kQuadThreads) ffn_quad_kernel(FfnProduct p, ui
 template <int OP, int EPI, int TYPE>
 int launch(mi355_dev *dev, const char *what, const FfnProduct &p) {
   constexpr bool kGated = epi_is_gated(EPI);
-  if (int rc = allow_full_lds(dev, &ffn_quad_kernel<OP, EPI, TYPE>, kLdsFfnQuad0 + (OP != kQuadI8 ? OP - kQuadBf16 : 2 + 3 * kGated + TYPE))) return rc;
+  if (int rc = allow_full_lds<kLdsFfnQuad, (OP != kQuadI8 ? OP - kQuadBf16 : 2 + 3 * kGated + TYPE)>(dev, &ffn_quad_kernel<OP, EPI, TYPE>)) return rc;
   const uint32_t cols = kGated ? 128 : 256;
   const uint64_t tiles_m = (p.m + 255ull) / 256u, tiles_n = (p.n + cols - 1ull) / cols;
   MI355_REQUIRE(dev, tiles_m * tiles_n <= 0x3fffffffull, "%s: %u x %u outputs are more than one launch takes", what, p.m, p.n);

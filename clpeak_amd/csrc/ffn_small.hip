@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kSmallThreads) ffn_small_kernel(FfnLaunch<EPI>
 template <int OP, int EPI, int MI>
 int launch_tiles(mi355_dev *dev, const char *what, const FfnProduct &p, uint32_t slices) {
   using Ring = SmallRing<MI>;
-  if (int rc = allow_full_lds(dev, &ffn_small_kernel<OP, EPI, MI>, (MI == 4 ? kLdsFfnSmall0 : kLdsFfnTall0) + ffn_kind(OP, EPI))) return rc;
+  if (int rc = allow_full_lds<MI == 4 ? kLdsFfnSmall : kLdsFfnTall, ffn_kind(OP, EPI)>(dev, &ffn_small_kernel<OP, EPI, MI>)) return rc;
   const uint32_t cols = epi_is_gated(EPI) ? 64 : 128;
   const uint64_t tiles_m = (p.m + Ring::kRows - 1ull) / Ring::kRows, tiles_n = (p.n + cols - 1ull) / cols;
   MI355_REQUIRE(dev, tiles_m * tiles_n <= 0xffffffull, "%s: %u x %u outputs are more than one launch takes", what, p.m, p.n);
@@ -173,7 +173,7 @@ int launch_kind(mi355_dev *dev, int op, int epi, const char *what, const FfnProd
 template <int OP, int MI>
 int launch_group(mi355_dev *dev, const char *what, const FfnGroup &g) {
   using Ring = SmallRing<MI>;
-  if (int rc = allow_full_lds(dev, &ffn_small_kernel<OP, kEpiPlain, MI>, (MI == 4 ? kLdsFfnSmall0 : kLdsFfnTall0) + ffn_kind(OP, kEpiPlain))) return rc;
+  if (int rc = allow_full_lds<MI == 4 ? kLdsFfnSmall : kLdsFfnTall, ffn_kind(OP, kEpiPlain)>(dev, &ffn_small_kernel<OP, kEpiPlain, MI>)) return rc;
   FfnLaunch<kEpiPlain> args{g};
   uint32_t blocks = 0;
   if (int rc = mi355_ffn_lay_out_group(dev, what, args.g, Ring::kRows, kSmallTile, blocks)) return rc;

@@ -235,7 +235,7 @@ extern "C" int mi355_gemm_f32(mi355_dev *dev, const float *A, const float *B, fl
                               uint32_t K) {
   MI355_ENTER(dev);
   if (int rc = check_shapes(dev, A, B, C, M, N, K, 4)) return rc;
-  if (int rc = allow_full_lds(dev, &gemm_f32_kernel, kLdsF32)) return rc;
+  if (int rc = allow_full_lds<kLdsF32, 0>(dev, &gemm_f32_kernel)) return rc;
   const uint32_t tiles_m = M / kTile, tiles_n = N / kTile;
   gemm_f32_kernel<<<gemm_workgroups(dev, tiles_m * tiles_n), kThreads, kRingBytes, dev->stream>>>(
       (const uint8_t *)A, (const uint8_t *)B, C, N, K * 4, tiles_m, tiles_n);

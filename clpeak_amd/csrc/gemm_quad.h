@@ -3,8 +3,6 @@
 #include "internal.h"
 
 enum { kQuadE4m3 = 0, kQuadE5m2 = 1, kQuadBf16 = 2, kQuadF16 = 3, kQuadI8 = 4, kQuadMx = 5 };
-enum { kLdsQuad0 = 8 };   // first bit of mi355_dev::full_lds_allowed used by the instantiations of gemm_quad_kernel
-enum { kLdsSmall0 = 16 };  // the same for gemm_small_kernel (gemm_small.hip)
 
 // Shapes have been checked by the caller (multiples of 256 x 256, K a multiple of 128 bytes, 16-byte aligned buffers).
 int mi355_launch_gemm_quad(mi355_dev *dev, int op, const char *what, const void *A, const void *B, void *C, uint32_t M, uint32_t N,

@@ -240,7 +240,7 @@ gemm_quad_kernel(const uint8_t *__restrict__ A, const uint8_t *__restrict__ B, v
 template <int OP>
 int launch_quad(mi355_dev *dev, const char *what, const void *A, const void *B, void *C, uint32_t M, uint32_t N, uint32_t k_bytes,
                 float scale, const uint8_t *scales_a = nullptr, const uint8_t *scales_b = nullptr) {
-  if (int rc = allow_full_lds(dev, &gemm_quad_kernel<OP>, kLdsQuad0 + OP)) return rc;
+  if (int rc = allow_full_lds<kLdsQuad, OP>(dev, &gemm_quad_kernel<OP>)) return rc;
   const uint32_t tiles_m = M / kTile, tiles_n = N / kTile;
   // A 16-bit C goes past the caches (non-temporal stores) when the operands alone fill the 256 MiB last-level cache: C
   // lines kept there would only push out operand rows that the next round of tiles reads again (bf16 8192^3: 524 ->

@@ -192,10 +192,18 @@ struct GemmRing {
 constexpr size_t kRingBytes = 5 * (size_t)kSlabBytes;   // five 32 KiB slots: all 160 KiB of a CU
 
 // A kernel that takes the whole LDS must be allowed to, once per device handle (the attribute belongs to
-// the function on the handle's device).  `bit` names the kernel within mi355_dev::full_lds_allowed.
-enum { kLdsF32 = 0 /* gemm_quad.h: kLdsQuad0 + the operand kind of gemm_quad_kernel */ };
-template <typename Kernel>
-inline int allow_full_lds(mi355_dev *dev, Kernel kernel, unsigned bit) {
+// the function on the handle's device).  mi355_dev::full_lds_allowed has a bit for each instance of them, family by family.
+enum LdsFamily { kLdsF32, kLdsQuad, kLdsSmall, kLdsFfnAcross, kLdsFfnQuad, kLdsFfnSmall, kLdsFfnMid, kLdsFfnTall, kLdsFamilies };
+constexpr unsigned kLdsInstances[kLdsFamilies] = {1, 6, 5, 8, 8, 7, 7, 7};
+constexpr unsigned lds_bit(int family, unsigned instance) {
+  for (int f = 0; f < family; f++) instance += kLdsInstances[f];
+  return instance;
+}
+static_assert(lds_bit(kLdsFamilies, 0) <= 64, "one bit for each instance");
+template <LdsFamily FAMILY, unsigned INSTANCE, typename Kernel>
+inline int allow_full_lds(mi355_dev *dev, Kernel kernel) {
+  static_assert(INSTANCE < kLdsInstances[FAMILY], "an instance of the family");
+  constexpr unsigned bit = lds_bit(FAMILY, INSTANCE);
   if (dev->full_lds_allowed & (1ull << bit)) return MI355_OK;
   MI355_HIP(dev, hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                                      (int)kRingBytes));

@@ -156,7 +156,7 @@ gemm_small_kernel(const uint8_t *__restrict__ A, const uint8_t *__restrict__ B, 
 
 template <int OP>
 int launch_small(mi355_dev *dev, const char *what, const void *A, const void *B, void *C, uint32_t M, uint32_t N, uint32_t k_bytes, float scale) {
-  if (int rc = allow_full_lds(dev, &gemm_small_kernel<OP>, kLdsSmall0 + OP)) return rc;
+  if (int rc = allow_full_lds<kLdsSmall, OP>(dev, &gemm_small_kernel<OP>)) return rc;
   const uint32_t tiles_m = M / kSmallTile, tiles_n = N / kSmallTile;
   gemm_small_kernel<OP><<<tiles_m * tiles_n, kSmallThreads, kRingBytes, dev->stream>>>((const uint8_t *)A, (const uint8_t *)B, C, N, k_bytes, scale,
                                                                                          tiles_m, tiles_n);

@@ -1,0 +1,108 @@
+"""What the entry points do on the host, on a HIP runtime without a GPU (tests/hip_stub.cpp), in a process of their own."""
+import json
+import os
+import subprocess
+import sys
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+PRELUDE = """
+import ctypes as C, json, sys
+stub = C.CDLL(%r, mode=C.RTLD_GLOBAL)
+stub.stub_stream.restype = C.c_void_p
+sys.path.insert(0, %r)
+from clpeak_amd import capi
+P = 1 << 20        # an address that nothing reads
+def counts():
+    a = (C.c_int * 4)()
+    stub.stub_counts(a)
+    return dict(zip(("launches", "refused", "wrong_device", "big_lds"), a))
+def gradients(d, type, T, F, D, dx=True, dw=True):
+    n = d.glu_backward_workspace(T, F, D)
+    d.glu_backward(type, 0, P, F, P, D, P, P, D, P, P, F, P if dx else None, D, P if dw else None, P if dw else None, D, T, F, D, P, n)
+"""
+
+
+@pytest.fixture(scope="module")
+def stub(tmp_path_factory):
+    so = str(tmp_path_factory.mktemp("hip") / "hip_stub.so")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", "-Wno-deprecated-declarations",
+                    os.path.join(ROOT, "tests", "hip_stub.cpp"), "-o", so], check=True, capture_output=True, timeout=300)
+
+    def run(code):
+        r = subprocess.run([sys.executable, "-c", PRELUDE % (so, ROOT) + code], capture_output=True, text=True, timeout=120)
+        assert r.returncode == 0, r.stderr[-3000:]
+        return json.loads(r.stdout.splitlines()[-1])
+    return run
+
+
+# One call for each kernel that takes more than 64 KiB of LDS, by name.
+LDS_CALLS = """
+def tiled(d, tiling, call):
+    d.gemm_tiling(tiling)
+    call()
+    d.gemm_tiling(capi.GEMM_TILING_AUTO)
+def glu(d, type, T):
+    d.glu_forward(type, 0, P, 128, P, P, 128, P, 512, None, None, 0, T, 512, 128)
+def i8(d, type, ws):
+    n = d.gemm_i8_scaled_workspace(512, 512, 16384) if ws else 0
+    d.gemm_i8_scaled(P, 16384, P, 16384, P, P, None, type, P, 512, 512, 512, 16384, P if ws else None, n)
+def glu_i8(d, type):
+    d.glu_i8(0, P, 128, P, P, 128, P, P, P, type, P, 512, 512, 512, 128)
+raw = lambda d, name, *a: d._check(getattr(d.lib, "mi355_" + name)(d.h, *a))
+big, mid, low, tall = capi.GEMM_TILING_256, capi.GEMM_TILING_128, capi.GEMM_TILING_64, capi.GEMM_TILING_256X128
+calls = {"f32": lambda d: raw(d, "gemm_f32", P, P, P, 512, 512, 512)}
+for t in (big, mid):
+    for name, more in (("gemm_bf16", ()), ("gemm_f16", ()), ("gemm_i8", ()), ("gemm_fp8_e4m3", (1.0, 1.0)), ("gemm_fp8_e5m2", (1.0, 1.0))):
+        calls["%s %d" % (name, t)] = lambda d, t=t, name=name, more=more: tiled(d, t, lambda: raw(d, name, P, P, P, 512, 512, 512, *more))
+calls["mxfp4"] = lambda d: raw(d, "gemm_mxfp4", P, P, P, P, P, 512, 512, 512)
+for t in (big, mid, low, tall):
+    for type in (0, 1):
+        calls["glu %d %d" % (type, t)] = lambda d, t=t, type=type: tiled(d, t, lambda: glu(d, type, 512))
+        calls["gradients %d %d" % (type, t)] = lambda d, t=t, type=type: tiled(d, t, lambda: gradients(d, type, 512, 512, 512))
+        calls["dW in slices %d %d" % (type, t)] = lambda d, t=t, type=type: tiled(d, t, lambda: gradients(d, type, 8192, 256, 256, dx=False))
+        calls["dX in slices %d %d" % (type, t)] = lambda d, t=t, type=type: tiled(d, t, lambda: gradients(d, type, 256, 8192, 256, dw=False))
+    for type in (0, 1, 2):
+        calls["int8 %d %d" % (type, t)] = lambda d, t=t, type=type: tiled(d, t, lambda: i8(d, type, False))
+        calls["int8 in slices %d %d" % (type, t)] = lambda d, t=t, type=type: tiled(d, t, lambda: i8(d, type, True))
+        calls["gated int8 %d %d" % (type, t)] = lambda d, t=t, type=type: tiled(d, t, lambda: glu_i8(d, type))
+"""
+
+
+def test_every_kernel_that_takes_a_whole_cus_lds_is_allowed_to_whatever_ran_before(stub):
+    """Every ordered pair of such calls on a handle of its own: no launch asks for more LDS than its kernel was allowed."""
+    got = stub(LDS_CALLS + """
+pairs = {}
+for a in calls:
+    for b in calls:
+        d = capi.Device(0)
+        before = counts()["refused"]
+        stub.stub_forget()
+        calls[a](d)
+        calls[b](d)
+        if counts()["refused"] != before:
+            pairs[a + ", " + b] = counts()["refused"] - before
+        d.close()
+print(json.dumps({"pairs": pairs, "counts": counts(), "calls": len(calls)}))
+""")
+    assert got["calls"] == 80 and got["counts"]["big_lds"] >= 2 * got["calls"] ** 2
+    assert got["pairs"] == {}
+
+
+def test_dW_of_a_training_batch_and_the_fp8_product(stub):
+    """The library's own choices: the sums of dW in slices in fp16, then the fp8 product on 256x256 tiles, and the other way."""
+    got = stub("""
+seen = []
+for order in (0, 1):
+    stub.stub_forget()
+    d = capi.Device(0)
+    one = lambda: gradients(d, capi.TYPE_F16, 8192, 1024, 4096)
+    two = lambda: d._check(d.lib.mi355_gemm_fp8_e4m3(d.h, P, P, P, 8192, 8192, 8192, 1.0, 1.0))
+    for call in ((one, two) if order else (two, one)):
+        call()
+    seen.append(counts()["refused"])
+print(json.dumps(seen))
+""")
+    assert got == [0, 0]
