@@ -53,7 +53,8 @@ static int open_device(int ordinal, const hipStream_t *stream, mi355_dev **out) 
     return mi355_fail(nullptr, MI355_ERR_ARCH,
                       "device %d is %s; this backend holds gfx950 code only", ordinal, p.gcnArchName);
 
-  e = hipSetDevice(ordinal);
+  mi355_on_device on;
+  e = on.to(ordinal);
   if (e != hipSuccess)
     return mi355_fail(nullptr, MI355_ERR_HIP, "hipSetDevice: %s", hipGetErrorString(e));
 
@@ -108,7 +109,8 @@ extern "C" int mi355_open_on_stream(int ordinal, void *stream, mi355_dev **out) 
 
 extern "C" int mi355_close(mi355_dev *dev) {
   if (!dev) return MI355_OK;
-  (void)hipSetDevice(dev->ordinal);
+  mi355_on_device on;
+  (void)on.to(dev->ordinal);
   // (a borrowed stream may be gone already: only the release of scratch memory below waits, for the whole device)
   if (dev->owns_stream && dev->stream) (void)hipStreamSynchronize(dev->stream);
   if (dev->mx_scratch) (void)hipFree(dev->mx_scratch);

@@ -54,17 +54,32 @@ int mi355_mx_resolve_static_scratch(mi355_dev *dev);
     if (!(cond)) return mi355_fail((dev), MI355_ERR_ARG, __VA_ARGS__);                  \
   } while (0)
 
+// A device current on the calling thread for the length of a scope; then the one that was, which is the caller's affair.
+struct mi355_on_device {
+  int before = -1;
+  hipError_t to(int ordinal) {
+    int now = -1;
+    if (hipGetDevice(&now) == hipSuccess && now == ordinal) return hipSuccess;
+    const hipError_t e = hipSetDevice(ordinal);
+    if (e == hipSuccess) before = now;
+    return e;
+  }
+  ~mi355_on_device() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+};
+
 // The two halves of MI355_ENTER below, for entry points that check their arguments before they touch the device.
 #define MI355_HANDLE(dev)                                                               \
   do {                                                                                  \
     if (!(dev)) return mi355_fail(nullptr, MI355_ERR_ARG, "null device handle");        \
   } while (0)
-#define MI355_SET_DEVICE(dev) MI355_HIP((dev), hipSetDevice((dev)->ordinal))
+#define MI355_SET_DEVICE(dev)                                                           \
+  mi355_on_device on_device_;                                                           \
+  MI355_HIP((dev), on_device_.to((dev)->ordinal))
 
 // Every entry point that touches the device starts with this: validates the handle
-// and makes its device current on the calling thread.
+// and makes its device current on the calling thread until the entry point returns.
 #define MI355_ENTER(dev)                                                                \
-  do {                                                                                  \
-    if (!(dev)) return mi355_fail(nullptr, MI355_ERR_ARG, "null device handle");        \
-    MI355_HIP((dev), hipSetDevice((dev)->ordinal));                                     \
-  } while (0)
+  MI355_HANDLE(dev);                                                                    \
+  MI355_SET_DEVICE(dev)

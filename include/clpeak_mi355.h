@@ -8,6 +8,8 @@
  * a handle is not thread-safe, different handles may be used from different
  * threads.  Every `*_launch_*`-style entry point ENQUEUES on the handle's stream
  * and returns without waiting; use mi355_sync() or the timer pair to wait.
+ * Calls run on the handle's device and leave the calling thread's current
+ * device as they found it.
  *
  * The reference has no C boundary between a backend and HIP (a backend is a C++
  * class that calls hipModuleLaunchKernel itself), so each entry point below

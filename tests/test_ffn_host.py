@@ -106,3 +106,57 @@ for order in (0, 1):
 print(json.dumps(seen))
 """)
     assert got == [0, 0]
+
+
+def test_calls_leave_the_current_device_as_they_found_it(stub):
+    """A program with torch on one GPU and a handle on another: what the handle launches runs on its device, refused calls and
+    errors included, and the thread's current device is the program's again afterwards."""
+    got = stub(LDS_CALLS + """
+moved, n = [], 0
+def check(what, at):
+    global n
+    n += 1
+    if stub.stub_current() != at:
+        moved.append([what, at, stub.stub_current()])
+        stub.stub_make_current(at)
+for at in (0, 1):
+    for on in (0, 1):
+        for borrowed in (False, True, None):
+            stub.stub_make_current(at)
+            d = capi.Device(on, stream=None if borrowed is None else stub.stub_stream(on) if borrowed else 0)
+            check("open", at)
+            for name, call in calls.items():
+                call(d)
+                check(name, at)
+            d.quantize_i8(0, P, 128, P, 128, P, 5, 128, 128)
+            check("quantize_i8", at)
+            b = d.alloc(4096)
+            check("alloc", at)
+            d._check(d.lib.mi355_memset(d.h, P, 0, 64))
+            check("memset", at)
+            d.fill_f32(b, 64, 1, 0, 0)
+            check("fill_f32", at)
+            d.timer_start(); check("timer_start", at)
+            d.timer_stop(); check("timer_stop", at)
+            d.sync(); check("sync", at)
+            try:
+                d.glu_forward(7, 0, P, 128, P, P, 128, P, 512, None, None, 0, 5, 512, 128)
+            except capi.Mi355Error:
+                check("refused", at)
+            try:
+                raw(d, "gemm_bf16", P, P, P, 100, 100, 100)
+            except capi.Mi355Error:
+                check("refused later", at)
+            b.free()
+            check("free", at)
+            d.close()
+            check("close", at)
+try:
+    capi.Device(5)
+except capi.Mi355Error:
+    check("open of no device", 1)
+print(json.dumps({"moved": moved[:10], "all": len(moved), "checked": n, "counts": counts()}))
+""")
+    assert got["checked"] > 12 * 85 and got["counts"]["launches"] > 12 * 85
+    assert got["moved"] == [] and got["all"] == 0
+    assert got["counts"]["wrong_device"] == 0
