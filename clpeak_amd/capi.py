@@ -6,6 +6,7 @@ at load time, and every non-zero status from the library raises :class:`Mi355Err
 """
 import ctypes as C
 import os
+import sys
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libclpeak_mi355.so")
@@ -128,12 +129,18 @@ def load_library(path=LIB_PATH):
     return lib
 
 
-def _ptr(buf):
-    """The device address of a DeviceBuffer, of anything else that has data_ptr() (a torch tensor), or a plain address;
-    None stays None."""
-    if buf is None or isinstance(buf, int):
-        return buf
-    return buf.data_ptr() if hasattr(buf, "data_ptr") else buf.ptr
+class _TorchTypes(dict):
+    """The torch type of elements of a kind (TYPE_*, "i8"); None for others.  Filled once torch is there."""
+
+    def __missing__(self, kind):
+        torch = sys.modules.get("torch")
+        if torch and not self:
+            self.update({TYPE_BF16: torch.bfloat16, TYPE_F16: torch.float16, TYPE_F32: torch.float32, "i8": torch.int8})
+            return self[kind]
+        return None
+
+
+_torch_types = _TorchTypes()
 
 
 class DeviceBuffer:
@@ -179,7 +186,7 @@ class Device:
         rc = self.lib.mi355_open(ordinal, C.byref(h)) if stream is None else self.lib.mi355_open_on_stream(ordinal, stream, C.byref(h))
         if rc != OK:
             raise Mi355Error(rc, (self.lib.mi355_last_error(None) or b"").decode())
-        self.h = h
+        self.h, self.ordinal = h, ordinal
         p = Props()
         self._check(self.lib.mi355_get_props(self.h, C.byref(p)))
         self.props = p
@@ -344,9 +351,45 @@ class Device:
         self._check(self.lib.mi355_gemm_fp8_e4m3(self.h, A.ptr, B.ptr, Cbuf.ptr, M, N, K, scale_a, scale_b))
 
     # --- feed-forward operators: buffers are DeviceBuffers, torch tensors or addresses; strides in elements ---------------
+    # A tensor or DeviceBuffer has to be on the handle's device, a tensor of the type that the call takes it for; where it starts,
+    # its strides and sizes are the caller's to say.
+    def _ptrs(self, call, names, kinds, bufs):
+        """Addresses of buffers, each of elements of a kind (TYPE_*, "i8")."""
+        out, types, ordinal = [], _torch_types, self.ordinal
+        for b, kind in zip(bufs, kinds):
+            if b is not None:
+                try:
+                    if b.get_device() != ordinal or b.dtype is not types[kind]:
+                        self._refuse(call, names.split()[len(out)], b, types[kind])
+                    b = b.data_ptr()
+                except AttributeError:   # (not a torch tensor)
+                    if not isinstance(b, int):
+                        if isinstance(b, DeviceBuffer) and b.dev.ordinal != ordinal:
+                            raise Mi355Error(ERR_ARG, f"{call}: {names.split()[len(out)]} is on GPU {b.dev.ordinal}, the handle is on GPU {ordinal}")
+                        b = b.data_ptr() if hasattr(b, "data_ptr") else b.ptr
+            out.append(b)
+        return out
+
+    def _refuse(self, call, name, tensor, wanted):
+        if tensor.get_device() != self.ordinal:
+            raise Mi355Error(ERR_ARG, f"{call}: {name} is a tensor on {tensor.device}, the handle is on GPU {self.ordinal}")
+        if wanted is not None:   # (None: no such type, which the library says)
+            raise Mi355Error(ERR_ARG, f"{call}: {name} is a tensor of {tensor.dtype}, elements of {wanted} are needed")
+
+    def _workspace(self, call, workspace, nbytes):
+        if workspace is None or isinstance(workspace, int):
+            return workspace
+        if workspace.nbytes < nbytes:
+            raise Mi355Error(ERR_ARG, f"{call}: the workspace has {workspace.nbytes} bytes, not {nbytes}")
+        if isinstance(workspace, DeviceBuffer):
+            return self._ptrs(call, "workspace", (None,), (workspace,))[0]
+        if workspace.get_device() != self.ordinal:
+            self._refuse(call, "workspace", workspace, None)
+        return workspace.data_ptr()
+
     def glu_forward(self, type, act, X, ldx, Wg, Wu, ldw, H, ldh, G, U, ldg, T, F, D):
-        self._check(self.lib.mi355_glu_forward(self.h, type, act, _ptr(X), ldx, _ptr(Wg), _ptr(Wu), ldw, _ptr(H), ldh, _ptr(G), _ptr(U), ldg,
-                                               T, F, D))
+        X, Wg, Wu, H, G, U = self._ptrs("glu_forward", "X Wg Wu H G U", (type,) * 6, (X, Wg, Wu, H, G, U)) if T else (None,) * 6
+        self._check(self.lib.mi355_glu_forward(self.h, type, act, X, ldx, Wg, Wu, ldw, H, ldh, G, U, ldg, T, F, D))
 
     def glu_backward_workspace(self, T, F, D):
         n = C.c_size_t()
@@ -355,11 +398,16 @@ class Device:
 
     def glu_backward(self, type, act, dH, lddh, X, ldx, Wg, Wu, ldw, G, U, ldg, dX, lddx, dWg, dWu, lddw, T, F, D, workspace,
                      workspace_bytes):
-        self._check(self.lib.mi355_glu_backward(self.h, type, act, _ptr(dH), lddh, _ptr(X), ldx, _ptr(Wg), _ptr(Wu), ldw, _ptr(G), _ptr(U), ldg,
-                                                _ptr(dX), lddx, _ptr(dWg), _ptr(dWu), lddw, T, F, D, _ptr(workspace), workspace_bytes))
+        if not T:
+            dH = X = Wg = Wu = G = U = dX = None
+        dWg, dWu, dH, X, Wg, Wu, G, U, dX = self._ptrs("glu_backward", "dWg dWu dH X Wg Wu G U dX", (type,) * 9, (dWg, dWu, dH, X, Wg, Wu, G, U, dX))
+        workspace = self._workspace("glu_backward", workspace, workspace_bytes)
+        self._check(self.lib.mi355_glu_backward(self.h, type, act, dH, lddh, X, ldx, Wg, Wu, ldw, G, U, ldg, dX, lddx, dWg, dWu, lddw, T, F, D,
+                                                workspace, workspace_bytes))
 
     def quantize_i8(self, type, X, ldx, Q, ldq, scale, M, K, k_pad):
-        self._check(self.lib.mi355_quantize_i8(self.h, type, _ptr(X), ldx, _ptr(Q), ldq, _ptr(scale), M, K, k_pad))
+        X, Q, scale = self._ptrs("quantize_i8", "X Q scale", (type, "i8", TYPE_F32), (X, Q, scale)) if M else (None,) * 3
+        self._check(self.lib.mi355_quantize_i8(self.h, type, X, ldx, Q, ldq, scale, M, K, k_pad))
 
     def gemm_i8_scaled_workspace(self, M, N, K):
         n = C.c_size_t()
@@ -367,9 +415,13 @@ class Device:
         return n.value
 
     def gemm_i8_scaled(self, A, lda, B, ldb, scale_a, scale_b, bias, type, Cbuf, ldc, M, N, K, workspace=None, workspace_bytes=0):
-        self._check(self.lib.mi355_gemm_i8_scaled(self.h, _ptr(A), lda, _ptr(B), ldb, _ptr(scale_a), _ptr(scale_b), _ptr(bias), type,
-                                                  _ptr(Cbuf), ldc, M, N, K, _ptr(workspace), workspace_bytes))
+        call = "gemm_i8_scaled"
+        A, B, scale_a, scale_b, bias, Cbuf = self._ptrs(call, "A B scale_a scale_b bias C", ("i8", "i8", TYPE_F32, TYPE_F32, TYPE_F32, type),
+                                                        (A, B, scale_a, scale_b, bias, Cbuf)) if M else (None,) * 6
+        workspace = self._workspace(call, workspace, workspace_bytes)
+        self._check(self.lib.mi355_gemm_i8_scaled(self.h, A, lda, B, ldb, scale_a, scale_b, bias, type, Cbuf, ldc, M, N, K, workspace, workspace_bytes))
 
     def glu_i8(self, act, A, lda, Bg, Bu, ldb, scale_a, scale_g, scale_u, type, H, ldh, M, F, K):
-        self._check(self.lib.mi355_glu_i8(self.h, act, _ptr(A), lda, _ptr(Bg), _ptr(Bu), ldb, _ptr(scale_a), _ptr(scale_g), _ptr(scale_u),
-                                          type, _ptr(H), ldh, M, F, K))
+        A, Bg, Bu, scale_a, scale_g, scale_u, H = self._ptrs("glu_i8", "A Bg Bu scale_a scale_g scale_u H", ("i8",) * 3 + (TYPE_F32,) * 3 + (type,),
+                                                             (A, Bg, Bu, scale_a, scale_g, scale_u, H)) if M else (None,) * 7
+        self._check(self.lib.mi355_glu_i8(self.h, act, A, lda, Bg, Bu, ldb, scale_a, scale_g, scale_u, type, H, ldh, M, F, K))

@@ -19,7 +19,7 @@ struct Config {
 thread_local Config config;
 std::map<std::pair<int, const void *>, int> allowed;
 int launches = 0, refused = 0, wrong_device = 0, big_lds = 0;
-char memory[1 << 16];
+alignas(4096) char memory[1 << 16];
 int stream_of[kDevices] = {0, 1};
 
 int device_of(hipStream_t s) { return s ? *reinterpret_cast<int *>(s) : current; }

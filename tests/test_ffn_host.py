@@ -160,3 +160,59 @@ print(json.dumps({"moved": moved[:10], "all": len(moved), "checked": n, "counts"
     assert got["checked"] > 12 * 85 and got["counts"]["launches"] > 12 * 85
     assert got["moved"] == [] and got["all"] == 0
     assert got["counts"]["wrong_device"] == 0
+
+
+def test_tensors_that_a_call_cannot_take_are_refused_before_it(stub):
+    """Each buffer of each Python call in turn: a tensor in host memory, on another GPU, of another type; a workspace shorter
+    than said; buffers of a handle on another GPU.  Nothing is launched.  The same calls with tensors that fit go through."""
+    got = stub("""
+import torch
+class Tensor:      # as much of a tensor as is looked at
+    def __init__(self, dtype, gpu=0, nbytes=1 << 30):
+        self.dtype, self.gpu, self.nbytes, self.device = dtype, gpu, nbytes, "cuda:%d" % gpu
+    def get_device(self):
+        return self.gpu
+    def data_ptr(self):
+        return P
+d, other = capi.Device(0), capi.Device(1)
+h, i8, f32 = torch.float16, torch.int8, torch.float32
+calls = {
+    "glu_forward": (lambda X, Wg, Wu, H, G, U: d.glu_forward(1, 0, X, 128, Wg, Wu, 128, H, 64, G, U, 64, 5, 64, 128), [h] * 6),
+    "glu_backward": (lambda dH, X, Wg, Wu, G, U, dX, dWg, dWu, ws: d.glu_backward(1, 0, dH, 64, X, 128, Wg, Wu, 128, G, U, 64, dX, 128, dWg, dWu, 128, 5, 64, 128, ws,
+                     d.glu_backward_workspace(5, 64, 128)), [h] * 9 + [None]),
+    "quantize_i8": (lambda X, Q, scale: d.quantize_i8(1, X, 128, Q, 128, scale, 5, 128, 128), [h, i8, f32]),
+    "gemm_i8_scaled": (lambda A, B, sa, sb, bias, C, ws: d.gemm_i8_scaled(A, 128, B, 128, sa, sb, bias, 1, C, 64, 5, 64, 128, ws, 64), [i8, i8, f32, f32, f32, h, None]),
+    "glu_i8": (lambda A, Bg, Bu, sa, sg, su, H: d.glu_i8(0, A, 128, Bg, Bu, 128, sa, sg, su, 1, H, 64, 5, 64, 128), [i8, i8, i8, f32, f32, f32, h]),
+}
+fits = lambda t: Tensor(t or torch.uint8)
+passed, refused, wrong = 0, 0, []
+for name, (call, types) in calls.items():
+    for buffers in ([fits(t) for t in types], [P] * len(types), [d.alloc(1 << 20) for _ in types]):
+        before = counts()["launches"]
+        call(*buffers)
+        passed += counts()["launches"] > before
+    for k, t in enumerate(types):
+        bad = [torch.zeros(64, dtype=t or torch.uint8), Tensor(t or torch.uint8, gpu=1), other.alloc(1 << 20)]
+        bad.append(Tensor(torch.bfloat16 if t in (h, f32) else torch.uint8) if t else Tensor(torch.uint8, nbytes=63))
+        for b in bad:
+            before = counts()["launches"]
+            try:
+                call(*[b if j == k else fits(u) for j, u in enumerate(types)])
+                wrong.append([name, k, "taken"])
+            except capi.Mi355Error as e:
+                refused += 1
+                if e.code != capi.ERR_ARG or name + ":" not in str(e):
+                    wrong.append([name, k, str(e)])
+            if counts()["launches"] != before:
+                wrong.append([name, k, "launched"])
+# no rows: nothing is looked at
+f = Tensor(torch.float64, gpu=1)
+d.glu_forward(1, 0, f, 128, f, f, 128, f, 64, f, f, 64, 0, 64, 128)
+d.quantize_i8(1, f, 128, f, 128, f, 0, 128, 128)
+d.gemm_i8_scaled(f, 128, f, 128, f, f, f, 1, f, 64, 0, 64, 128)
+d.glu_i8(0, f, 128, f, f, 128, f, f, f, 1, f, 64, 0, 64, 128)
+d.glu_backward(1, 0, f, 64, f, 128, f, f, 128, f, f, 64, f, 128, fits(h), fits(h), 128, 0, 64, 128, P, d.glu_backward_workspace(0, 64, 128))
+print(json.dumps({"passed": passed, "refused": refused, "wrong": wrong}))
+""")
+    assert got["wrong"] == []
+    assert got["passed"] == 15 and got["refused"] == 4 * 33
