@@ -1,9 +1,11 @@
 """Paths of the feed-forward operators that tests/test_gpu_ffn.py does not reach."""
+import math
+
 import pytest
 import torch
 
 from clpeak_amd import capi
-from test_gpu_ffn import E, TYPES, dv, gen, operand, padded, untouched, within  # noqa: F401
+from test_gpu_ffn import E, TYPES, dv, gen, operand, padded, quantized, untouched, within  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -30,3 +32,23 @@ def test_glu_forward_many_rounds_of_rows_that_start_on_lines(dv, type, keep):
         assert untouched(gb, G, ld, -7.0) and untouched(ub, U, ld, -7.0)
     else:
         assert bool((gb == -7.0).all()) and bool((ub == -7.0).all())
+
+
+@pytest.mark.parametrize("type", list(TYPES))
+@pytest.mark.parametrize("M, K, k_pad", [(3, 65535, 65536), (2, 65536, 65536), (3, 65537, 65664), (2, 73729, 73729), (3, 130957, 131072)])
+def test_quantize_rows_that_registers_do_not_hold(dv, type, M, K, k_pad):
+    """Rows around and past 65536 elements, which are read twice; the largest value in the last, partial chunk, in the first
+    or in between."""
+    dt = TYPES[type]
+    g = gen(K)
+    ldx, ldq = K + 3, k_pad + 1
+    _, x = padded(M, K, ldx, dt, math.nan)
+    x.copy_(torch.randn(M, K, generator=g, device="cuda").to(dt))
+    for m, at in enumerate((K - 1, 0, 40000)[:M]):
+        x[m, at] = -9.0
+    qb, q = padded(M, k_pad, ldq, torch.int8, 77)
+    s = torch.full((M + 1,), -1.0, device="cuda")
+    dv.quantize_i8(type, x, ldx, q, ldq, s, M, K, k_pad)
+    rq, rs = quantized(x)
+    assert torch.equal(q[:, :K].double(), rq) and torch.equal(s[:-1], rs) and s[-1] == -1
+    assert bool((q[:, K:] == 0).all()) and untouched(qb, q, ldq, 77)
