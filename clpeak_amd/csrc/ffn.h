@@ -243,8 +243,9 @@ __device__ __forceinline__ void ffn_store1(void *base, uint64_t at, int type, fl
   static_cast<uint16_t *>(base)[at] = (uint16_t)p;
 }
 
-// int32 sum -> value.  The sum is rounded to fp32 (exact below 2^24), then multiplied by the two scales in turn, so that
-// neither product of a small and a large scale leaves the range before the sum is in it.
+// int32 sum -> value.  The sum is rounded to fp32 (exact below 2^24), then multiplied by the two scales in turn.  The first
+// product never loses bits below the range (the sum is a whole number) and leaves it above only for scale_a of 2^97 and
+// more, which the header rules out: to take the smaller scale first would cost three operations a sum.
 __device__ __forceinline__ float ffn_scaled(int32_t sum, float sa, float sb) { return (float)sum * sa * sb; }
 // (the addition as one operation with the second product, in every kernel alike)
 __device__ __forceinline__ float ffn_scaled_plus(int32_t sum, float sa, float sb, float bias) { return fmaf((float)sum * sa, sb, bias); }

@@ -404,7 +404,8 @@ int mi355_quantize_i8(mi355_dev *dev, int type, const void *X, uint64_t ldx, int
                       uint32_t M, uint32_t K, uint32_t k_pad);
 /* The product of such rows:  C[m][n] = scale_a[m] * scale_b[n] * sum_k A[m][k] B[n][k] + bias[n].   A[M][K], B[N][K] int8,
  * scales and bias fp32 (bias NULL: none), C[M][N] of `type` (MI355_TYPE_*).  The sum is exact (int32; K at most 130944);
- * the rest is fp32, C is rounded once.
+ * the rest is fp32, C is rounded once.  scale_a times the sum has to be in fp32's range, as it is for every scale_a below 2^97
+ * (beyond, the result is infinite also where a small scale_b would bring it back); scale_b may be anything.
  * A workspace lets a product of few tiles and a long K be split along K (the sums stay exact); without one (NULL, 0) it
  * is not split.  mi355_gemm_i8_scaled_workspace: the bytes that M, N, K can use, 0 where the product is not split anyway;
  * a smaller workspace counts as none.  On 16 bytes. */
@@ -414,7 +415,7 @@ int mi355_gemm_i8_scaled(mi355_dev *dev, const int8_t *A, uint64_t lda, const in
                          void *workspace, size_t workspace_bytes);
 /* The gated projection on such rows, in one kernel:
  *     H[m][f] = act(scale_a[m] * scale_g[f] * (A Bg^T)[m][f]) * (scale_a[m] * scale_u[f] * (A Bu^T)[m][f])
- * A[M][K], Bg[F][K], Bu[F][K] (both ldb apart) int8, H[M][F] of `type`. */
+ * A[M][K], Bg[F][K], Bu[F][K] (both ldb apart) int8, H[M][F] of `type`; scale_a as in mi355_gemm_i8_scaled. */
 int mi355_glu_i8(mi355_dev *dev, int act, const int8_t *A, uint64_t lda, const int8_t *Bg, const int8_t *Bu, uint64_t ldb,
                  const float *scale_a, const float *scale_g, const float *scale_u, int type, void *H, uint64_t ldh,
                  uint32_t M, uint32_t F, uint32_t K);

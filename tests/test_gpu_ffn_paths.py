@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from clpeak_amd import capi
-from test_gpu_ffn import E, TYPES, dv, gen, operand, padded, quantized, untouched, within  # noqa: F401
+from test_gpu_ffn import E, TYPES, dv, gen, i8_problem, operand, padded, quantized, tiled, untouched, within  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -52,3 +52,19 @@ def test_quantize_rows_that_registers_do_not_hold(dv, type, M, K, k_pad):
     rq, rs = quantized(x)
     assert torch.equal(q[:, :K].double(), rq) and torch.equal(s[:-1], rs) and s[-1] == -1
     assert bool((q[:, K:] == 0).all()) and untouched(qb, q, ldq, 77)
+
+
+def test_gemm_i8_scaled_scales_at_the_ends_of_their_range(tiled):
+    """scale_a below 2^97 against any scale_b: the product with the largest sum stays in fp32's range, and with a scale_b as
+    small as scale_a is large so does the result."""
+    dv = tiled
+    M, N, K = 40, 50, 256
+    g, a, lda, (b,), ldb, sa, (sb,) = i8_problem(M, N, K, 10)
+    a[1, :], b[1, :] = -128, -128
+    sa[1], sb[1], sa[2], sb[2] = 2.0 ** 96, 2.0 ** -96, 2.0 ** -126, 2.0 ** 120
+    c = torch.empty(M, N, device="cuda")
+    dv.gemm_i8_scaled(a, lda, b, ldb, sa, sb, None, capi.TYPE_F32, c, N, M, N, K)
+    prod = (a.double() @ b.double().T) * sa.double()[:, None] * sb.double()[None, :]
+    for m, n in ((1, 1), (2, 2)):
+        assert abs(float(c[m, n]) - float(prod[m, n])) <= 4 * E * abs(float(prod[m, n]))
+    assert float(c[1, 1]) == 128 * 128 * K
