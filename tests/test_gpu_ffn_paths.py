@@ -68,3 +68,34 @@ def test_gemm_i8_scaled_scales_at_the_ends_of_their_range(tiled):
     for m, n in ((1, 1), (2, 2)):
         assert abs(float(c[m, n]) - float(prod[m, n])) <= 4 * E * abs(float(prod[m, n]))
     assert float(c[1, 1]) == 128 * 128 * K
+
+
+@pytest.mark.parametrize("first", ["gradients", "product"])
+def test_fp16_gradients_in_slices_and_the_fp8_product_on_one_handle(first):
+    """Both kernels take the whole LDS of a CU, each by a permission of its own."""
+    T, F, D, n = 8192, 512, 4096, 512
+    d = capi.Device(0, stream=torch.cuda.current_stream().cuda_stream)
+    g = gen(5)
+    dh, x, G, U = (operand(g, T, c, c, torch.float16) for c in (F, D, F, F))
+    dw = torch.empty(2, F, D, dtype=torch.float16, device="cuda")
+    a, b = (torch.randint(0, 8, (n, n), generator=g, device="cuda").float().to(torch.float8_e4m3fn) for _ in range(2))
+    c = torch.empty(n, n, dtype=torch.bfloat16, device="cuda")
+    size = d.glu_backward_workspace(T, F, D)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+
+    def gradients():
+        d.glu_backward(capi.TYPE_F16, capi.GLU_RELU, dh, F, x, D, None, None, D, G, U, F, None, D, dw[0], dw[1], D, T, F, D, ws, size)
+
+    def product():
+        d.gemm_tiling(capi.GEMM_TILING_256)
+        d._check(d.lib.mi355_gemm_fp8_e4m3(d.h, a.data_ptr(), b.data_ptr(), c.data_ptr(), n, n, n, 1.0, 1.0))
+        d.gemm_tiling(capi.GEMM_TILING_AUTO)
+
+    for call in ((gradients, product) if first == "gradients" else (product, gradients)):
+        call()
+    ref = a.double() @ b.double().T
+    within(c, ref, 2 * n * E * ref.abs(), torch.bfloat16)
+    dU = dh.double() * G.double().clamp(min=0)
+    within(dw[1], dU.T @ x.double(), (2.0 ** -11 + 2 * T * E) * (dU.abs().T @ x.double().abs()), torch.float16)
+    torch.cuda.synchronize()
+    d.close()
