@@ -118,3 +118,57 @@ def test_bf16_gradients_of_factors_that_are_far_apart(tiled, rows):
     assert float(ref.abs().max()) < 3.38e38
     # (of many values dG is rounded to bf16 first)
     within(dwg[:, :T].T, ref, (50 * E + (0 if T * F <= 32768 else UNIT[dt])) * ref.abs(), dt)
+
+
+@pytest.mark.parametrize("at", [(0, 0), (4199, 1098), (0, 1098), (4199, 0), (2111, 700), (4100, 1050)])
+def test_fp16_gradients_with_the_largest_value_anywhere(dv, at):
+    """More tiles of dH than there are workgroups that look for its largest value, and one value 10^8 times the others, in the
+    first and in the last of rows and columns that are no multiples of anything: missed, it would overflow."""
+    T, F, D = 4200, 1099, 64
+    g = gen(at[0] + at[1])
+    h = lambda r, c, s: (torch.randn(r, c, generator=g, device="cuda") * s).half()  # noqa: E731
+    dh, x, wg, wu, G, U = h(T, F, 1e-5), h(T, D, 1 / 16), h(F, D, 1 / 16), h(F, D, 1 / 16), h(T, F, 1.5), h(T, F, 1)
+    dh[at], G[at], U[at] = 1000.0, 3.0, 1.0
+    got, ref, off = gradients_f16(dv, capi.GLU_SILU, dh, x, wg, wu, G, U)
+    for a, b, o in zip(got, ref, off):
+        within(a, b, o, torch.float16)
+
+
+@pytest.mark.parametrize("T, F", [(3, 384), (300, 384)])
+def test_fp16_gradients_captured_and_replayed_on_dh_of_other_sizes(T, F):
+    """The scaling is found anew on every replay: dH from 1e-6 to 1e4, infinities in between, each replay as the eager call."""
+    D = 128
+    st = torch.cuda.Stream()
+    d = capi.Device(0, stream=st.cuda_stream)
+    g = gen(61)
+    h = lambda r, c, s: (torch.randn(r, c, generator=g, device="cuda") * s).half()  # noqa: E731
+    x, wg, wu, G, U = h(T, D, 1e-3), h(F, D, 1e-3), h(F, D, 1e-3), h(T, F, 1.5), h(T, F, 1)
+    dh = torch.zeros(T, F, dtype=torch.float16, device="cuda")
+    outs = [torch.zeros(r, D, dtype=torch.float16, device="cuda") for r in (T, F, F)]
+    n = d.glu_backward_workspace(T, F, D)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+
+    def call():
+        d.glu_backward(capi.TYPE_F16, capi.GLU_SILU, dh, F, x, D, wg, wu, D, G, U, F, outs[0], D, outs[1], outs[2], D, T, F, D, ws, n)
+
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        call()
+    for size in (1e4, 1e-6, 1.0, math.inf, 1e-3, 0.0, 100.0):
+        dh.copy_(h(T, F, size if math.isfinite(size) else 1.0))
+        if not math.isfinite(size):
+            dh[1, 5] = size
+        for o in outs:
+            o.fill_(7.0)
+        ws.fill_(0xFF)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [o.clone() for o in outs]
+        call()
+        d.sync()
+        assert all(torch.equal(a.view(torch.int16), o.view(torch.int16)) for a, o in zip(got, outs)), size
+        assert bool(torch.isfinite(got[0]).all()) == math.isfinite(size) and not bool((got[0] == 7.0).any())
+    del graph
+    d.close()
