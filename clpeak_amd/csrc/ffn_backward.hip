@@ -6,7 +6,7 @@
 // and dU writes them both ways and X and the weights are turned once into the workspace.  Which of these goes by the
 // expected times: turning costs the products of a training batch (8192x8192x4096) 106 of 1585 us; one launch for all
 // three products instead of one each takes a call of 1024x1024x1024 from 41.9 to 28.2 us, of 200x700x512 from 24.4 to 16.8,
-// of 1009x2752x1024 from 55.0 to 51.4 (in graphs).  Either way the workspace's copies are padded with zeros
+// of 1009x2752x1024 from 55.0 to 51.4 (in graphs; fp16's pass for the largest value is not in these).  Either way the workspace's copies are padded with zeros
 // to the kernels' 64 values of the sum, which is what lets T and F be anything.
 //
 // The pass that makes dG and dU rounds them to the operands' 16 bits, half a step each: what the matrix instructions take.
@@ -16,7 +16,7 @@
 // rows: dW sums over both (X stands twice), dX is the sum of two rows of its product.  That is so for up to 2^15 values (of
 // products of three normal values as many as some hundred alike), where it is the launch that adds the rows that takes
 // time: 1x100x512 bf16 8.3 -> 10.2 us, 300x100x512 10.9 -> 14.5, 1x8192x4096 77.8 -> 79.5.
-// The pass is bound by memory, 3 T F values read and 2 T F written (131 us at 8192x8192).
+// The pass is bound by memory, 3 T F values read and 2 T F written (126 us at 8192x8192).
 //
 // fp16 has five bits of exponent: dG and dU of a loss that is a mean over many tokens lie below its normal values, those of
 // one that is scaled up may lie above its largest, where the results, sums with other factors, are in range.  They are
