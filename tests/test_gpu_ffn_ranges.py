@@ -172,3 +172,12 @@ def test_fp16_gradients_captured_and_replayed_on_dh_of_other_sizes(T, F):
         assert bool(torch.isfinite(got[0]).all()) == math.isfinite(size) and not bool((got[0] == 7.0).any())
     del graph
     d.close()
+
+
+def test_fp16_gradients_without_rows(tiled):
+    F, D = 100, 128
+    n = tiled.glu_backward_workspace(0, F, D)
+    ws = torch.full((n,), 0xFF, dtype=torch.uint8, device="cuda")
+    dwg, dwu = (torch.full((F, D), 3.0, dtype=torch.float16, device="cuda") for _ in range(2))
+    tiled.glu_backward(capi.TYPE_F16, capi.GLU_GELU, None, F, None, D, None, None, D, None, None, F, None, D, dwg, dwu, D, 0, F, D, ws, n)
+    assert bool((dwg == 0).all()) and bool((dwu == 0).all())
