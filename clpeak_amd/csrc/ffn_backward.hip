@@ -6,8 +6,8 @@
 // and dU writes them both ways and X and the weights are turned once into the workspace.  Which of these goes by the
 // expected times: turning costs the products of a training batch (8192x8192x4096) 106 of 1585 us; one launch for all
 // three products instead of one each takes a call of 1024x1024x1024 from 41.9 to 28.2 us, of 200x700x512 from 24.4 to 16.8,
-// of 1009x2752x1024 from 55.0 to 51.4 (in graphs; fp16's pass for the largest value is not in these).  Either way the workspace's copies are padded with zeros
-// to the kernels' 64 values of the sum, which is what lets T and F be anything.
+// of 1009x2752x1024 from 55.0 to 51.4 (in graphs; fp16's pass for the largest value is not in these).  Either way the
+// workspace's copies are padded with zeros to the kernels' 64 values of the sum, which is what lets T and F be anything.
 //
 // The pass that makes dG and dU rounds them to the operands' 16 bits, half a step each: what the matrix instructions take.
 // Beside the rounding of the results it is the only one, and where there are many values their errors, independent and
@@ -40,7 +40,8 @@ constexpr uint32_t kLargest = 1024;   // workgroups that look for the largest va
 
 // The workspace: dG | dU by rows [Tp][2 Fk]; by columns 2 x [Fp][Tp] where dW wants that; the weights turned [D][2 Fk], or
 // their last rows 2 x [64][D]; X turned [D][Tp], or its last rows [64][D] (where it stands twice, all of it [Tp][D]); and
-// what the products use of it where they are cut along their sums; of fp16 the workgroups' largest values and the factor that undoes the scaling.
+// what the products use of it where they are cut along their sums; of fp16 the workgroups' largest values and the factor
+// that undoes the scaling.
 struct Plan {
   bool twice;                                  // a value is two rows
   uint32_t rows_of;                            // T or 2 T
